@@ -45,6 +45,11 @@ class State(C.Structure):
                                    "status")]
 
 
+class Cache(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n_groups", "n_heads", "head_dim", "n_blocks")] + \
+               [(n, _fp) for n in ("codes", "scales", "bounds", "lens")]
+
+
 _LIB: Optional[C.CDLL] = None
 LIB_PATH = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "libartab_b200.so")
 
@@ -69,6 +74,11 @@ _SIGNATURES = {
     "artab_hybrid_attention": (_i, [_i, _p, _p, _p, _p, _p, _p, C.POINTER(C.c_int64), _i, _i, _i, _i, _i, _i, _p, _p,
                                     C.c_int64, _p, _p]),
     "artab_kv_append": (_i, [_i, _p, _p, _p, _i, _i, _i, _i, _i, _p]),
+    "artab_cache_write": (_i, [_i, _p, _p, _p, _p, _i, _p, _p, _i, _p, _p]),
+    "artab_cache_read": (_i, [_i, _p, _p, _i, _p, _p, _p]),
+    "artab_cache_attention": (_i, [_i, _p, _p, _i, _i, _p, _i, C.c_float, _p, _p, _p]),
+    "artab_cache_select": (_i, [_i, _p, _p, _i, _i, _p, _i, _i, _p, _p]),
+    "artab_cache_block_attention": (_i, [_i, _p, _p, _i, _i, _p, _p, _i, C.c_float, _p, _p, _p]),
     "artab_embed": (_i, [C.POINTER(Model), _p, _p, _p, _i, _i, _i, _p, _p]),
     "artab_head_logpdf": (_i, [C.POINTER(Model), _p, _p, _i, _p, _p]),
     "artab_head_sample": (_i, [C.POINTER(Model), _p, _p, _p, _i, _p, _p, _p, _p]),

@@ -1,0 +1,119 @@
+// The 8-bit context cache: layout, argument records and the fragment helpers its kernels share.
+//
+// Keys and values are kept in blocks of 64 rows.  A (group, head, block) has one record of 128 * Dh code bytes (the
+// keys row by row, then the values transposed), two scales, and the smallest / largest key code per channel.
+// A code c stands for (c - 128) * scale.  Codes are unsigned because a byte then becomes a half-precision number in
+// one permute and one subtraction (0x6400 | byte is 1024 + byte), exactly; whole numbers up to 127 are exact in
+// half precision, so products with them cost no accuracy beyond the other operand's.
+//
+// Order inside a record, chosen so that every thread of a warp reads its mma.m16n8k16 fragments as one contiguous
+// piece (g = lane / 4, t = lane % 4):
+//   keys     [64][Dh]; the four k indices of thread t in k step s are channels t * Dh/4 + 4 s + {0,1,2,3}, so the
+//            thread reads Dh/4 bytes of a row at once
+//   values   [Dh][64]; place 16 t + 4 s + 2 h + e of a channel holds row 16 s + 8 h + 2 t + e, so the thread reads the 16
+//            bytes of its four k steps at once
+#pragma once
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace artab {
+
+constexpr int kCacheBlock = 64;
+
+__host__ __device__ constexpr int cache_value_place(int row) {  // place of a block's row in a value channel
+  return 16 * ((row >> 1) & 3) + 4 * (row >> 4) + 2 * ((row >> 3) & 1) + (row & 1);
+}
+
+// Rows of a [.., .., rows, Dh] tensor by strides (in elements) of its three leading axes.
+struct RowView {
+  const void* p;
+  long s0, s1, s2;
+};
+
+// ---- fragments -------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+// two neighbouring code bytes -> two halves (byte - 128); `high`: bytes 2, 3 of the word instead of 0, 1
+__device__ __forceinline__ uint32_t codes_to_halves(uint32_t w, bool high) {
+  const uint32_t x = __byte_perm(w, 0x64646464u, high ? 0x4342u : 0x4140u);  // 1024 + byte
+  const uint32_t off = 0x64806480u;                                         // 1152
+  return h2_bits(__hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&off)));
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {  // 8 x 8 halves over the warp, two per thread
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ void cache_cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cache_cp8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Power of two that brings a row with largest magnitude `top` into [1, 2), and its inverse.  Queries go to the
+// tensor cores as one or two half-precision parts (11 bits each) of the scaled row: what falls below the range of
+// halves is then less than 2^-24 of the row's largest element.  Both are normal numbers for every finite row.
+__device__ __forceinline__ void row_scale(float top, float& to, float& back) {
+  int e = (int)((__float_as_uint(top) >> 23) & 255u);
+  e = e < 1 ? 1 : e > 253 ? 253 : e;
+  to = __uint_as_float((uint32_t)(254 - e) << 23);
+  back = __uint_as_float((uint32_t)e << 23);
+}
+
+// NN consecutive elements of a query row as floats; `vec`: the row is aligned to the 16 (8, 4) bytes read at a time
+template <typename T, int NN>
+__device__ __forceinline__ void load_elements(const T* p, bool vec, float (&x)[NN]) {
+  constexpr int kBytes = NN * (int)sizeof(T);
+  if (vec) {
+    constexpr int kUnit = kBytes >= 16 ? 16 : 8;
+    constexpr int kPer = kUnit / (int)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < NN / kPer; ++i) {
+      uint32_t w[4];
+      if constexpr (kUnit == 16) {
+        const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+      } else {
+        const uint2 v = reinterpret_cast<const uint2*>(p)[i];
+        w[0] = v.x, w[1] = v.y;
+      }
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        if constexpr (sizeof(T) == 4)
+          x[i * kPer + j] = __uint_as_float(w[j]);
+        else
+          x[i * kPer + j] = __uint_as_float((j & 1) ? (w[j >> 1] & 0xffff0000u) : (w[j >> 1] << 16));
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NN; ++i) x[i] = to_f32<T>(p[i]);
+  }
+}
+
+// A cache and query tensor that fit each other: checked by every entry point that takes queries.
+int check_cache(const artab_cache* c, const char* what);
+int check_queries(int dtype, const void* q, const int64_t* strides, int n_streams, int n_q, const artab_cache* c,
+                  const char* what);
+// every strided row starts on a 16-byte (fp32, bf16 with at least eight elements per thread) boundary
+inline bool rows_aligned(const RowView& v, int elem) {
+  return ((reinterpret_cast<uintptr_t>(v.p) | (uintptr_t)(v.s0 * elem) | (uintptr_t)(v.s1 * elem) | (uintptr_t)(v.s2 * elem)) & 15) == 0;
+}
+
+}  // namespace artab

@@ -359,6 +359,61 @@ ARTAB_API int artab_hybrid_attention(int dtype, const void* q, const void* k_ctx
 ARTAB_API int artab_kv_append(int dtype, void* kv_buf, const void* k_new, const void* v_new, int n_streams, int n_heads,
                     int head_dim, int max_buf, int pos, void* stream);
 
+/* ------------------------- 8-bit context cache ---------------------------- */
+/* Context keys and values in blocks of 64 rows, eight bits a number.  (No counterpart in the reference: its caches
+ * hold the projected type.)  Of every (group, head, block):
+ *   codes   2 * 64 * Dh bytes: keys [64][Dh], then values transposed, [Dh][64] with place 16t + 4s + 2h + e of a channel
+ *           holding row 16s + 8h + 2t + e; a byte c stands for (c - 128) * scale;
+ *   scales  largest magnitude / 127, of the keys and of the values (NaN once a value that is not finite came in);
+ *   bounds  half precision: smallest key code (less 128) of every channel over the rows in use, then the largest.
+ * G = 1: one context for every stream; else one per stream.  lens[g] rows are in use, the first ones; kernels read it
+ * on the device.  head_dim 16, 32 or 64.  codes and bounds are 16-byte aligned. */
+typedef struct artab_cache {
+  int32_t n_groups;   /* G */
+  int32_t n_heads;    /* H */
+  int32_t head_dim;   /* Dh */
+  int32_t n_blocks;   /* capacity of a group, in blocks */
+  uint8_t* codes;     /* [G][H][n_blocks][2][64 * Dh] */
+  float* scales;      /* [G][H][n_blocks][2] */
+  void* bounds;       /* [G][H][n_blocks][2][Dh] half */
+  int32_t* lens;      /* [G] */
+} artab_cache;
+
+/* Rows into the cache.  k, v [G][H][n_rows][Dh] of `dtype`, by HOST arrays of three strides (elements; group, head,
+ * row).  Group g takes its first counts[g] rows (NULL: n_rows; clamped to [0, n_rows]) and keeps them as rows
+ * start[g] .. (NULL: lens[g] ..) of the context; what lay at or behind start[g] is dropped and lens[g] becomes
+ * start[g] + counts[g].  Rows beyond the capacity are left out.  start / counts may be lens itself, not
+ * overlap it otherwise.  A block's scale is the larger of the one it had (where rows before start[g] are kept) and that
+ * of the new rows; kept rows are rounded again to it.
+ * fresh != 0: the whole cache is laid out (unused blocks get zero scales and bounds), start must be NULL and means 0. */
+ARTAB_API int artab_cache_write(int dtype, const void* k, const int64_t* k_strides, const void* v,
+                                const int64_t* v_strides, int n_rows, const int32_t* start, const int32_t* counts,
+                                int fresh, artab_cache* c, void* stream);
+
+/* Rows start[g] .. start[g] + n_rows - 1 (NULL: from row 0) of every group as k, v [G][H][n_rows][Dh] of `dtype`,
+ * contiguous; rows that are not in use read as zero. */
+ARTAB_API int artab_cache_read(int dtype, const artab_cache* c, const int32_t* start, int n_rows, void* k, void* v,
+                               void* stream);
+
+/* Attention of q [B][H][Lq][Dh] (HOST array of three strides: stream, head, query) over the rows in use:
+ * out [B][H][Lq][Dh] of `dtype`, lse [B][H][Lq] (natural log).  A context of no rows gives 0 and -inf.
+ * max_len: a bound of lens known to the host, for the choice of launch only (results do not depend on its truth). */
+ARTAB_API int artab_cache_attention(int dtype, const void* q, const int64_t* q_strides, int n_streams, int n_q,
+                                    const artab_cache* c, int max_len, float scale, void* out, float* lse,
+                                    void* stream);
+
+/* For every query the n_pick blocks with the largest upper bound of a score, index [B][H][Lq][n_pick] int32 in
+ * ascending order, -1 behind them where a context has fewer blocks.  The bound is formed with the query rounded to
+ * whole numbers (largest magnitude 127), exactly; equal bounds go to the lower index.  At most 221184 rows of capacity. */
+ARTAB_API int artab_cache_select(int dtype, const void* q, const int64_t* q_strides, int n_streams, int n_q,
+                                 const artab_cache* c, int max_len, int n_pick, int32_t* index, void* stream);
+
+/* artab_cache_attention over the rows of the blocks that blocks [B][H][Lq][n_list] int32 lists for every query: an index
+ * that is no block in use counts for nothing, one that is listed twice counts twice. */
+ARTAB_API int artab_cache_block_attention(int dtype, const void* q, const int64_t* q_strides, int n_streams, int n_q,
+                                          const artab_cache* c, const int32_t* blocks, int n_list, float scale,
+                                          void* out, float* lse, void* stream);
+
 /* Embedder: out[r][:] = mean_F(x[r][:]) * wx + bx (+ y[r] * wy + by) + marker[kind] (+ ar_tokens[ar_idx[r]]).
  *   x [rows][F], y [rows] or NULL, ar_idx [rows] or NULL.
  * Replaces Embedder.embed_context / embed_buffer / embed_target (ar_tabpfn/model/model.py:51-76). */

@@ -1,0 +1,203 @@
+"""Arguments of the 8-bit context cache, checked before anything reaches the device: the native entry points see
+addresses only.  Also the host's side of lengths and capacities.  Runs without a GPU."""
+import pytest
+import torch
+
+from ar_tabpfn import _lib
+from ar_tabpfn.model import context_cache as cc
+
+G, H, D, N = 3, 2, 32, 100
+
+
+class FakeLibrary:
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name, args))
+            return 0
+        return call
+
+
+@pytest.fixture
+def fake(monkeypatch):
+    """Calls are recorded, and host tensors pass for device tensors."""
+    lib = FakeLibrary()
+
+    class Launch:
+        def __init__(self, device):
+            pass
+
+        def __enter__(self):
+            return lib, None
+
+        def __exit__(self, *exc):
+            return False
+    monkeypatch.setattr(cc, "_Launch", Launch)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    return lib
+
+
+def tensors(blocks=2, g=G, h=H, d=D):
+    return dict(codes=torch.zeros(g, h, blocks, 2, 64 * d, dtype=torch.uint8), scales=torch.zeros(g, h, blocks, 2),
+                bounds=torch.zeros(g, h, blocks, 2, d, dtype=torch.float16), lens=torch.zeros(g, dtype=torch.int32))
+
+
+def cache(**kw):
+    return cc.ContextCache(**tensors(**kw))
+
+
+@pytest.mark.parametrize("change", [
+    dict(codes=torch.zeros(G, H, 2, 2, 64 * D)), dict(codes=torch.zeros(G, H, 2, 64 * D, dtype=torch.uint8)),
+    dict(codes=torch.zeros(G, H, 2, 2, 64 * D + 1, dtype=torch.uint8)), dict(codes=torch.zeros(G, H, 2, 2, 64 * 48, dtype=torch.uint8)),
+    dict(codes=torch.zeros(G, H, 2, 1, 64 * D, dtype=torch.uint8)), dict(codes=torch.zeros(G, H, 0, 2, 64 * D, dtype=torch.uint8)),
+    dict(codes=torch.zeros(H, G, 2, 2, 64 * D, dtype=torch.uint8).transpose(0, 1)), dict(scales=torch.zeros(G, H, 3, 2)),
+    dict(scales=torch.zeros(G, H, 2, 2, dtype=torch.float16)), dict(bounds=torch.zeros(G, H, 2, 2, D)),
+    dict(bounds=torch.zeros(G, H, 2, D, dtype=torch.float16)), dict(lens=torch.zeros(G, dtype=torch.int64)),
+    dict(lens=torch.zeros(G + 1, dtype=torch.int32)), dict(lens=torch.zeros(2 * G, dtype=torch.int32)[::2]),
+], ids=lambda c: next(f"{k}{tuple(v.shape)}{v.dtype}" for k, v in c.items()))
+def test_tensors_that_are_no_cache(change):
+    cache()
+    with pytest.raises(ValueError, match="ContextCache"):
+        cc.ContextCache(**(tensors() | change))
+
+
+@pytest.mark.parametrize("k,v,kw", [
+    ((H, N, D), (H, N + 1, D), {}), ((N, D), (N, D), {}), ((H, N, 24), (H, N, 24), {}), ((H, N, 128), (H, N, 128), {}),
+    ((G, H, N, D), (H, N, D), {}), ((H, N, D), (H, N, D), dict(capacity=N - 1)), ((H, 0, D), (H, 0, D), {}),
+    ((0, H, N, D), (0, H, N, D), {}), ((G, H, N, D), (G, H, N, D), dict(lens=[N] * (G + 1))),
+    ((G, H, N, D), (G, H, N, D), dict(lens=torch.ones(G))), ((G, H, N, D), (G, H, N, D), dict(lens=torch.ones(1, G, dtype=torch.int32))),
+], ids=str)
+def test_contexts_that_do_not_fit(fake, k, v, kw):
+    with pytest.raises(ValueError):
+        cc.quantize_context(torch.zeros(k), torch.zeros(v), **kw)
+    assert not fake.calls
+
+
+def test_types(fake):
+    x = torch.zeros(H, N, D)
+    for k, v in ((x, x.bfloat16()), (x.half(), x.half()), (x.double(), x.double()), (x.int(), x.int())):
+        with pytest.raises(ValueError):
+            cc.quantize_context(k, v)
+    with pytest.raises(ValueError):
+        cc.read_context(cache(), dtype=torch.float16)
+    for op in (lambda q: cc.context_cache_attention(q, cache()), lambda q: cc.select_context_blocks(q, cache(), 1)):
+        with pytest.raises(ValueError):
+            op(torch.zeros(G, H, 1, D).half())
+    assert not fake.calls
+
+
+@pytest.mark.parametrize("q", [(G, H, D), (G, H + 1, 1, D), (G, H, 1, 16), (G + 1, H, 1, D), (1, H, 1, D)], ids=str)
+def test_queries_that_do_not_fit(fake, q):
+    q = torch.zeros(q)
+    blocks = torch.zeros(*q.shape[:3], 2, dtype=torch.int32) if q.dim() == 4 else torch.zeros(1, dtype=torch.int32)
+    for op in (lambda: cc.context_cache_attention(q, cache()), lambda: cc.select_context_blocks(q, cache(), 3),
+               lambda: cc.block_context_attention(q, cache(), blocks)):
+        with pytest.raises(ValueError):
+            op()
+    assert not fake.calls
+
+
+def test_blocks_that_do_not_fit(fake):
+    q = torch.zeros(G, H, 2, D)
+    for blocks in (torch.zeros(G, H, 2, 3), torch.zeros(G, H, 2, 3, dtype=torch.int64), torch.zeros(G, H, 1, 3, dtype=torch.int32),
+                   torch.zeros(G, H, 2, dtype=torch.int32), torch.zeros(1, H, 2, 3, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="blocks"):
+            cc.block_context_attention(q, cache(), blocks)
+    for n in (0, -1):
+        with pytest.raises(ValueError):
+            cc.select_context_blocks(q, cache(), n)
+    with pytest.raises(ValueError):
+        cc.read_context(cache(), n=-1)
+    assert not fake.calls
+
+
+@pytest.mark.parametrize("shape", [(H, 1, D), (G, H, 1, 16), (G, H + 1, 1, D), (G + 1, H, 1, D)], ids=str)
+def test_rows_that_do_not_fit_a_cache(fake, shape):
+    with pytest.raises(ValueError):
+        cc.append_context(cache(), torch.zeros(shape), torch.zeros(shape))
+    x = torch.zeros(G, H, 1, D)
+    for kw in (dict(counts=[1, 1]), dict(start=torch.zeros(G)), dict(start=torch.zeros(G, dtype=torch.bool))):
+        with pytest.raises(ValueError):
+            cc.append_context(cache(), x, x, **kw)
+    assert not fake.calls
+
+
+def test_room_is_counted_before_rows_are_written(fake, monkeypatch):
+    c = cc.ContextCache(**tensors(), length=100)
+    x = torch.zeros(G, H, 20, D)
+    c.lens.fill_(100)
+    cc.append_context(c, x, x)                              # the fake leaves lens as it is
+    assert c.length == 120 and len(fake.calls) == 1
+    c.lens.fill_(120)
+    with pytest.raises(ValueError, match="capacity"):
+        cc.append_context(c, x, x)
+    with pytest.raises(ValueError, match="capacity"):
+        cc.append_context(c, x, x, counts=[0, 0, 9])
+    cc.append_context(c, x, x, counts=[0, 8, 8])
+    cc.append_context(c, x, x, start=[0, 0, 0])
+    cc.append_context(c, x[:, :, :0], x[:, :, :0])          # nothing to do
+    assert len(fake.calls) == 3
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(ValueError, match="capture"):
+        cc.append_context(c, x, x)
+    assert len(fake.calls) == 3
+
+
+def test_views_are_passed_by_their_strides(fake):
+    x = torch.zeros(N, 3, H, D)
+    k, v = x[:, 0].transpose(0, 1), x[:, 1].transpose(0, 1)
+    cc.quantize_context(k, v)
+    args = fake.calls[-1][1]
+    assert args[1] == k.data_ptr() and list(args[2])[1:] == [D, 3 * H * D] and args[3] == v.data_ptr()
+    q = torch.zeros(G, 2, H, D).transpose(1, 2)
+    cc.context_cache_attention(q, cache())
+    assert fake.calls[-1][1][1] == q.data_ptr() and list(fake.calls[-1][1][2]) == list(q.stride()[:3])
+
+
+def test_no_device_no_result():
+    if torch.cuda.is_available():
+        x = torch.zeros(H, N, D)
+        with pytest.raises(ValueError, match="CUDA"):
+            cc.quantize_context(x, x)
+    else:
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            cc.quantize_context(torch.zeros(H, N, D), torch.zeros(H, N, D))
+
+
+def test_the_library_refuses_what_does_not_fit_without_a_device():
+    """The C entry points: codes, never exceptions or aborts."""
+    import ctypes as C
+    lib = _lib.load_library()
+    p = 4096
+    st = (C.c_int64 * 3)(1, 1, 1)
+    good = lambda **kw: _lib.Cache(**(dict(n_groups=2, n_heads=2, head_dim=32, n_blocks=2, codes=p, scales=p, bounds=p, lens=p) | kw))
+    bad = [good(n_groups=0), good(n_groups=70000), good(n_heads=0), good(head_dim=48), good(n_blocks=0), good(n_blocks=1 << 25),
+           good(codes=None), good(scales=None), good(bounds=None), good(lens=None), good(codes=p + 8), good(bounds=p + 2), good(scales=p + 4)]
+    for c in bad:
+        r = C.byref(c)
+        assert lib.artab_cache_write(0, p, st, p, st, 4, None, None, 1, r, None) == -1
+        assert lib.artab_cache_read(0, r, None, 4, p, p, None) == -1
+        assert lib.artab_cache_attention(0, p, st, 2, 1, r, 0, 1.0, p, p, None) == -1
+        assert lib.artab_cache_select(0, p, st, 2, 1, r, 0, 1, p, None) == -1
+        assert lib.artab_cache_block_attention(0, p, st, 2, 1, r, p, 1, 1.0, p, p, None) == -1
+    r = C.byref(good())
+    assert lib.artab_cache_write(7, p, st, p, st, 4, None, None, 1, r, None) == -1
+    assert lib.artab_cache_write(0, None, st, p, st, 4, None, None, 1, r, None) == -1
+    assert lib.artab_cache_write(0, p, st, p, st, 0, None, None, 1, r, None) == -1
+    assert lib.artab_cache_write(0, p, st, p, st, 129, None, None, 1, r, None) == -2
+    assert lib.artab_cache_write(0, p, st, p, st, 4, p, None, 1, r, None) == -1
+    assert lib.artab_cache_write(0, p, st, p, st, 4, p + 4, None, 0, r, None) == -1       # start inside lens
+    assert lib.artab_cache_write(0, p, st, p, st, 4, None, p + 4, 0, r, None) == -1
+    assert lib.artab_cache_read(0, r, None, 0, p, p, None) == -1
+    assert lib.artab_cache_read(0, r, None, 1, p + 4, p, None) == -1
+    assert lib.artab_cache_attention(3, p, st, 2, 1, r, 0, 1.0, p, p, None) == -1
+    assert lib.artab_cache_attention(0, p, st, 3, 1, r, 0, 1.0, p, p, None) == -1
+    assert lib.artab_cache_attention(0, p, st, 2, 0, r, 0, 1.0, p, p, None) == -1
+    assert lib.artab_cache_attention(0, p, st, 2, 1, r, 0, 1.0, None, p, None) == -1
+    assert lib.artab_cache_select(0, p, st, 2, 1, r, 0, 0, p, None) == -1
+    assert lib.artab_cache_select(0, p, st, 2, 1, C.byref(good(n_blocks=3457)), 0, 1, p, None) == -1
+    assert lib.artab_cache_block_attention(0, p, st, 2, 1, r, None, 1, 1.0, p, p, None) == -1
+    assert lib.artab_cache_block_attention(0, p, st, 2, 1, r, p, 0, 1.0, p, p, None) == -1
+    assert b"cache" in lib.artab_last_error()
