@@ -50,14 +50,15 @@ class ContextCache:
     __slots__ = ("codes", "scales", "bounds", "lens", "length", "n_groups", "n_heads", "head_dim", "capacity", "_c", "_ref")
 
     def __init__(self, codes: Tensor, scales: Tensor, bounds: Tensor, lens: Tensor, length: Optional[int] = None):
-        if codes.dim() != 5 or codes.shape[3] != 2 or codes.dtype is not torch.uint8:
+        shape = codes.shape
+        if len(shape) != 5 or shape[3] != 2 or codes.dtype is not torch.uint8:
             raise ValueError("ContextCache: codes must be uint8 [G,H,blocks,2,64*Dh]")
-        G, H, blocks, _, size = codes.shape
+        G, H, blocks, _, size = shape
         Dh = size // CONTEXT_BLOCK
         if Dh not in (16, 32, 64) or size % CONTEXT_BLOCK:
             raise ValueError(f"ContextCache: head size {size / CONTEXT_BLOCK:g} not supported (16, 32, 64)")
         if G < 1 or H < 1 or blocks < 1:
-            raise ValueError(f"ContextCache: empty cache {tuple(codes.shape)}")
+            raise ValueError(f"ContextCache: empty cache {tuple(shape)}")
         if scales.shape != (G, H, blocks, 2) or scales.dtype is not torch.float32:
             raise ValueError("ContextCache: scales must be float32 [G,H,blocks,2]")
         if bounds.shape != (G, H, blocks, 2, Dh) or bounds.dtype is not torch.float16:
@@ -66,8 +67,7 @@ class ContextCache:
             raise ValueError("ContextCache: lens must be int32 [G]")
         if not (codes.is_contiguous() and scales.is_contiguous() and bounds.is_contiguous() and lens.is_contiguous()):
             raise ValueError("ContextCache: tensors must be contiguous")
-        device = codes.get_device()
-        if not scales.get_device() == bounds.get_device() == lens.get_device() == device:
+        if not scales.get_device() == bounds.get_device() == lens.get_device() == codes.get_device():
             raise ValueError("ContextCache: all tensors must live on one device")
         self.codes, self.scales, self.bounds, self.lens = codes, scales, bounds, lens
         self.n_groups, self.n_heads, self.head_dim, self.capacity = G, H, Dh, blocks * CONTEXT_BLOCK
@@ -79,32 +79,29 @@ class ContextCache:
     def device(self) -> torch.device:
         return self.codes.device
 
-    @property
-    def dtype(self) -> torch.dtype:
-        return torch.uint8
-
 
 # row of a block at each place of a value channel
 VALUE_ROWS = tuple(16 * s + 8 * h + 2 * t + e for t in range(4) for s in range(4) for h in range(2) for e in range(2))
 
 
 class _Launch:
-    """The library and the stream of ``device``, which is the current one inside (a launch goes to the current one)."""
+    """The library and the current stream of the device with number ``device``, which is the current device inside (a
+    launch goes to the current one)."""
 
     __slots__ = ("device", "outer")
 
-    def __init__(self, device: torch.device):
+    def __init__(self, device: int):
         self.device = device
 
     def __enter__(self):
         lib = _lib.lib()
-        if self.device.type != "cuda":
+        if self.device < 0:
             raise ValueError("context cache: tensors must live on a CUDA device")
         self.outer = None
-        if torch.cuda.current_device() != self.device.index:
+        if _current_device() != self.device:
             self.outer = torch.cuda.device(self.device)
             self.outer.__enter__()
-        return lib, _lib.stream_ptr()
+        return lib, _raw_stream(self.device)
 
     def __exit__(self, *exc):
         if self.outer is not None:
@@ -112,8 +109,23 @@ class _Launch:
         return False
 
 
-def _strided(t: Tensor) -> Tensor:
-    return t if t.stride(-1) == 1 else t.contiguous()
+def _current_device() -> int:
+    return torch._C._cuda_getDevice()      # torch.cuda.current_device() without its check that CUDA is up
+
+
+def _raw_stream(device: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(device)   # the address alone, no Stream object
+
+
+def _strided(t: Tensor):
+    """``t`` with neighbouring elements in its last axis, its address and its other strides (None: contiguous)."""
+    if t.is_contiguous():
+        return t, t.data_ptr(), None
+    strides = t.stride()
+    if strides[-1] != 1:
+        t = t.contiguous()
+        return t, t.data_ptr(), None
+    return t, t.data_ptr(), _Strides(*strides[:3])
 
 
 def _lengths(x: Optional[Lengths], G: int, device: torch.device, what: str) -> Optional[Tensor]:
@@ -131,17 +143,29 @@ def _lengths(x: Optional[Lengths], G: int, device: torch.device, what: str) -> O
     return x
 
 
-def _rows_of(k: Tensor, v: Tensor, what: str) -> Tuple[Tensor, Tensor]:
+def _rows_of(k: Tensor, v: Tensor, what: str) -> Tuple[Tensor, Tensor, int]:
+    """Keys and values as [G,H,N,Dh], and the code of their type."""
     if k.dim() == 3:
         k, v = k.unsqueeze(0), v.unsqueeze(0)
     if k.dim() != 4 or v.shape != k.shape:
         raise ValueError(f"{what}: keys {tuple(k.shape)} and values {tuple(v.shape)} must both be [H,N,Dh] or [G,H,N,Dh]")
     if v.dtype is not k.dtype:
         raise ValueError(f"{what}: keys are {k.dtype}, values {v.dtype}")
-    _lib.dtype_code(k.dtype)
+    code = _lib.dtype_code(k.dtype)
     if v.get_device() != k.get_device():
         raise ValueError(f"{what}: keys and values must live on one device")
-    return _strided(k), _strided(v)
+    return k, v, code
+
+
+def _write(lib, stream, cache: ContextCache, code: int, k: Tensor, v: Tensor, start, counts, fresh: int) -> None:
+    k, k_at, k_strides = _strided(k)
+    v, v_at, v_strides = _strided(v)
+    _lib.check(lib.artab_cache_write(code, k_at, k_strides, v_at, v_strides, k.shape[2], _address(start), _address(counts),
+                                     fresh, cache._ref, stream))
+
+
+def _address(t: Optional[Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 def quantize_context(k_ctx: Tensor, v_ctx: Tensor, lens: Optional[Lengths] = None,
@@ -149,7 +173,7 @@ def quantize_context(k_ctx: Tensor, v_ctx: Tensor, lens: Optional[Lengths] = Non
     """A cache of the context rows k_ctx / v_ctx, [H,Nc,Dh] (shared by all streams) or [G,H,Nc,Dh] (one context per
     stream).  ``lens`` [G]: rows in use of each (default: all Nc; the others are not read).  ``capacity``: rows that
     there is room for (rounded up to whole blocks; default Nc)."""
-    k, v = _rows_of(k_ctx, v_ctx, "quantize_context")
+    k, v, code = _rows_of(k_ctx, v_ctx, "quantize_context")
     G, H, N, Dh = k.shape
     if Dh not in (16, 32, 64):
         raise ValueError(f"quantize_context: head_dim {Dh} not supported (16, 32, 64)")
@@ -158,16 +182,13 @@ def quantize_context(k_ctx: Tensor, v_ctx: Tensor, lens: Optional[Lengths] = Non
         raise ValueError(f"quantize_context: no room for {N} rows of {G} x {H} heads in a capacity of {capacity}")
     counts = _lengths(lens, G, k.device, "lens")
     blocks = (capacity + CONTEXT_BLOCK - 1) // CONTEXT_BLOCK
-    with _Launch(k.device) as (lib, stream):
-        new = lambda make, dtype, *shape: make(shape, dtype=dtype, device=k.device)
-        make = torch.zeros if N == 0 else torch.empty      # without rows nothing is launched
-        cache = ContextCache(new(torch.empty, torch.uint8, G, H, blocks, 2, CONTEXT_BLOCK * Dh),
-                             new(make, torch.float32, G, H, blocks, 2), new(make, torch.float16, G, H, blocks, 2, Dh),
-                             new(make, torch.int32, G), N)
+    with _Launch(k.get_device()) as (lib, stream):
+        new = k.new_zeros if N == 0 else k.new_empty      # without rows nothing is launched
+        cache = ContextCache(k.new_empty((G, H, blocks, 2, CONTEXT_BLOCK * Dh), dtype=torch.uint8),
+                             new((G, H, blocks, 2), dtype=torch.float32), new((G, H, blocks, 2, Dh), dtype=torch.float16),
+                             new((G,), dtype=torch.int32), N)
         if N:
-            _lib.check(lib.artab_cache_write(_lib.dtype_code(k.dtype), k.data_ptr(), _Strides(*k.stride()[:3]),
-                                             v.data_ptr(), _Strides(*v.stride()[:3]), N, None, _lib.ptr(counts), 1,
-                                             cache._ref, stream))
+            _write(lib, stream, cache, code, k, v, None, counts, 1)
     return cache
 
 
@@ -179,7 +200,7 @@ def append_context(cache: ContextCache, k_new: Tensor, v_new: Tensor, counts: Op
     (default: ``cache.lens``); what was at or behind it is dropped, which takes rows back that did not stand.  ``lens``
     becomes start + counts.  ``start`` is at most ``lens``, and rows beyond the capacity are left out; without
     ``start`` they raise before anything is written."""
-    k, v = _rows_of(k_new, v_new, "append_context")
+    k, v, code = _rows_of(k_new, v_new, "append_context")
     G, H, n, Dh = k.shape
     if (G, H, Dh) != (cache.n_groups, cache.n_heads, cache.head_dim):
         raise ValueError(f"append_context: rows {tuple(k.shape)} do not fit a cache of {cache.n_groups} contexts, "
@@ -190,7 +211,7 @@ def append_context(cache: ContextCache, k_new: Tensor, v_new: Tensor, counts: Op
     start = _lengths(start, G, k.device, "start")
     if n == 0 and start is None:
         return
-    with _Launch(k.device) as (lib, stream):
+    with _Launch(k.get_device()) as (lib, stream):
         if start is None and cache.length + n > cache.capacity:
             # the bound that the host keeps may be too high: contexts that took fewer rows, a cache put together from tensors
             if torch.cuda.is_current_stream_capturing():
@@ -202,9 +223,7 @@ def append_context(cache: ContextCache, k_new: Tensor, v_new: Tensor, counts: Op
         if n == 0:
             k = v = cache.scales.new_empty(G, H, 1, Dh)      # nothing is read from it: start alone takes effect
             counts = torch.zeros(G, dtype=torch.int32, device=k.device)
-        _lib.check(lib.artab_cache_write(_lib.dtype_code(k.dtype), k.data_ptr(), _Strides(*k.stride()[:3]), v.data_ptr(),
-                                         _Strides(*v.stride()[:3]), max(n, 1), _lib.ptr(start), _lib.ptr(counts), 0,
-                                         cache._ref, stream))
+        _write(lib, stream, cache, code, k, v, start, counts, 0)
     cache.length = min(cache.length + n, cache.capacity)
 
 
@@ -218,42 +237,39 @@ def read_context(cache: ContextCache, start: Optional[Lengths] = None, n: Option
     if n < 0:
         raise ValueError(f"read_context: {n} rows")
     start = _lengths(start, G, cache.device, "start")
-    k = torch.empty(G, H, n, Dh, dtype=dtype, device=cache.device)
+    k = cache.scales.new_empty((G, H, n, Dh), dtype=dtype)
     v = torch.empty_like(k)
     if n:
-        with _Launch(cache.device) as (lib, stream):
-            _lib.check(lib.artab_cache_read(code, cache._ref, _lib.ptr(start), n, k.data_ptr(), v.data_ptr(), stream))
+        with _Launch(k.get_device()) as (lib, stream):
+            _lib.check(lib.artab_cache_read(code, cache._ref, _address(start), n, k.data_ptr(), v.data_ptr(), stream))
     return k, v
 
 
-def _queries(q: Tensor, cache: ContextCache, what: str) -> Tensor:
-    if q.dim() != 4 or q.shape[1] != cache.n_heads or q.shape[3] != cache.head_dim:
-        raise ValueError(f"{what}: queries {tuple(q.shape)} do not fit a cache of {cache.n_heads} heads of size "
+def _queries(q: Tensor, cache: ContextCache, what: str):
+    """Sizes [B,H,Lq,Dh], type and device of queries that fit the cache."""
+    shape = q.shape
+    if len(shape) != 4 or shape[1] != cache.n_heads or shape[3] != cache.head_dim:
+        raise ValueError(f"{what}: queries {tuple(shape)} do not fit a cache of {cache.n_heads} heads of size "
                          f"{cache.head_dim}")
-    if cache.n_groups not in (1, q.shape[0]):
-        raise ValueError(f"{what}: {cache.n_groups} contexts for {q.shape[0]} streams (one, or one each)")
-    _lib.dtype_code(q.dtype)
-    if q.get_device() != cache.codes.get_device():
+    if cache.n_groups != 1 and cache.n_groups != shape[0]:
+        raise ValueError(f"{what}: {cache.n_groups} contexts for {shape[0]} streams (one, or one each)")
+    code, device = _lib.dtype_code(q.dtype), q.get_device()
+    if device != cache.codes.get_device():
         raise ValueError(f"{what}: queries must live on the device of the cache")
-    return _strided(q)
-
-
-def _outputs(q: Tensor) -> Tuple[Tensor, Tensor]:
-    return (torch.empty(q.shape, dtype=q.dtype, device=q.device),
-            torch.empty(q.shape[:3], dtype=torch.float32, device=q.device))
+    return shape, code, device
 
 
 def context_cache_attention(q: Tensor, cache: ContextCache, scale: Optional[float] = None) -> Tuple[Tensor, Tensor]:
     """Attention of q [B,H,Lq,Dh] over every row in use of its context: out [B,H,Lq,Dh] (q dtype), lse [B,H,Lq] fp32
     (natural log), as ``triton_context_attention``.  A context without rows gives 0 and -inf."""
-    q = _queries(q, cache, "context_cache_attention")
-    B, _, Lq, Dh = q.shape
-    out, lse = _outputs(q)
+    (B, H, Lq, Dh), code, device = _queries(q, cache, "context_cache_attention")
+    out, lse = q.new_empty((B, H, Lq, Dh)), q.new_empty((B, H, Lq), dtype=torch.float32)
     if B and Lq:
-        with _Launch(q.device) as (lib, stream):
-            _lib.check(lib.artab_cache_attention(_lib.dtype_code(q.dtype), q.data_ptr(), _Strides(*q.stride()[:3]), B, Lq,
-                                                 cache._ref, cache.length, Dh ** -0.5 if scale is None else float(scale),
-                                                 out.data_ptr(), lse.data_ptr(), stream))
+        q, at, strides = _strided(q)
+        with _Launch(device) as (lib, stream):
+            _lib.check(lib.artab_cache_attention(code, at, strides, B, Lq, cache._ref, cache.length,
+                                                 Dh ** -0.5 if scale is None else float(scale), out.data_ptr(),
+                                                 lse.data_ptr(), stream))
     return out, lse
 
 
@@ -264,16 +280,16 @@ def select_context_blocks(q: Tensor, cache: ContextCache, n_blocks: int) -> Tens
     The bound of a block is sum_d max(q_d lo_d, q_d hi_d) over the extreme keys of its channels, with the query rounded
     to whole numbers (largest magnitude 127): whole-number arithmetic, so the choice is reproducible to the bit; equal
     bounds go to the lower index.  A query that is not finite gets the first blocks."""
-    q = _queries(q, cache, "select_context_blocks")
-    B, H, Lq, _ = q.shape
+    (B, H, Lq, _), code, device = _queries(q, cache, "select_context_blocks")
     n = int(n_blocks)
     if n < 1:
         raise ValueError(f"select_context_blocks: {n} blocks")
-    index = torch.empty(B, H, Lq, n, dtype=torch.int32, device=q.device)
+    index = q.new_empty((B, H, Lq, n), dtype=torch.int32)
     if B and Lq:
-        with _Launch(q.device) as (lib, stream):
-            _lib.check(lib.artab_cache_select(_lib.dtype_code(q.dtype), q.data_ptr(), _Strides(*q.stride()[:3]), B, Lq,
-                                              cache._ref, cache.length, n, index.data_ptr(), stream))
+        q, at, strides = _strided(q)
+        with _Launch(device) as (lib, stream):
+            _lib.check(lib.artab_cache_select(code, at, strides, B, Lq, cache._ref, cache.length, n, index.data_ptr(),
+                                              stream))
     return index
 
 
@@ -282,20 +298,20 @@ def block_context_attention(q: Tensor, cache: ContextCache, blocks: Tensor,
     """``context_cache_attention`` over the rows of the listed blocks only: blocks int32 [B,H,Lq,S], as
     ``select_context_blocks`` gives them.  An index that is no block in use counts for nothing, one listed twice counts
     twice, a query whose list holds no block gets 0 and -inf."""
-    q = _queries(q, cache, "block_context_attention")
-    B, H, Lq, Dh = q.shape
-    if blocks.dim() != 4 or blocks.shape[:3] != (B, H, Lq) or blocks.dtype is not torch.int32:
+    (B, H, Lq, Dh), code, device = _queries(q, cache, "block_context_attention")
+    shape = blocks.shape
+    if len(shape) != 4 or shape[:3] != (B, H, Lq) or blocks.dtype is not torch.int32:
         raise ValueError(f"block_context_attention: blocks must be int32 [{B},{H},{Lq},S]")
-    if blocks.get_device() != q.get_device():
+    if blocks.get_device() != device:
         raise ValueError("block_context_attention: blocks must live on the device of the queries")
-    out, lse = _outputs(q)
-    if blocks.shape[3] == 0:
+    out, lse = q.new_empty((B, H, Lq, Dh)), q.new_empty((B, H, Lq), dtype=torch.float32)
+    if shape[3] == 0:
         return out.zero_(), lse.fill_(float("-inf"))
-    blocks = blocks.contiguous()
     if B and Lq:
-        with _Launch(q.device) as (lib, stream):
-            _lib.check(lib.artab_cache_block_attention(_lib.dtype_code(q.dtype), q.data_ptr(), _Strides(*q.stride()[:3]),
-                                                       B, Lq, cache._ref, blocks.data_ptr(), blocks.shape[3],
+        blocks = blocks.contiguous()
+        q, at, strides = _strided(q)
+        with _Launch(device) as (lib, stream):
+            _lib.check(lib.artab_cache_block_attention(code, at, strides, B, Lq, cache._ref, blocks.data_ptr(), shape[3],
                                                        Dh ** -0.5 if scale is None else float(scale), out.data_ptr(),
                                                        lse.data_ptr(), stream))
     return out, lse

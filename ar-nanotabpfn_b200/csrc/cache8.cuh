@@ -21,15 +21,81 @@ namespace artab {
 
 constexpr int kCacheBlock = 64;
 
-__host__ __device__ constexpr int cache_value_place(int row) {  // place of a block's row in a value channel
-  return 16 * ((row >> 1) & 3) + 4 * (row >> 4) + 2 * ((row >> 3) & 1) + (row & 1);
-}
-
 // Rows of a [.., .., rows, Dh] tensor by strides (in elements) of its three leading axes.
 struct RowView {
   const void* p;
   long s0, s1, s2;
 };
+
+// strides as the entry points take them: null for a contiguous tensor
+inline RowView row_view(const void* p, const int64_t* strides, int n1, int n2, int dh) {
+  if (!strides) return {p, (long)n1 * n2 * dh, (long)n2 * dh, (long)dh};
+  return {p, (long)strides[0], (long)strides[1], (long)strides[2]};
+}
+
+// ---- whole numbers nearest to a quotient ------------------------------------------------------------------
+// The nearest whole number to x / scale in exact arithmetic, ties to even.  A first value c comes from one fused product
+// with the reciprocal, rounded by adding 1.5 * 2^23 (the low byte of the sum is then the code).  Next to a tie it may be
+// off by one, and ties are not rare (rows of eight-bit numbers such as bf16 meet one in some 200): the rest x - c * scale,
+// one fused operation that is exact next to a tie, is compared with half the scale.  Steps near the smallest normal
+// number, and kept rows next to a tie (whose x is a product itself), go through 64 bits.
+constexpr float kRound = 12582912.0f + 128.0f;   // 1.5 * 2^23, and the 128 that is added to a code
+
+__device__ __forceinline__ uint32_t low_bytes(const uint32_t (&w)[4]) {
+  return __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
+}
+// bytes of a word as numbers less 128
+__device__ __forceinline__ void code_values(uint32_t w, float (&x)[4]) {
+  const uint32_t u[4] = {__byte_perm(w, 0x4b000000u, 0x7440), __byte_perm(w, 0x4b000000u, 0x7441),
+                         __byte_perm(w, 0x4b000000u, 0x7442), __byte_perm(w, 0x4b000000u, 0x7443)};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] = __uint_as_float(u[j]) - 8388736.0f;
+}
+static __device__ __noinline__ uint32_t exact_codes(float x0, float x1, float x2, float x3, float was, float scale) {
+  const float x[4] = {x0, x1, x2, x3};
+  uint32_t w = 0;
+  for (int j = 0; j < 4; ++j) {
+    const double c = rint((double)x[j] * (double)was / (double)scale);
+    w |= (uint32_t)(128 + (int)fmin(fmax(c, -127.0), 127.0)) << (8 * j);
+  }
+  return w;
+}
+// Four codes of x at a step of `scale` (> 0)
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[4], float scale, float inv) {
+  uint32_t w[4];
+  float rest[4];
+  const float half = 0.5f * scale;
+  bool sure = scale > 2e-38f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float r = fmaf(x[j], inv, kRound);
+    rest[j] = fmaf(kRound - r, scale, x[j]);
+    sure = sure && fabsf(rest[j]) < half;             // false for what is not finite, too
+    w[j] = __float_as_uint(r);
+  }
+  if (!sure) {
+    if (scale <= 2e-38f) return exact_codes(x[0], x[1], x[2], x[3], 1.0f, scale);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool off = fabsf(rest[j]) > half || (fabsf(rest[j]) == half && (w[j] & 1u));
+      w[j] += off ? (rest[j] > 0.0f ? 1u : 0xffffffffu) : 0u;
+    }
+  }
+  return low_bytes(w);
+}
+// Four codes of x * was (whole numbers x at an older step `was`) at a step of `scale`.  The first quotient is off by less
+// than 3e-5: closer than 5e-5 to a tie it is formed again.
+__device__ __forceinline__ uint32_t kept_codes(const float (&x)[4], float was, float scale, float inv) {
+  uint32_t w[4];
+  bool sure = scale > 2e-38f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float y = x[j] * was, r = fmaf(y, inv, kRound);
+    sure = sure && fabsf(fmaf(y, inv, kRound - r)) <= 0.49995f;
+    w[j] = __float_as_uint(r);
+  }
+  return sure ? low_bytes(w) : exact_codes(x[0], x[1], x[2], x[3], was, scale);
+}
 
 // ---- fragments -------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
@@ -109,8 +175,7 @@ __device__ __forceinline__ void load_elements(const T* p, bool vec, float (&x)[N
 
 // A cache and query tensor that fit each other: checked by every entry point that takes queries.
 int check_cache(const artab_cache* c, const char* what);
-int check_queries(int dtype, const void* q, const int64_t* strides, int n_streams, int n_q, const artab_cache* c,
-                  const char* what);
+int check_queries(int dtype, const void* q, int n_streams, int n_q, const artab_cache* c, const char* what);
 // every strided row starts on a 16-byte (fp32, bf16 with at least eight elements per thread) boundary
 inline bool rows_aligned(const RowView& v, int elem) {
   return ((reinterpret_cast<uintptr_t>(v.p) | (uintptr_t)(v.s0 * elem) | (uintptr_t)(v.s1 * elem) | (uintptr_t)(v.s2 * elem)) & 15) == 0;

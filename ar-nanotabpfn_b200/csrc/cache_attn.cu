@@ -13,34 +13,17 @@
 // walks blocks of its own with a running maximum; its ring of records is filled by 16-byte asynchronous copies
 // and no warp waits for another until the end, where the warps of a CTA and the CTAs of a cluster (up to eight
 // share the rows of a context) merge maximum, sum and output through shared memory.
-#include <math_constants.h>
-
-#include "cache8.cuh"
-#include "cluster.cuh"
+#include "cache_attn.cuh"
 
 namespace artab {
 namespace {
 
 constexpr int kWarps = 8;
 
-struct AttnArgs {
-  artab_cache c;
-  RowView q;
-  int n_streams, n_q;
-  int rows;               // query rows of a group
-  int tiles;              // tiles of a group's rows
-  long units;             // (group, head, tile) or (stream, head, query)
-  int splits;             // CTAs of a cluster
-  const int32_t* list;    // [B][H][Lq][n_list], or null: every block
-  int n_list;
-  float scale_log2;       // scale * log2 e
-  int vec_q;
-  void* out;              // [B][H][Lq][Dh]
-  float* lse;             // [B][H][Lq]
-};
-
 // numerators are 2^14 times exp(s - max): halves keep 11 bits of them down to 2^-28 of the largest
 constexpr float kLift = 14.0f;
+// query rows of a group from which the row tiles are taken (fp32: half as many)
+constexpr int kManyRows = 96;
 
 template <int DH, int PARTS>
 struct Tile {
@@ -207,7 +190,11 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const AttnArgs 
   extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int rank = (int)(blockIdx.x % a.splits);
-  const long unit = blockIdx.x / a.splits;
+  const int per_cta = LIST ? a.per_cta : 1, warps = kWarps / per_cta;
+  long unit = blockIdx.x / a.splits;
+  if (LIST) unit = unit * per_cta + warp / warps;
+  const bool spare = LIST && unit >= a.units;                 // the last CTA may have warps without a unit
+  if (spare) unit = a.units - 1;
   const int H = a.c.n_heads;
   int group, h, row0, n_rows;
   if (LIST) {
@@ -230,7 +217,7 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const AttnArgs 
   const int cap = a.c.n_blocks * kCacheBlock;
   len = len < 0 ? 0 : len > cap ? cap : len;
   const int held = (len + kCacheBlock - 1) / kCacheBlock;
-  const int n = LIST ? a.n_list : held;                      // blocks of the unit
+  const int n = spare ? 0 : LIST ? a.n_list : held;           // blocks of the unit
   const int32_t* list = LIST ? a.list + unit * a.n_list : nullptr;
   const size_t gh = (size_t)group * H + h;
   const uint8_t* codes = a.c.codes + gh * a.c.n_blocks * (size_t)R::kRecord;
@@ -238,11 +225,17 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const AttnArgs 
 
   uint8_t* ring = smem + warp * R::kBytes;
   const uint32_t ring_addr = smem_u32(ring);
-  const int first = rank * kWarps + warp, step = a.splits * kWarps;
-  const auto block_of = [&](int i) {                          // -1: nothing there
-    if (i >= n) return -1;
-    if (!LIST) return i;
-    const int b = list[i];
+  const int first = rank * warps + warp % warps, step = a.splits * warps;
+  // block to fetch next; -1: nothing there.  Of a list, the lanes keep 32 entries of the warp's share
+  int fetched = 0, entries = -1;
+  const auto next_block = [&]() {
+    const int k = fetched++, i = first + k * step;
+    if (!LIST) return i < n ? i : -1;
+    if (k % 32 == 0) {
+      const int mine = i + lane * step;
+      entries = mine < n ? list[mine] : -1;
+    }
+    const int b = __shfl_sync(0xffffffffu, entries, k % 32);
     return b < 0 || b >= held ? -1 : b;
   };
   const auto fetch = [&](int blk, int stage) {
@@ -258,7 +251,7 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const AttnArgs 
   int ahead[R::kStages - 1];
 #pragma unroll
   for (int i = 0; i < R::kStages - 1; ++i) {
-    ahead[i] = block_of(first + i * step);
+    ahead[i] = next_block();
     fetch(ahead[i], i);
   }
   Tl tile;
@@ -271,7 +264,7 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const AttnArgs 
   }
   int stage = 0;
   for (int i = first; i < n; i += step) {
-    const int next = block_of(i + (R::kStages - 1) * step);
+    const int next = next_block();
     fetch(next, stage == 0 ? R::kStages - 1 : stage - 1);
     cp_wait<R::kStages - 1>();
     __syncwarp();
@@ -309,8 +302,7 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const AttnArgs 
   }
   __syncthreads();
   float* mine = part + kWarps * ROWS * P;
-  const auto merge = [&](auto at, int count, int e, float& m, float& l, float& o) {
-    const int row = e / DH, d = e % DH;
+  const auto merge = [&](auto at, int count, int row, int d, float& m, float& l, float& o) {
     m = -CUDART_INF_F;
     for (int w = 0; w < count; ++w) m = fmaxf(m, at(w, row * P + DH));
     const float base = m == -CUDART_INF_F ? 0.0f : m;
@@ -321,74 +313,377 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const AttnArgs 
       o = fmaf(at(w, row * P + d), x, o);
     }
   };
-  const auto store = [&](int e, float m, float l, float o) {
-    const int row = row0 + e / DH, d = e % DH;
-    if (row >= n_rows) return;
+  const auto store = [&](int r, int d, float m, float l, float o) {
+    const int row = row0 + r;
+    if (row >= n_rows || spare) return;
     const size_t at = ((size_t)stream_of(row) * H + h) * a.n_q + query_of(row);
     reinterpret_cast<T*>(a.out)[at * DH + d] = from_f32<T>(l == 0.0f ? 0.0f : o / l);
     if (d == 0) a.lse[at] = l == 0.0f ? -CUDART_INF_F : (m - kLift) * kLn2 + logf(l);
   };
-  for (int e = tid; e < ROWS * DH; e += kWarps * 32) {
+  // the threads of a unit's warps write its results
+  const float* of_unit = part + (LIST ? warp / warps * warps : 0) * ROWS * P;
+  for (int e = LIST ? tid % (warps * 32) : tid; e < ROWS * DH; e += warps * 32) {
     float m, l, o;
-    merge([&](int w, int i) { return part[w * ROWS * P + i]; }, kWarps, e, m, l, o);
+    merge([&](int w, int i) { return of_unit[w * ROWS * P + i]; }, warps, e / DH, e % DH, m, l, o);
     if (a.splits == 1) {
-      store(e, m, l, o);
+      store(e / DH, e % DH, m, l, o);
     } else {
       mine[e / DH * P + e % DH] = o;
       if (e % DH == 0) mine[e / DH * P + DH] = m, mine[e / DH * P + DH + 1] = l;
     }
   }
   if (a.splits == 1) return;
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_meet();
   const uint32_t base = smem_u32(mine);
   for (int e = rank * kWarps * 32 + tid; e < ROWS * DH; e += a.splits * kWarps * 32) {
     float m, l, o;
     merge([&](int w, int i) {
-      float v;
-      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_rank(base + i * 4, w)) : "memory");
-      return v;
-    }, a.splits, e, m, l, o);
-    store(e, m, l, o);
+      return ld_cluster(base + i * 4, w);
+    }, a.splits, e / DH, e % DH, m, l, o);
+    store(e / DH, e % DH, m, l, o);
   }
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_meet();
+}
+
+// ---- many rows on one context ------------------------------------------------------------------------------
+// cache_attn_rows_kernel: the queries are the 16-row operand.  A CTA of four warps owns 64 rows a part (PARTS = 1: 128
+// rows; PARTS = 2: 64, part p of query g of a tile in row g + 8 p) and walks the blocks of its share together: each
+// warp turns a quarter of a block's codes into half-precision fragments in shared memory, in the order in which a
+// lane reads them with 16-byte loads, while the block before is worked on; the numerators go from the accumulators
+// of one product straight into the operand registers of the next.  The value scale of a block is folded into the
+// exponent, relative to the largest of the context, so that one accumulator serves all blocks.
+template <int DH, int PARTS>
+struct RowTile {
+  static constexpr int MT = 2, NW = 4;
+  static constexpr int ROWS = NW * MT * 16 / PARTS;
+  static constexpr int kBlockBytes = 2 * kCacheBlock * DH * 2;      // keys and values as halves
+  static constexpr int kSmem = 2 * kBlockBytes > ROWS * (DH + 2) * 4 ? 2 * kBlockBytes : ROWS * (DH + 2) * 4;
+};
+template <typename T, int DH, int PARTS>
+__global__ void __launch_bounds__(128, DH == 64 ? 2 : 3) cache_attn_rows_kernel(const AttnArgs a) {
+  using RT = RowTile<DH, PARTS>;
+  constexpr int MT = RT::MT, NW = RT::NW, KS = DH / 16, ND = DH / 8, P = DH + 2, R = 3 - PARTS;
+  constexpr int KN = 8 / NW, VN = ND > NW ? ND / NW : 1;         // key and value tiles that a warp lays out
+  constexpr int KQ = KS >= 2 ? KS / 2 : 1;                       // 16-byte pieces of a lane's key fragments
+  constexpr size_t kRecord = 2 * kCacheBlock * DH;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float s_max[NW];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int rank = (int)(blockIdx.x % a.splits);
+  const long unit = blockIdx.x / a.splits;
+  const int H = a.c.n_heads, row0 = (int)(unit % a.tiles) * RT::ROWS, h = (int)(unit / a.tiles % H);
+  const int group = (int)(unit / a.tiles / H);
+  const bool one = a.c.n_groups == 1;
+  const auto stream_of = [&](int row) { return one ? row / a.n_q : group; };
+  const auto query_of = [&](int row) { return one ? row % a.n_q : row; };
+  int len = a.c.lens[group];
+  const int cap = a.c.n_blocks * kCacheBlock;
+  len = len < 0 ? 0 : len > cap ? cap : len;
+  const int held = (len + kCacheBlock - 1) / kCacheBlock;
+  const size_t gh = (size_t)group * H + h;
+  const uint8_t* codes = a.c.codes + gh * a.c.n_blocks * kRecord;
+  const float2* scales = reinterpret_cast<const float2*>(a.c.scales) + gh * a.c.n_blocks;
+
+  uint32_t rk[KN][KS];
+  uint4 rv[VN];
+  const auto load = [&](int blk) {                                // raw codes of this warp's tiles
+    const uint8_t* rec = codes + (size_t)blk * kRecord;
+#pragma unroll
+    for (int i = 0; i < KN; ++i) {
+      const uint8_t* p = rec + (8 * (warp + i * NW) + g) * DH + t * (DH / 4);
+      if constexpr (KS == 1) rk[i][0] = *reinterpret_cast<const uint32_t*>(p);
+      if constexpr (KS == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        rk[i][0] = v.x, rk[i][1] = v.y;
+      }
+      if constexpr (KS == 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        rk[i][0] = v.x, rk[i][1] = v.y, rk[i][2] = v.z, rk[i][3] = v.w;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VN; ++i)
+      if (ND >= NW || warp < ND)
+        rv[i] = *reinterpret_cast<const uint4*>(rec + kCacheBlock * DH + (8 * (warp + i * NW) + g) * kCacheBlock + 16 * t);
+  };
+  const auto lay_out = [&](uint8_t* to) {
+#pragma unroll
+    for (int i = 0; i < KN; ++i) {
+      const int j = warp + i * NW;
+      if constexpr (KS == 1) {
+        reinterpret_cast<uint2*>(to)[j * 32 + lane] = make_uint2(codes_to_halves(rk[i][0], false), codes_to_halves(rk[i][0], true));
+      } else {
+#pragma unroll
+        for (int q = 0; q < KQ; ++q)
+          reinterpret_cast<uint4*>(to)[(j * KQ + q) * 32 + lane] =
+              make_uint4(codes_to_halves(rk[i][2 * q], false), codes_to_halves(rk[i][2 * q], true),
+                         codes_to_halves(rk[i][2 * q + 1], false), codes_to_halves(rk[i][2 * q + 1], true));
+      }
+    }
+    uint4* v = reinterpret_cast<uint4*>(to + 2 * kCacheBlock * DH);
+#pragma unroll
+    for (int i = 0; i < VN; ++i)
+      if (ND >= NW || warp < ND) {
+        const int j = warp + i * NW;
+        v[(j * 2 + 0) * 32 + lane] = make_uint4(codes_to_halves(rv[i].x, false), codes_to_halves(rv[i].x, true),
+                                                codes_to_halves(rv[i].y, false), codes_to_halves(rv[i].y, true));
+        v[(j * 2 + 1) * 32 + lane] = make_uint4(codes_to_halves(rv[i].z, false), codes_to_halves(rv[i].z, true),
+                                                codes_to_halves(rv[i].w, false), codes_to_halves(rv[i].w, true));
+      }
+  };
+  if (rank < held) load(rank);
+
+  // largest value scale of the context (a NaN among them shows in its own block)
+  float vmax = 0.0f;
+  for (int i = tid; i < held; i += 32 * NW) vmax = fmaxf(vmax, scales[i].y);
+  vmax = warp_max(vmax);
+  if (lane == 0) s_max[warp] = vmax;
+
+  // queries: fragments a0 .. a3 of every k step
+  uint32_t q[MT][KS][4];
+  float f[MT][R];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      constexpr int NE = DH / 4;
+      const int row = row0 + (warp * MT + mt) * (16 / PARTS) + g + 8 * r;
+      float x[NE];
+#pragma unroll
+      for (int i = 0; i < NE; ++i) x[i] = 0.0f;
+      if (row < a.rows)
+        load_elements<T, NE>(reinterpret_cast<const T*>(a.q.p) + stream_of(row) * a.q.s0 + h * a.q.s1 +
+                                 query_of(row) * a.q.s2 + t * NE, a.vec_q, x);
+      float top = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NE; ++i) top = fmaxf(top, fabsf(x[i]));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      float to, back;
+      row_scale(top, to, back);
+      f[mt][r] = back * fabsf(a.scale_log2);
+      to = copysignf(to, a.scale_log2);
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float u = x[4 * s + 2 * j] * to, w = x[4 * s + 2 * j + 1] * to;
+          const __half2 hi = __floats2half2_rn(u, w);
+          q[mt][s][2 * j + r] = h2_bits(hi);
+          if constexpr (PARTS == 2)
+            q[mt][s][2 * j + 1] = h2_bits(__floats2half2_rn(u - __low2float(hi), w - __high2float(hi)));
+        }
+    }
+  float m[MT][R], l[MT][R], o[MT][ND][4];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) m[mt][r] = -CUDART_INF_F, l[mt][r] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < ND; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[mt][j][e] = 0.0f;
+  }
+  if (rank < held) {
+    lay_out(smem);
+    if (rank + a.splits < held) load(rank + a.splits);
+  }
+  __syncthreads();
+  vmax = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+  float poison = 0.0f;
+
+  int buf = 0;
+  for (int blk = rank; blk < held; blk += a.splits) {
+    const float2 sc = scales[blk];
+    const uint8_t* kv = smem + buf * RT::kBlockBytes;
+    const int live = len - blk * kCacheBlock;
+    // value scale: a factor of the numerators (in the exponent) and, back, of their sum
+    float ratio = vmax > 0.0f ? sc.y / vmax : 0.0f;
+    if (ratio != ratio) poison = sc.y, ratio = 1.0f;   // a block with values that are not finite: the weights are sound
+    ratio = fmaxf(ratio, kLeastRatio);
+    const float lift = kLift + __log2f(ratio), unlift = 1.0f / ratio;
+    float c[MT][8][4];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      uint32_t b[KS][2];
+      if constexpr (KS == 1) {
+        const uint2 v = reinterpret_cast<const uint2*>(kv)[j * 32 + lane];
+        b[0][0] = v.x, b[0][1] = v.y;
+      } else {
+#pragma unroll
+        for (int i = 0; i < KQ; ++i) {
+          const uint4 v = reinterpret_cast<const uint4*>(kv)[(j * KQ + i) * 32 + lane];
+          b[2 * i][0] = v.x, b[2 * i][1] = v.y, b[2 * i + 1][0] = v.z, b[2 * i + 1][1] = v.w;
+        }
+      }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[mt][j][e] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) mma_f16(c[mt][j], q[mt][s][0], q[mt][s][1], q[mt][s][2], q[mt][s][3], b[s][0], b[s][1]);
+      }
+    }
+    uint32_t p[MT][4][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      if constexpr (PARTS == 2)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) c[mt][j][0] += c[mt][j][2], c[mt][j][1] += c[mt][j][3];
+      if (live < kCacheBlock)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 2 * R; ++e)
+            if (8 * j + 2 * t + (e & 1) >= live) c[mt][j][e] = -CUDART_INF_F;
+      float alpha[R], sl[R], add[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float mx = c[mt][0][2 * r];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fmaxf(c[mt][j][2 * r], c[mt][j][2 * r + 1]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float x = f[mt][r] * sc.x;
+        sl[r] = !(x <= 1e-37f) ? x : 1e-37f;      // never 0 (a masked score stays -inf), NaN as it is
+        mx = fmaxf(m[mt][r], mx * sl[r]);
+        const float base = mx == -CUDART_INF_F ? 0.0f : mx;
+        alpha[r] = ex2(m[mt][r] - base);
+        m[mt][r] = mx;
+        add[r] = lift - base;
+      }
+      bool moved = alpha[0] != 1.0f;
+      if (R == 2) moved |= alpha[R - 1] != 1.0f;
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int j = 0; j < ND; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[mt][j][e] *= alpha[PARTS == 2 ? 0 : e >> 1];
+      }
+      float sum[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) sum[r] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float x = ex2(fmaf(c[mt][j][2 * r], sl[r], add[r])), y = ex2(fmaf(c[mt][j][2 * r + 1], sl[r], add[r]));
+          sum[r] += x + y;
+          const __half2 hi = __floats2half2_rn(x, y);
+          p[mt][j >> 1][2 * (j & 1) + r] = h2_bits(hi);
+          if constexpr (PARTS == 2)
+            p[mt][j >> 1][2 * (j & 1) + 1] = h2_bits(__floats2half2_rn(x - __low2float(hi), y - __high2float(hi)));
+        }
+#pragma unroll
+      for (int r = 0; r < R; ++r) l[mt][r] = fmaf(l[mt][r], alpha[r], sum[r] * unlift);
+    }
+    const uint4* v = reinterpret_cast<const uint4*>(kv + 2 * kCacheBlock * DH);
+#pragma unroll
+    for (int j = 0; j < ND; ++j) {
+      const uint4 b0 = v[(j * 2 + 0) * 32 + lane], b1 = v[(j * 2 + 1) * 32 + lane];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        mma_f16(o[mt][j], p[mt][0][0], p[mt][0][1], p[mt][0][2], p[mt][0][3], b0.x, b0.y);
+        mma_f16(o[mt][j], p[mt][1][0], p[mt][1][1], p[mt][1][2], p[mt][1][3], b0.z, b0.w);
+        mma_f16(o[mt][j], p[mt][2][0], p[mt][2][1], p[mt][2][2], p[mt][2][3], b1.x, b1.y);
+        mma_f16(o[mt][j], p[mt][3][0], p[mt][3][1], p[mt][3][2], p[mt][3][3], b1.z, b1.w);
+      }
+    }
+    buf ^= 1;
+    if (blk + a.splits < held) {
+      lay_out(smem + buf * RT::kBlockBytes);      // the buffer of the block before this one: all warps are past it
+      if (blk + 2 * a.splits < held) load(blk + 2 * a.splits);
+    }
+    __syncthreads();
+  }
+
+  float* part = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int row = (warp * MT + mt) * (16 / PARTS) + g + 8 * r;
+      float s = l[mt][r];
+      s += __shfl_xor_sync(0xffffffffu, s, 1);
+      s += __shfl_xor_sync(0xffffffffu, s, 2);
+#pragma unroll
+      for (int j = 0; j < ND; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          part[row * P + 8 * j + 2 * t + e] = (PARTS == 2 ? o[mt][j][e] + o[mt][j][2 + e] : o[mt][j][2 * r + e]) * vmax + poison;
+      if (t == 0) part[row * P + DH] = m[mt][r], part[row * P + DH + 1] = s;
+    }
+  if (a.splits == 1)
+    __syncthreads();
+  else
+    cluster_meet();
+  const uint32_t base = smem_u32(part);
+  const auto at = [&](int w, int i) { return a.splits == 1 ? part[i] : ld_cluster(base + i * 4, w); };
+  merge_rows<T, DH>(a, at, a.splits, rank * 32 * NW + tid, a.splits * 32 * NW, RT::ROWS, row0, h, group, kLift);
+  if (a.splits > 1) cluster_meet();
 }
 
 template <typename T, int DH, int PARTS, bool LIST>
 int launch(const AttnArgs& a, cudaStream_t s) {
   static SmemConfig config;
-  const auto kernel = cache_attn_kernel<T, DH, PARTS, LIST>;
   const size_t part = (size_t)(kWarps + 1) * partial_floats<DH, PARTS>() * sizeof(float);
   const size_t ring = (size_t)kWarps * Ring<DH>::kBytes;
-  const size_t smem = part > ring ? part : ring;
-  cudaError_t e = config.ensure(kernel, smem, true);
-  ARTAB_REQUIRE(e == cudaSuccess, ARTAB_ELAUNCH, "cache_attention: %s", cudaGetErrorString(e));
-  ARTAB_REQUIRE(a.units * a.splits <= 0x7fffffffL, ARTAB_EINVAL, "cache_attention: too many query rows");
-  PlainLaunchScope plain;
-  count_launch();
-  e = launch_dependent_cluster(kernel, dim3((unsigned)(a.units * a.splits)), dim3(kWarps * 32), smem, s,
-                               (unsigned)a.splits, a);
-  ARTAB_REQUIRE(e == cudaSuccess, ARTAB_ELAUNCH, "cache_attention: %s", cudaGetErrorString(e));
-  return ARTAB_OK;
+  return launch_attn(cache_attn_kernel<T, DH, PARTS, LIST>, config, part > ring ? part : ring, kWarps * 32, a, s);
 }
-
-template <typename T, int DH>
-int by_form(AttnArgs& a, cudaStream_t s) {
-  if (a.list) return launch<T, DH, 2, true>(a, s);
-  if (sizeof(T) == 2 && a.rows > 4) {
-    a.tiles = (a.rows + 7) / 8;
-    a.units *= a.tiles;
-    return launch<T, DH, 1, false>(a, s);
-  }
-  a.tiles = (a.rows + 3) / 4;
-  a.units *= a.tiles;
-  return launch<T, DH, 2, false>(a, s);
+template <typename T, int DH, int PARTS>
+int launch_rows(const AttnArgs& a, cudaStream_t s) {
+  static SmemConfig config;
+  return launch_attn(cache_attn_rows_kernel<T, DH, PARTS>, config, RowTile<DH, PARTS>::kSmem, RowTile<DH, PARTS>::NW * 32, a, s);
 }
 
 // CTAs that share the blocks of a unit: as many as fill the GPU twice, none without a block for every warp
 int plan_splits(long units, long blocks) {
   int s = 1;
-  while (s < 8 && units * s * 2 <= 2 * 148 && blocks >= 2L * s * kWarps) s *= 2;
+  while (s < 8 && units * s * 2 <= 2 * kSms && blocks >= 2L * s * kWarps) s *= 2;
   return s;
+}
+// the same for the row tiles: the share of the last wave that is idle, and four blocks' worth of work around each share
+int plan_row_splits(long units, long blocks, int per_sm) {
+  int best = 1;
+  double least = 0.0;
+  for (int s = 1; s <= 8; s *= 2) {
+    const double waves = (double)((units * s + (long)kSms * per_sm - 1) / ((long)kSms * per_sm));
+    const double cost = waves * ((double)((blocks + s - 1) / s) + 4.0);
+    if (s == 1 || cost < least) best = s, least = cost;
+  }
+  return best;
+}
+
+template <typename T, int DH>
+int by_form(AttnArgs& a, long blocks, cudaStream_t s) {
+  constexpr int kParts = sizeof(T) == 2 ? 1 : 2;
+  const auto tiles = [&a](int rows) { a.tiles = (a.rows + rows - 1) / rows, a.units *= a.tiles; };
+  if (a.list) {
+    // as many warps share a list as leave each two blocks, fewer where the lists alone fill the GPU
+    int warps = kWarps;
+    while (warps > 1 && (2 * warps > a.n_list || a.units * warps > 8L * kWarps * kSms)) warps /= 2;
+    a.per_cta = kWarps / warps;
+    if (warps == kWarps) a.splits = plan_splits(a.units, blocks);
+    return launch<T, DH, 2, true>(a, s);
+  }
+  if (kParts == 1 && a.rows >= kManyRows) {
+    tiles(128);
+    a.splits = plan_row_splits(a.units, blocks, 2);
+    return launch_cache_attn_tc(a, s);
+  }
+  if (a.rows >= kManyRows / kParts) {
+    tiles(RowTile<DH, kParts>::ROWS);
+    a.splits = plan_row_splits(a.units, blocks, DH == 64 ? 2 : 3);
+    return launch_rows<T, DH, kParts>(a, s);
+  }
+  if (kParts == 1 && a.rows > 4) {
+    tiles(8);
+    a.splits = plan_splits(a.units, blocks);
+    return launch<T, DH, kParts, false>(a, s);
+  }
+  tiles(4);
+  a.splits = plan_splits(a.units, blocks);
+  return launch<T, DH, 2, false>(a, s);
 }
 
 int attention(int dtype, const void* q, const int64_t* strides, int n_streams, int n_q, const artab_cache* c,
@@ -396,12 +691,12 @@ int attention(int dtype, const void* q, const int64_t* strides, int n_streams, i
               const char* what) {
   int rc = check_cache(c, what);
   if (rc) return rc;
-  rc = check_queries(dtype, q, strides, n_streams, n_q, c, what);
+  rc = check_queries(dtype, q, n_streams, n_q, c, what);
   if (rc) return rc;
   ARTAB_REQUIRE(out && lse, ARTAB_EINVAL, "%s: null pointer", what);
   AttnArgs a;
   a.c = *c;
-  a.q = {q, (long)strides[0], (long)strides[1], (long)strides[2]};
+  a.q = row_view(q, strides, c->n_heads, n_q, c->head_dim);
   a.n_streams = n_streams;
   a.n_q = n_q;
   a.rows = c->n_groups == 1 ? n_streams * n_q : n_q;
@@ -414,24 +709,23 @@ int attention(int dtype, const void* q, const int64_t* strides, int n_streams, i
   a.lse = lse;
   a.units = list ? (long)n_streams * c->n_heads * n_q : (long)c->n_groups * c->n_heads;
   const long blocks = list ? n_list : (max_len + kCacheBlock - 1L) / kCacheBlock;
-  const int per = list ? 1 : dtype == ARTAB_BF16 && a.rows > 4 ? 8 : 4;
-  a.splits = plan_splits(list ? a.units : a.units * ((a.rows + per - 1) / per), blocks);
+  a.splits = 1;
+  a.per_cta = 1;
   if (dtype == ARTAB_F32) {
-    if (c->head_dim == 16) return by_form<float, 16>(a, s);
-    if (c->head_dim == 32) return by_form<float, 32>(a, s);
-    return by_form<float, 64>(a, s);
+    if (c->head_dim == 16) return by_form<float, 16>(a, blocks, s);
+    if (c->head_dim == 32) return by_form<float, 32>(a, blocks, s);
+    return by_form<float, 64>(a, blocks, s);
   }
-  if (c->head_dim == 16) return by_form<__nv_bfloat16, 16>(a, s);
-  if (c->head_dim == 32) return by_form<__nv_bfloat16, 32>(a, s);
-  return by_form<__nv_bfloat16, 64>(a, s);
+  if (c->head_dim == 16) return by_form<__nv_bfloat16, 16>(a, blocks, s);
+  if (c->head_dim == 32) return by_form<__nv_bfloat16, 32>(a, blocks, s);
+  return by_form<__nv_bfloat16, 64>(a, blocks, s);
 }
 
 }  // namespace
 
-int check_queries(int dtype, const void* q, const int64_t* strides, int n_streams, int n_q, const artab_cache* c,
-                  const char* what) {
+int check_queries(int dtype, const void* q, int n_streams, int n_q, const artab_cache* c, const char* what) {
   ARTAB_REQUIRE(dtype == ARTAB_F32 || dtype == ARTAB_BF16, ARTAB_EINVAL, "%s: bad dtype %d", what, dtype);
-  ARTAB_REQUIRE(q && strides, ARTAB_EINVAL, "%s: null pointer", what);
+  ARTAB_REQUIRE(q, ARTAB_EINVAL, "%s: null pointer", what);
   ARTAB_REQUIRE(n_streams >= 1 && n_q >= 1 && (long)n_streams * n_q <= (1L << 28), ARTAB_EINVAL, "%s: bad query sizes",
                 what);
   ARTAB_REQUIRE(c->n_groups == 1 || c->n_groups == n_streams, ARTAB_EINVAL,

@@ -7,8 +7,8 @@
 // depend on tiling, and ties (broken by the lowest index) are real ties.
 //
 // One CTA = 16 queries of a (group, head): scores of all blocks into shared memory as ordered keys (products of
-// 16 queries x 8 blocks a warp), then one warp per query finds the n-th largest key bit by bit and writes the chosen
-// indices in ascending order.
+// 16 queries x 8 blocks a warp), then a warp takes two queries at a time, finds their n-th largest keys bit by bit
+// and writes the chosen indices in ascending order.
 #include "cache8.cuh"
 
 namespace artab {
@@ -25,12 +25,74 @@ struct SelectArgs {
   int32_t* index;          // [B][H][Lq][n_pick]
 };
 
-__device__ __forceinline__ float nearest_whole(float x, float step, float inv) {
-  const float f = x * inv;
-  float c = rintf(f);
-  if (!(fabsf(f - c) < 0.49995f)) c = (float)rint((double)x / (double)step);
-  return fminf(fmaxf(c, -127.0f), 127.0f);
-}
+constexpr int kHeld = 8;   // keys of a lane that are kept in registers: contexts of up to 16384 rows
+
+// Finds the n-th largest of `held` keys (n < held; lanes i, i + 32, ... hold key i) and writes the n indices chosen.
+struct Pick {
+  uint32_t key[kHeld];
+  const uint32_t* row;
+  uint32_t nth, bit;
+  int at_least;
+
+  template <typename F>
+  __device__ __forceinline__ int count(int held, F f) const {
+    int n = 0;
+    if (held <= 32 * kHeld) {
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) n += f(key[i]);
+    } else {
+      for (int i = threadIdx.x & 31; i < held; i += 32) n += f(row[i]);
+    }
+    return __reduce_add_sync(0xffffffffu, n);
+  }
+  __device__ __forceinline__ void start(const uint32_t* r, int held) {
+    const int lane = threadIdx.x & 31;
+    row = r;
+    uint32_t lo = 0xffffffffu, hi = 0;
+    if (held <= 32 * kHeld) {
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        const bool in = i * 32 + lane < held;
+        key[i] = in ? r[i * 32 + lane] : 0u;       // below every key
+        lo = in ? min(lo, key[i]) : lo, hi = max(hi, key[i]);
+      }
+    } else {
+      for (int i = lane; i < held; i += 32) lo = min(lo, r[i]), hi = max(hi, r[i]);
+    }
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    // bits that all keys share need no search
+    bit = lo == hi ? 0u : 0x80000000u >> __clz(lo ^ hi);
+    nth = bit ? hi & ~(2u * bit - 1u) : hi;
+    at_least = held;
+  }
+  __device__ __forceinline__ void narrow(int held, int n) {
+    const uint32_t trial = nth | bit;
+    const int c = count(held, [trial](uint32_t k) { return k >= trial ? 1 : 0; });
+    if (c >= n) nth = trial, at_least = c;
+    bit = at_least > n ? bit >> 1 : 0u;
+  }
+  __device__ __forceinline__ void write(int held, int n, int32_t* out) const {
+    const int lane = threadIdx.x & 31;
+    const uint32_t last = nth;
+    // every key above the n-th, and the first of those equal to it
+    int ties = n;
+    if (at_least > n) ties -= count(held, [last](uint32_t k) { return k > last ? 1 : 0; });
+    const bool exact = at_least == n;                // every key from nth on is taken
+    int done = 0;
+    for (int i0 = 0; i0 < held && done < n; i0 += 32) {
+      const bool there = i0 + lane < held;
+      const uint32_t k = there ? row[i0 + lane] : 0u;
+      const bool tie = there && !exact && k == last;
+      const uint32_t tied = __ballot_sync(0xffffffffu, tie);
+      const bool take = (there && (exact ? k >= last : k > last)) || (tie && __popc(tied & ((1u << lane) - 1u)) < ties);
+      const uint32_t taken = __ballot_sync(0xffffffffu, take);
+      if (take) out[done + __popc(taken & ((1u << lane) - 1u))] = i0 + lane;
+      ties -= min(ties, __popc(tied));
+      done += __popc(taken);
+    }
+  }
+};
 
 template <typename T, int DH>
 __global__ void __launch_bounds__(kThreads) cache_select_kernel(const SelectArgs a) {
@@ -48,35 +110,38 @@ __global__ void __launch_bounds__(kThreads) cache_select_kernel(const SelectArgs
   const int held = (len + kCacheBlock - 1) / kCacheBlock;
   const size_t gh = (size_t)group * H + h;
 
-  // thread t < 2: negative parts of channels t * NE .., for the lower bounds; t >= 2: positive parts, upper bounds
-  uint32_t qa[KS][4];
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int row = row0 + g + 8 * half;
-    float x[NE];
-#pragma unroll
-    for (int i = 0; i < NE; ++i) x[i] = 0.0f;
+  // the queries as whole numbers, four channels a thread
+  constexpr int C4 = DH / 4;
+  __shared__ __align__(16) __half s_q[kRows][DH];
+  for (int i = tid; i < kRows * C4; i += kThreads) {     // 64 - 256 pieces: whole warps
+    const int row = row0 + i / C4, c4 = i % C4;
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (row < a.rows) {
       const int b = one ? row / a.n_q : group, l = one ? row % a.n_q : row;
-      load_elements<T, NE>(reinterpret_cast<const T*>(a.q.p) + b * a.q.s0 + h * a.q.s1 + l * a.q.s2 + (t & 1) * NE, a.vec_q, x);
+      load_elements<T, 4>(reinterpret_cast<const T*>(a.q.p) + b * a.q.s0 + h * a.q.s1 + l * a.q.s2 + c4 * 4, a.vec_q, x);
     }
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < NE; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    for (int j = 0; j < 4; ++j) top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 1; o < C4; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float step = top < 0x7f800000u ? __fdiv_rn(__uint_as_float(top), 127.0f) : 0.0f;  // not finite: all zero
-    const float inv = step > 0.0f ? 1.0f / step : 0.0f;
-#pragma unroll
-    for (int i = 0; i < NE; ++i) {
-      x[i] = step > 0.0f ? nearest_whole(x[i], step, inv) : 0.0f;
-      x[i] = t < 2 ? fminf(x[i], 0.0f) : fmaxf(x[i], 0.0f);
-    }
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      qa[s][half] = h2_bits(__floats2half2_rn(x[4 * s], x[4 * s + 1]));
-      qa[s][2 + half] = h2_bits(__floats2half2_rn(x[4 * s + 2], x[4 * s + 3]));
-    }
+    const uint32_t w = step > 0.0f ? codes_of(x, step, 1.0f / step) : 0x80808080u;
+    *reinterpret_cast<uint2*>(&s_q[i / C4][c4 * 4]) = make_uint2(codes_to_halves(w, false), codes_to_halves(w, true));
   }
+  __syncthreads();
+  // thread t < 2: negative parts of channels t * NE .., for the lower bounds; t >= 2: positive parts, upper bounds
+  uint32_t qa[KS][4];
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const uint2 v = *reinterpret_cast<const uint2*>(&s_q[g + 8 * half][(t & 1) * NE + 4 * s]);
+      const __half2 zero = __float2half2_rn(0.0f);
+      const __half2 x = *reinterpret_cast<const __half2*>(&v.x), y = *reinterpret_cast<const __half2*>(&v.y);
+      qa[s][half] = h2_bits(t < 2 ? __hmin2(x, zero) : __hmax2(x, zero));
+      qa[s][2 + half] = h2_bits(t < 2 ? __hmin2(y, zero) : __hmax2(y, zero));
+    }
   const __half* bounds = reinterpret_cast<const __half*>(a.c.bounds) + gh * a.c.n_blocks * 2 * DH;
   const float* scales = a.c.scales + gh * a.c.n_blocks * 2;
   for (int j = warp * 8; j < held; j += kThreads / 32 * 8) {
@@ -107,45 +172,34 @@ __global__ void __launch_bounds__(kThreads) cache_select_kernel(const SelectArgs
     }
   }
   __syncthreads();
-  for (int r = warp; r < kRows; r += kThreads / 32) {
-    const int row = row0 + r;
-    if (row >= a.rows) break;
-    const uint32_t* key = s_key + r * a.pitch;
+  // two queries a warp, side by side: the steps of one hide in the latencies of the other
+  Pick pick[2];
+  int32_t* out[2];
+  const int n = a.n_pick;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row = row0 + 2 * warp + i;
     const int b = one ? row / a.n_q : group, l = one ? row % a.n_q : row;
-    int32_t* out = a.index + (((size_t)b * H + h) * a.n_q + l) * a.n_pick;
-    int done = 0;
-    if (held <= a.n_pick) {
-      for (int i = lane; i < held; i += 32) out[i] = i;
-      done = held;
-    } else {
-      uint32_t nth = 0;                                    // the n-th largest key
-      int at_least = held;                                 // keys >= nth
-      for (uint32_t bit = 0x80000000u; bit && at_least > a.n_pick; bit >>= 1) {
-        const uint32_t trial = nth | bit;
-        int count = 0;
-        for (int i = lane; i < held; i += 32) count += key[i] >= trial;
-        count = __reduce_add_sync(0xffffffffu, count);
-        if (count >= a.n_pick) nth = trial, at_least = count;
-      }
-      // every key above nth, and the first of those equal to it
-      int above = 0;
-      if (at_least > a.n_pick) {
-        for (int i = lane; i < held; i += 32) above += key[i] > nth;
-        above = __reduce_add_sync(0xffffffffu, above);
-      }
-      int ties = at_least > a.n_pick ? a.n_pick - above : a.n_pick;
-      for (int i0 = 0; i0 < held && done < a.n_pick; i0 += 32) {
-        const uint32_t k = i0 + lane < held ? key[i0 + lane] : 0u;
-        const bool in = i0 + lane < held && k > nth, tie = i0 + lane < held && k == nth;
-        const uint32_t tied = __ballot_sync(0xffffffffu, tie);
-        const bool take = in || (tie && __popc(tied & ((1u << lane) - 1u)) < ties);
-        const uint32_t taken = __ballot_sync(0xffffffffu, take);
-        if (take) out[done + __popc(taken & ((1u << lane) - 1u))] = i0 + lane;
-        ties -= min(ties, __popc(tied));
-        done += __popc(taken);
-      }
+    out[i] = row < a.rows ? a.index + (((size_t)b * H + h) * a.n_q + l) * n : nullptr;
+  }
+  if (!out[0]) return;
+  if (held > n) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) pick[i].start(s_key + (2 * warp + i) * a.pitch, held);   // the scores of a row of zeros, if need be
+    while (pick[0].bit | pick[1].bit) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (pick[i].bit) pick[i].narrow(held, n);
     }
-    for (int i = done + lane; i < a.n_pick; i += 32) out[i] = -1;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (!out[i]) continue;
+    if (held > n) {
+      pick[i].write(held, n, out[i]);
+    } else {
+      for (int j = lane; j < n; j += 32) out[i][j] = j < held ? j : -1;
+    }
   }
 }
 
@@ -172,7 +226,7 @@ extern "C" int artab_cache_select(int dtype, const void* q, const int64_t* q_str
                                   const artab_cache* c, int max_len, int n_pick, int32_t* index, void* stream) {
   int rc = check_cache(c, "cache_select");
   if (rc) return rc;
-  rc = check_queries(dtype, q, q_strides, n_streams, n_q, c, "cache_select");
+  rc = check_queries(dtype, q, n_streams, n_q, c, "cache_select");
   if (rc) return rc;
   ARTAB_REQUIRE(index && n_pick >= 1, ARTAB_EINVAL, "cache_select: no blocks asked for");
   ARTAB_REQUIRE(c->n_blocks <= kMaxBlocks, ARTAB_EINVAL, "cache_select: a cache of more than %d rows is not supported",
@@ -180,7 +234,7 @@ extern "C" int artab_cache_select(int dtype, const void* q, const int64_t* q_str
   (void)max_len;
   SelectArgs a;
   a.c = *c;
-  a.q = {q, (long)q_strides[0], (long)q_strides[1], (long)q_strides[2]};
+  a.q = row_view(q, q_strides, c->n_heads, n_q, c->head_dim);
   a.n_streams = n_streams;
   a.n_q = n_q;
   a.rows = c->n_groups == 1 ? n_streams * n_q : n_q;

@@ -1,17 +1,15 @@
 // Writing rows into the 8-bit context cache, and reading them back.
 //
-// write: one CTA per (group, head, touched block).  The scale of a block is its largest magnitude / 127; rows that
-// come behind others of a block may raise it, and the older rows are then rounded again to the new step.  Code
-// of x: the whole number nearest to x / scale in exact arithmetic, ties to even.  It is taken from a product with
-// the reciprocal in fp32; that is off by less than 3e-5, so where it lies closer than 5e-5 to a tie the quotient is
-// formed in 64 bits (once in 10 000 elements).
+// write: one CTA per (group, head, touched block), half of its threads on the keys, half on the values, 16 elements a
+// thread.  The scale of a block is its largest magnitude / 127; rows that come behind others of a block may raise
+// it, and the older rows are then rounded again to the new step.
+// Keys go out as they came in; of the values a thread holds the four rows that are neighbours in a channel's order, so
+// that it turns 4 x 4 bytes with permutes, and shared memory brings the words into the order of the record.
 // Both kernels move each byte once and are bounded by HBM for whole contexts, by one launch for a few rows.
 #include "cache8.cuh"
 
 namespace artab {
 namespace {
-
-constexpr int kWriteThreads = 256;
 
 struct WriteArgs {
   artab_cache c;
@@ -22,6 +20,7 @@ struct WriteArgs {
   int fresh;               // the whole cache is laid out: every block of it is given scales and bounds
   int set_lens;            // lens[g] = end of the rows written here
   int vec_k, vec_v;
+  int per_cta;             // blocks of a CTA
 };
 
 // the group's first row to write, and the row behind its last one
@@ -35,148 +34,227 @@ __device__ __forceinline__ void write_range(const WriteArgs& a, int g, int& star
   end = n > cap - s ? cap : s + n;
 }
 
-__device__ __forceinline__ int nearest_code(float x, float scale, float inv) {
-  const float f = x * inv;
-  float c = rintf(f);
-  if (!(fabsf(f - c) < 0.49995f)) c = (float)rint((double)x / (double)scale);
-  return (int)fminf(fmaxf(c, -127.0f), 127.0f);
+// 4 x 4 bytes: word r of the result holds byte r of every word
+__device__ __forceinline__ void turn(uint32_t (&w)[4]) {
+  const uint32_t a = __byte_perm(w[0], w[1], 0x5140), b = __byte_perm(w[2], w[3], 0x5140);
+  const uint32_t c = __byte_perm(w[0], w[1], 0x7362), d = __byte_perm(w[2], w[3], 0x7362);
+  w[0] = __byte_perm(a, b, 0x5410), w[1] = __byte_perm(a, b, 0x7632);
+  w[2] = __byte_perm(c, d, 0x5410), w[3] = __byte_perm(c, d, 0x7632);
 }
-__device__ __forceinline__ int moved_code(int code, float was, float scale, float inv) {
-  const float f = (float)code * was * inv;
-  float c = rintf(f);
-  if (!(fabsf(f - c) < 0.49995f)) c = (float)rint((double)code * (double)was / (double)scale);
-  return (int)fminf(fmaxf(c, -127.0f), 127.0f);
-}
+// first of the four rows {r, r + 1, r + 8, r + 9} that are neighbours in word `word` (0 .. 15) of a value channel
+__device__ __forceinline__ int first_row(int word) { return 16 * (word & 3) + 2 * (word >> 2); }
+
 __device__ __forceinline__ float step_of(uint32_t top_bits) {
   return top_bits >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : __fdiv_rn(__uint_as_float(top_bits), 127.0f);
 }
 // a block with a value that is not finite has NaN for its scale, for good
 __device__ __forceinline__ float larger_step(float a, float b) { return a != a ? a : b != b ? b : fmaxf(a, b); }
 
+template <int DH>
+struct Half {                      // threads of a CTA that work on the keys; as many again on the values
+  static constexpr int C4 = DH / 4, N = 16 * C4, WARPS = N / 32, VP = 17;   // VP: words of a padded value channel
+};
+
+__device__ __forceinline__ float larger_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// four neighbouring elements as they are stored
+template <typename T>
+struct Four;
+template <>
+struct Four<float> {
+  using Raw = uint4;
+  __device__ static __forceinline__ void values(const Raw& r, float (&x)[4]) {
+    x[0] = __uint_as_float(r.x), x[1] = __uint_as_float(r.y), x[2] = __uint_as_float(r.z), x[3] = __uint_as_float(r.w);
+  }
+  __device__ static __forceinline__ Raw zero() { return make_uint4(0u, 0u, 0u, 0u); }
+  __device__ static __forceinline__ float largest(const Raw (&r)[4]) {   // magnitude, NaN if there is one
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float x[4];
+      values(r[i], x);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = larger_or_nan(top, fabsf(x[j]));
+    }
+    return top;
+  }
+};
+template <>
+struct Four<__nv_bfloat16> {
+  using Raw = uint2;
+  __device__ static __forceinline__ void values(const Raw& r, float (&x)[4]) {
+    x[0] = __uint_as_float(r.x << 16), x[1] = __uint_as_float(r.x & 0xffff0000u);
+    x[2] = __uint_as_float(r.y << 16), x[3] = __uint_as_float(r.y & 0xffff0000u);
+  }
+  __device__ static __forceinline__ Raw zero() { return make_uint2(0u, 0u); }
+  __device__ static __forceinline__ float largest(const Raw (&r)[4]) {
+    __nv_bfloat162 top = __floats2bfloat162_rn(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&r[i].x)));
+      top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&r[i].y)));
+    }
+    return larger_or_nan(__low2float(top), __high2float(top));
+  }
+};
+template <typename T>
+__device__ __noinline__ typename Four<T>::Raw load_unaligned(const T* p) {
+  typename Four<T>::Raw r;
+  T* to = reinterpret_cast<T*>(&r);
+  for (int j = 0; j < 4; ++j) to[j] = p[j];
+  return r;
+}
 template <typename T, int DH>
-__global__ void __launch_bounds__(kWriteThreads) cache_write_kernel(const WriteArgs a) {
-  constexpr int C4 = DH / 4;                       // four-channel pieces of a row
-  constexpr int NC = kCacheBlock * C4 / kWriteThreads;
-  constexpr int VP = kCacheBlock + 4;              // padded value channel: byte stores of a warp spread over the banks
-  __shared__ __align__(16) uint8_t s_k[kCacheBlock * DH];
-  __shared__ __align__(16) uint8_t s_v[DH * VP];
-  __shared__ uint32_t s_top[2][8];
-  __shared__ uint32_t s_lo[8][C4], s_hi[8][C4];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+__global__ void __launch_bounds__(2 * Half<DH>::N, 768 / (2 * Half<DH>::N)) cache_write_kernel(const WriteArgs a) {
+  using F = Half<DH>;
+  using Raw = typename Four<T>::Raw;
+  constexpr int C4 = F::C4;
+  __shared__ uint32_t s_v[DH * F::VP];
+  __shared__ uint32_t s_top[2 * F::WARPS];
+  __shared__ uint2 s_lo[F::WARPS][C4], s_hi[F::WARPS][C4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool vals = threadIdx.x >= F::N;
+  const int tid = vals ? threadIdx.x - F::N : threadIdx.x, c4 = tid % C4, word = tid / C4;
   const int h = blockIdx.y, g = blockIdx.z;
   int start, end;
   write_range(a, g, start, end);
-  if (a.set_lens && blockIdx.x == 0 && h == 0 && tid == 0) a.c.lens[g] = end;
-  const int blk = a.fresh ? (int)blockIdx.x : start / kCacheBlock + (int)blockIdx.x;
-  if (blk >= a.c.n_blocks) return;
-  const int base = blk * kCacheBlock;
-  const size_t rec = ((size_t)g * a.c.n_heads + h) * a.c.n_blocks + blk;
-  float* scales = a.c.scales + rec * 2;
-  __half* bounds = reinterpret_cast<__half*>(a.c.bounds) + rec * 2 * DH;
-  if (end <= base) {                               // no row of this block
-    if (a.fresh) {
-      if (tid < 2) scales[tid] = 0.0f;
-      if (tid < 2 * DH) bounds[tid] = __float2half(0.0f);
+  if (a.set_lens && blockIdx.x == 0 && h == 0 && threadIdx.x == 0) a.c.lens[g] = end;
+  // the blocks of this CTA: `per_cta` neighbours
+  int blk = (a.fresh ? 0 : start / kCacheBlock) + (int)blockIdx.x * a.per_cta;
+  const int last = blk + a.per_cta < a.c.n_blocks ? blk + a.per_cta : a.c.n_blocks;
+  const size_t rec0 = ((size_t)g * a.c.n_heads + h) * a.c.n_blocks;
+  const RowView& src = vals ? a.v : a.k;
+  // the rows of a thread's four pieces: of keys 16 apart, of values those of a word
+  const int row0 = vals ? first_row(word) : word, d1 = vals ? 1 : 16, d2 = vals ? 8 : 32;
+  const long p1 = d1 * src.s2, p2 = d2 * src.s2;
+  const T* from = reinterpret_cast<const T*>(src.p) + g * src.s0 + h * src.s1 + ((long)blk * kCacheBlock + row0 - start) * src.s2 + c4 * 4;
+  const int vec = vals ? a.vec_v : a.vec_k;
+  const auto load = [&](int b, const T* p, Raw (&raw)[4]) {      // new rows of block b, zeros for the others
+    const int lo = start - b * kCacheBlock, hi = end - b * kCacheBlock;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = row0 + (i & 1) * d1 + (i >> 1) * d2;
+      const T* at = p + (i & 1) * p1 + (i >> 1) * p2;
+      raw[i] = Four<T>::zero();
+      if (row >= lo && row < hi) raw[i] = vec ? *reinterpret_cast<const Raw*>(at) : load_unaligned(at);
     }
-    return;
-  }
-  uint8_t* codes = a.c.codes + rec * (size_t)(2 * kCacheBlock * DH);
-  const int n_old = start > base ? start - base : 0;     // rows that are there already
-  const int n_live = end - base < kCacheBlock ? end - base : kCacheBlock;
-  const T* k0 = reinterpret_cast<const T*>(a.k.p) + g * a.k.s0 + h * a.k.s1;
-  const T* v0 = reinterpret_cast<const T*>(a.v.p) + g * a.v.s0 + h * a.v.s1;
-  const int c4 = tid % C4;
-  float x[2][NC][4];
-  uint32_t top_k = 0, top_v = 0;
-#pragma unroll
-  for (int i = 0; i < NC; ++i) {
-    const int row = (tid + i * kWriteThreads) / C4;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[0][i][j] = x[1][i][j] = 0.0f;
-    if (row >= n_old && row < n_live) {
-      const long src = base + row - start;
-      load_elements<T, 4>(k0 + src * a.k.s2 + c4 * 4, a.vec_k, x[0][i]);
-      load_elements<T, 4>(v0 + src * a.v.s2 + c4 * 4, a.vec_v, x[1][i]);
+  };
+  Raw next[4];
+  if (blk < last) load(blk, from, next);
+  for (; blk < last; ++blk) {
+    const int base = blk * kCacheBlock;
+    float* scales = a.c.scales + (rec0 + blk) * 2;
+    __half* bounds = reinterpret_cast<__half*>(a.c.bounds) + (rec0 + blk) * 2 * DH;
+    if (end <= base) {                               // no row of this block
+      if (!a.fresh) return;
+      if (threadIdx.x < 2) scales[threadIdx.x] = 0.0f;
+      if (threadIdx.x < 2 * DH) bounds[threadIdx.x] = __float2half(0.0f);
+      continue;
     }
+    uint32_t* codes = reinterpret_cast<uint32_t*>(a.c.codes + (rec0 + blk) * (size_t)(2 * kCacheBlock * DH)) + (vals ? kCacheBlock * C4 : 0);
+    const int n_old = start > base ? start - base : 0;     // rows that are there already
+    const int n_live = end - base < kCacheBlock ? end - base : kCacheBlock;
+    Raw raw[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {                  // magnitudes order like their bit patterns, NaN above all
-      top_k = max(top_k, __float_as_uint(x[0][i][j]) & 0x7fffffffu);
-      top_v = max(top_v, __float_as_uint(x[1][i][j]) & 0x7fffffffu);
+    for (int i = 0; i < 4; ++i) raw[i] = next[i];
+    from += kCacheBlock * src.s2;
+    if (blk + 1 < last) load(blk + 1, from, next);
+    const float was = n_old ? scales[vals] : 0.0f;
+    const float top = Four<T>::largest(raw);
+    const uint32_t warp_top = __reduce_max_sync(0xffffffffu, __float_as_uint(top));   // NaN above all
+    if (lane == 0) s_top[warp] = warp_top;
+    uint32_t old[4] = {0u, 0u, 0u, 0u};
+    if (n_old) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) old[i] = vals ? codes[(c4 * 4 + i) * 16 + word] : codes[(word + 16 * i) * C4 + c4];
+      if (vals) turn(old);
     }
-  }
-  top_k = __reduce_max_sync(0xffffffffu, top_k);
-  top_v = __reduce_max_sync(0xffffffffu, top_v);
-  if (lane == 0) s_top[0][warp] = top_k, s_top[1][warp] = top_v;
-  const float was_k = n_old ? scales[0] : 0.0f, was_v = n_old ? scales[1] : 0.0f;
-  __syncthreads();
-  top_k = top_v = 0;
+    __syncthreads();   // also: every thread has read the old codes and scales
+    uint32_t block_top = 0;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) top_k = max(top_k, s_top[0][w]), top_v = max(top_v, s_top[1][w]);
-  const float ks = larger_step(was_k, step_of(top_k)), vs = larger_step(was_v, step_of(top_v));
-  // a step of zero (or NaN) has zero codes: the reciprocal is then zero and no quotient is formed
-  const float ki = ks > 0.0f ? 1.0f / ks : 0.0f, vi = vs > 0.0f ? 1.0f / vs : 0.0f;
-  uint32_t lo = 0xffffffffu, hi = 0;
+    for (int w = 0; w < F::WARPS; ++w) block_top = max(block_top, s_top[(vals ? F::WARPS : 0) + w]);
+    // a step of zero (or NaN) has zero codes
+    const float step = larger_step(was, step_of(block_top)), inv = 1.0f / step;
+    uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < NC; ++i) {
-    const int row = (tid + i * kWriteThreads) / C4;
-    uint32_t wk = 0x80808080u, wv = 0x80808080u;
-    if (row < n_old) {
-      wk = *reinterpret_cast<const uint32_t*>(codes + row * DH + c4 * 4);
-      wv = 0;
+    for (int i = 0; i < 4; ++i) {
+      float x[4];
+      Four<T>::values(raw[i], x);
+      w[i] = step > 0.0f ? codes_of(x, step, inv) : 0x80808080u;   // rows that are not new are zeros
+    }
+    if (n_old) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        wv |= (uint32_t)codes[kCacheBlock * DH + (c4 * 4 + j) * kCacheBlock + cache_value_place(row)] << (8 * j);
-      if (ks > was_k) {
-        uint32_t y = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          y |= (uint32_t)(moved_code((int)((wk >> (8 * j)) & 255u) - 128, was_k, ks, ki) + 128) << (8 * j);
-        wk = y;
-      }
-      if (vs > was_v) {
-        uint32_t y = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          y |= (uint32_t)(moved_code((int)((wv >> (8 * j)) & 255u) - 128, was_v, vs, vi) + 128) << (8 * j);
-        wv = y;
-      }
-    } else if (row < n_live) {
-      wk = wv = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        wk |= (uint32_t)((ks > 0.0f ? nearest_code(x[0][i][j], ks, ki) : 0) + 128) << (8 * j);
-        wv |= (uint32_t)((vs > 0.0f ? nearest_code(x[1][i][j], vs, vi) : 0) + 128) << (8 * j);
+      for (int i = 0; i < 4; ++i) {
+        if (row0 + (i & 1) * d1 + (i >> 1) * d2 >= n_old) continue;
+        w[i] = old[i];
+        if (step > was) {
+          float y[4];
+          code_values(old[i], y);
+          w[i] = kept_codes(y, was, step, inv);
+        }
       }
     }
-    if (row < n_live) lo = __vminu4(lo, wk), hi = __vmaxu4(hi, wk);
-    *reinterpret_cast<uint32_t*>(s_k + row * DH + c4 * 4) = wk;
+    if (vals) {
+      turn(w);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s_v[(c4 * 4 + j) * VP + cache_value_place(row)] = (uint8_t)(wv >> (8 * j));
-  }
+      for (int i = 0; i < 4; ++i) s_v[(c4 * 4 + i) * F::VP + word] = w[i];
+    } else {
+      // smallest and largest code of the channels, as halves 1024 + byte
+      __half2 lo[2], hi[2];
 #pragma unroll
-  for (int o = C4; o < 32; o <<= 1) {
-    lo = __vminu4(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = __vmaxu4(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  }
-  if (lane < C4) s_lo[warp][lane] = lo, s_hi[warp][lane] = hi;
-  __syncthreads();   // also: every thread has read the old codes and scales
+      for (int j = 0; j < 2; ++j) lo[j] = __float2half2_rn(2048.0f), hi[j] = __float2half2_rn(0.0f);
 #pragma unroll
-  for (int i = tid; i < kCacheBlock * DH / 16; i += kWriteThreads)
-    reinterpret_cast<uint4*>(codes)[i] = reinterpret_cast<const uint4*>(s_k)[i];
+      for (int i = 0; i < 4; ++i) {
+        codes[(word + 16 * i) * C4 + c4] = w[i];
+        if (row0 + 16 * i >= n_live) continue;
 #pragma unroll
-  for (int i = tid; i < kCacheBlock * DH / 4; i += kWriteThreads)
-    reinterpret_cast<uint32_t*>(codes + kCacheBlock * DH)[i] =
-        *reinterpret_cast<const uint32_t*>(s_v + (i / 16) * VP + (i % 16) * 4);
-  if (tid < C4) {
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t u = __byte_perm(w[i], 0x64646464u, j ? 0x4342u : 0x4140u);
+          lo[j] = __hmin2(lo[j], *reinterpret_cast<const __half2*>(&u));
+          hi[j] = __hmax2(hi[j], *reinterpret_cast<const __half2*>(&u));
+        }
+      }
 #pragma unroll
-    for (int w = 0; w < 8; ++w) lo = __vminu4(w ? lo : s_lo[0][tid], s_lo[w][tid]), hi = __vmaxu4(w ? hi : s_hi[0][tid], s_hi[w][tid]);
+      for (int o = C4; o < 32; o <<= 1)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      bounds[tid * 4 + j] = __int2half_rn((int)((lo >> (8 * j)) & 255u) - 128);
-      bounds[DH + tid * 4 + j] = __int2half_rn((int)((hi >> (8 * j)) & 255u) - 128);
+        for (int j = 0; j < 2; ++j) {
+          lo[j] = __hmin2(lo[j], __shfl_xor_sync(0xffffffffu, lo[j], o));
+          hi[j] = __hmax2(hi[j], __shfl_xor_sync(0xffffffffu, hi[j], o));
+        }
+      if (lane < C4) {
+        s_lo[warp][lane] = make_uint2(h2_bits(lo[0]), h2_bits(lo[1]));
+        s_hi[warp][lane] = make_uint2(h2_bits(hi[0]), h2_bits(hi[1]));
+      }
     }
+    __syncthreads();
+    if (vals) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = tid + i * F::N;
+        codes[at] = s_v[(at / 16) * F::VP + at % 16];
+      }
+    } else if (tid < 2 * C4) {                       // a thread per four channels of either bound
+      const bool upper = tid >= C4;
+      uint2 best = upper ? s_hi[0][tid - C4] : s_lo[0][tid];
+      const __half2 off = __float2half2_rn(1152.0f);
+#pragma unroll
+      for (int r = 1; r < F::WARPS; ++r) {
+        const uint2 u = upper ? s_hi[r][tid - C4] : s_lo[r][tid];
+        const __half2 x = *reinterpret_cast<const __half2*>(&u.x), y = *reinterpret_cast<const __half2*>(&u.y);
+        __half2 &bx = *reinterpret_cast<__half2*>(&best.x), &by = *reinterpret_cast<__half2*>(&best.y);
+        bx = upper ? __hmax2(bx, x) : __hmin2(bx, x);
+        by = upper ? __hmax2(by, y) : __hmin2(by, y);
+      }
+      best.x = h2_bits(__hsub2(*reinterpret_cast<__half2*>(&best.x), off));
+      best.y = h2_bits(__hsub2(*reinterpret_cast<__half2*>(&best.y), off));
+      reinterpret_cast<uint2*>(bounds)[tid] = best;
+    }
+    if (tid == 0) scales[vals] = step;
   }
-  if (tid == 0) scales[0] = ks, scales[1] = vs;
 }
 
 // lens[g] moves behind the rows that cache_write_kernel has put there from lens[g] on
@@ -195,57 +273,64 @@ struct ReadArgs {
   void *k, *v;
 };
 
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const float (&x)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+  } else {
+    __nv_bfloat162 y[2] = {__floats2bfloat162_rn(x[0], x[1]), __floats2bfloat162_rn(x[2], x[3])};
+    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(y);
+  }
+}
+
 template <typename T, int DH>
-__global__ void __launch_bounds__(kWriteThreads) cache_read_kernel(const ReadArgs a) {
-  constexpr int C4 = DH / 4, NC = kCacheBlock * C4 / kWriteThreads, VP = kCacheBlock + 4;
-  __shared__ __align__(16) uint8_t s_v[DH * VP];
-  const int tid = threadIdx.x, h = blockIdx.y, g = blockIdx.z;
+__global__ void __launch_bounds__(2 * Half<DH>::N) cache_read_kernel(const ReadArgs a) {
+  using F = Half<DH>;
+  constexpr int C4 = F::C4;
+  __shared__ uint32_t s_v[DH * F::VP];
+  const bool vals = threadIdx.x >= F::N;
+  const int tid = vals ? threadIdx.x - F::N : threadIdx.x, c4 = tid % C4, word = tid / C4;
+  const int h = blockIdx.y, g = blockIdx.z;
   const int cap = a.c.n_blocks * kCacheBlock;
   int len = a.c.lens[g], start = a.start ? a.start[g] : 0;
   len = len < 0 ? 0 : len > cap ? cap : len;
   start = start < 0 ? 0 : start;
   const long base = ((long)(start / kCacheBlock) + blockIdx.x) * kCacheBlock;
   if (base >= (long)start + a.n_rows) return;
-  const size_t out0 = ((size_t)g * a.c.n_heads + h) * a.n_rows;
   const bool any = base < len;
   const size_t rec = ((size_t)g * a.c.n_heads + h) * a.c.n_blocks + (any ? base / kCacheBlock : 0);
-  const uint8_t* codes = a.c.codes + rec * (size_t)(2 * kCacheBlock * DH);
-  float ks = 0.0f, vs = 0.0f;
-  uint32_t wk[NC];
+  const uint32_t* codes = reinterpret_cast<const uint32_t*>(a.c.codes + rec * (size_t)(2 * kCacheBlock * DH)) + (vals ? kCacheBlock * C4 : 0);
+  uint32_t w[4] = {0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};
+  const float step = any ? a.c.scales[rec * 2 + vals] : 0.0f;
   if (any) {
-    ks = a.c.scales[rec * 2], vs = a.c.scales[rec * 2 + 1];
 #pragma unroll
-    for (int i = 0; i < NC; ++i) wk[i] = reinterpret_cast<const uint32_t*>(codes)[tid + i * kWriteThreads];
+    for (int i = 0; i < 4; ++i) w[i] = codes[tid + i * F::N];
+  }
+  if (vals) {
 #pragma unroll
-    for (int i = tid; i < kCacheBlock * DH / 4; i += kWriteThreads)
-      *reinterpret_cast<uint32_t*>(s_v + (i / 16) * VP + (i % 16) * 4) =
-          reinterpret_cast<const uint32_t*>(codes + kCacheBlock * DH)[i];
+    for (int i = 0; i < 4; ++i) {
+      const int at = tid + i * F::N;
+      s_v[(at / 16) * F::VP + at % 16] = w[i];
+    }
   }
   __syncthreads();
-  const int c4 = tid % C4;
+  if (vals) {
 #pragma unroll
-  for (int i = 0; i < NC; ++i) {
-    const int row = (tid + i * kWriteThreads) / C4;
+    for (int i = 0; i < 4; ++i) w[i] = s_v[(c4 * 4 + i) * F::VP + word];
+    turn(w);
+  }
+  T* out = reinterpret_cast<T*>(vals ? a.v : a.k) + ((size_t)g * a.c.n_heads + h) * a.n_rows * DH + c4 * 4;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = vals ? first_row(word) + (i & 1) + 8 * (i >> 1) : word + 16 * i;
     const long at = base + row - start;
     if (at < 0 || at >= a.n_rows) continue;
-    float k[4] = {0.0f, 0.0f, 0.0f, 0.0f}, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (base + row < len) {
+    float x[4];
+    code_values(w[i], x);
+    const bool live = base + row < len;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        k[j] = (float)((int)((wk[i] >> (8 * j)) & 255u) - 128) * ks;
-        v[j] = (float)((int)s_v[(c4 * 4 + j) * VP + cache_value_place(row)] - 128) * vs;
-      }
-    }
-    const size_t o = (out0 + (size_t)at) * DH + c4 * 4;
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.k) + o) = make_float4(k[0], k[1], k[2], k[3]);
-      *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.v) + o) = make_float4(v[0], v[1], v[2], v[3]);
-    } else {
-      __nv_bfloat162 p[2] = {__floats2bfloat162_rn(k[0], k[1]), __floats2bfloat162_rn(k[2], k[3])};
-      __nv_bfloat162 r[2] = {__floats2bfloat162_rn(v[0], v[1]), __floats2bfloat162_rn(v[2], v[3])};
-      *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.k) + o) = *reinterpret_cast<uint2*>(p);
-      *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.v) + o) = *reinterpret_cast<uint2*>(r);
-    }
+    for (int j = 0; j < 4; ++j) x[j] = live ? x[j] * step : 0.0f;
+    store4<T>(out + at * DH, x);
   }
 }
 
@@ -264,7 +349,7 @@ template <typename T, int DH>
 struct LaunchWrite {
   static int go(const WriteArgs& a, dim3 grid, cudaStream_t s) {
     count_launch();
-    cache_write_kernel<T, DH><<<grid, kWriteThreads, 0, s>>>(a);
+    cache_write_kernel<T, DH><<<grid, 2 * Half<DH>::N, 0, s>>>(a);
     return check_launch("cache_write");
   }
 };
@@ -272,7 +357,7 @@ template <typename T, int DH>
 struct LaunchRead {
   static int go(const ReadArgs& a, dim3 grid, cudaStream_t s) {
     count_launch();
-    cache_read_kernel<T, DH><<<grid, kWriteThreads, 0, s>>>(a);
+    cache_read_kernel<T, DH><<<grid, 2 * Half<DH>::N, 0, s>>>(a);
     return check_launch("cache_read");
   }
 };
@@ -304,15 +389,15 @@ int artab_cache_write(int dtype, const void* k, const int64_t* k_strides, const 
   int rc = check_cache(c, "cache_write");
   if (rc) return rc;
   ARTAB_REQUIRE(dtype == ARTAB_F32 || dtype == ARTAB_BF16, ARTAB_EINVAL, "cache_write: bad dtype %d", dtype);
-  ARTAB_REQUIRE(k && v && k_strides && v_strides && n_rows >= 1, ARTAB_EINVAL, "cache_write: no rows");
+  ARTAB_REQUIRE(k && v && n_rows >= 1, ARTAB_EINVAL, "cache_write: no rows");
   ARTAB_REQUIRE(!(fresh && start), ARTAB_EINVAL, "cache_write: a fresh cache starts at row 0");
   ARTAB_REQUIRE(!fresh || (n_rows + kCacheBlock - 1) / kCacheBlock <= c->n_blocks, ARTAB_ECAPACITY,
                 "cache_write: %d rows in a cache of %d", n_rows, c->n_blocks * kCacheBlock);
   cudaStream_t s = (cudaStream_t)stream;
   WriteArgs a;
   a.c = *c;
-  a.k = {k, (long)k_strides[0], (long)k_strides[1], (long)k_strides[2]};
-  a.v = {v, (long)v_strides[0], (long)v_strides[1], (long)v_strides[2]};
+  a.k = row_view(k, k_strides, c->n_heads, n_rows, c->head_dim);
+  a.v = row_view(v, v_strides, c->n_heads, n_rows, c->head_dim);
   a.start = fresh ? nullptr : start ? start : c->lens;
   a.counts = counts;
   a.n_rows = n_rows;
@@ -327,7 +412,11 @@ int artab_cache_write(int dtype, const void* k, const int64_t* k_strides, const 
   a.vec_v = rows_aligned(a.v, elem);
   long nb = fresh ? c->n_blocks : (n_rows + 2L * kCacheBlock - 2) / kCacheBlock;   // n rows from anywhere in a block
   if (nb > c->n_blocks) nb = c->n_blocks;
-  rc = by_type_and_size<LaunchWrite>(dtype, c->head_dim, a, dim3((unsigned)nb, c->n_heads, c->n_groups), s);
+  // several blocks a CTA once there are many: the rows of the next are on their way while one is worked on
+  const long all = nb * c->n_heads * c->n_groups;
+  a.per_cta = (int)(all / (148L * 16) < 1 ? 1 : all / (148L * 16) > 8 ? 8 : all / (148L * 16));
+  rc = by_type_and_size<LaunchWrite>(dtype, c->head_dim, a,
+                                     dim3((unsigned)((nb + a.per_cta - 1) / a.per_cta), c->n_heads, c->n_groups), s);
   if (rc || a.set_lens) return rc;
   count_launch();
   cache_advance_kernel<<<(c->n_groups + 255) / 256, 256, 0, s>>>(a);

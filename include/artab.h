@@ -380,7 +380,7 @@ typedef struct artab_cache {
 } artab_cache;
 
 /* Rows into the cache.  k, v [G][H][n_rows][Dh] of `dtype`, by HOST arrays of three strides (elements; group, head,
- * row).  Group g takes its first counts[g] rows (NULL: n_rows; clamped to [0, n_rows]) and keeps them as rows
+ * row; NULL: contiguous).  Group g takes its first counts[g] rows (NULL: n_rows; clamped to [0, n_rows]) and keeps them as rows
  * start[g] .. (NULL: lens[g] ..) of the context; what lay at or behind start[g] is dropped and lens[g] becomes
  * start[g] + counts[g].  Rows beyond the capacity are left out.  start / counts may be lens itself, not
  * overlap it otherwise.  A block's scale is the larger of the one it had (where rows before start[g] are kept) and that
@@ -395,7 +395,7 @@ ARTAB_API int artab_cache_write(int dtype, const void* k, const int64_t* k_strid
 ARTAB_API int artab_cache_read(int dtype, const artab_cache* c, const int32_t* start, int n_rows, void* k, void* v,
                                void* stream);
 
-/* Attention of q [B][H][Lq][Dh] (HOST array of three strides: stream, head, query) over the rows in use:
+/* Attention of q [B][H][Lq][Dh] (HOST array of three strides: stream, head, query; NULL: contiguous) over the rows in use:
  * out [B][H][Lq][Dh] of `dtype`, lse [B][H][Lq] (natural log).  A context of no rows gives 0 and -inf.
  * max_len: a bound of lens known to the host, for the choice of launch only (results do not depend on its truth). */
 ARTAB_API int artab_cache_attention(int dtype, const void* q, const int64_t* q_strides, int n_streams, int n_q,

@@ -345,6 +345,27 @@ def test_scales_of_scores_and_magnitudes(dtype, B):
         check_attention(c.context_cache_attention(x, cache), attention(x, cache, 32 ** -0.5), dtype, 32)
 
 
+@pytest.mark.parametrize("B", [2, 100])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_values_that_are_not_finite_leave_the_weights_sound(dtype, B):
+    c = cc()
+    k, v = rows(28, 1, 3, 300, 32, dtype)
+    q = torch.randn(B, 3, 1, 32, device="cuda", generator=gen(29)).to(dtype)
+    sound = c.quantize_context(k, v)
+    want = attention(q, sound, 32 ** -0.5)
+    v[0, 1, 200, 3], k[0, 2, 0, 0] = float("nan"), float("-inf")
+    out, lse = c.context_cache_attention(q, c.quantize_context(k, v))
+    # the value scales of a head are factors of its numerators, taken out of their sum again: not the same bits as with
+    # sound values, but the same bound.  Head 1's outputs are NaN, so the sound ones stand in for them here.
+    assert bool(torch.isnan(out[:, 1:]).all()) and bool(torch.isnan(lse[:, 2]).all())
+    mixed = torch.where(torch.isnan(out), want[0].to(dtype), out), torch.where(torch.isnan(lse), want[1].float(), lse)
+    check_attention(mixed, want, dtype, 32)
+    v[0, 1], k[0, 2] = v[0, 1] * 0, k[0, 2] * 0               # a head of zero values, one of zero keys
+    v[0, 1, 200, 3] = k[0, 2, 0, 0] = 0.0
+    cache = c.quantize_context(torch.nan_to_num(k), torch.nan_to_num(v))
+    check_attention(c.context_cache_attention(q, cache), attention(q, cache, 32 ** -0.5), dtype, 32)
+
+
 @pytest.mark.parametrize("B", [3, 130])
 def test_queries_by_strides_and_odd_addresses(B):
     c = cc()
