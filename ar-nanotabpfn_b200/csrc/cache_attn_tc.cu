@@ -12,8 +12,7 @@
 // queries of bf16 are exact in them (scaled by a power of two per row), codes are whole numbers, numerators keep
 // 11 bits.  Scales of keys go into the exponent's factor, scales of values into its offset (relative to the largest of the
 // context, taken out of the row sum again), so O accumulates over all blocks.
-// What bounds it is the exponential: 64 per row and block, 16 a clock and SM on the special-function unit; a
-// quarter of them is computed on the FMA pipe.  Two CTAs share an SM (256 TMEM columns each), so four warpgroups are in
+// Two CTAs share an SM (256 TMEM columns each), so four warpgroups are in
 // different phases of their blocks.  head_dim 64 has no room for P beside S: it overwrites the scores it came from, and the
 // next scores wait for P . V.
 // Every wait is bounded; a CTA that gives up writes NaN for its rows.
@@ -22,15 +21,10 @@
 namespace artab {
 namespace {
 
-constexpr int BM = 128, BN = kCacheBlock, kStages = 4, kThreads = 384, kConvert = 64;
+constexpr int BM = 128, BN = kCacheBlock, kStages = 4, kAhead = 3, kThreads = 384, kConvert = 64;
 constexpr uint32_t kTmemCols = 256;
-// numerators are 2^6 times exp(s - reference); the reference lags by at most 2^8 before it is raised
-constexpr float kLiftTc = 6.0f, kLag = 8.0f;
-// 2^f on [-0.5, 0.5]: least largest relative error, 2.6e-6
-constexpr float kExp0 = 0.999999285f, kExp1 = 0.69312185f, kExp2 = 0.240247443f, kExp3 = 0.0559177138f, kExp4 = 0.00957003608f;
-#ifndef ARTAB_CACHE_POLY_OF_8
-#define ARTAB_CACHE_POLY_OF_8 2
-#endif
+// numerators are 2^6 times exp(s - reference)
+constexpr float kLiftTc = 6.0f;
 
 struct Ctl {
   int abort_flag, pad;
@@ -41,6 +35,7 @@ struct __align__(1024) TcSmem {
   uint8_t k[kStages][BN * DH * 2];       // [64 rows][DH] halves
   uint8_t v[kStages][DH * 128];          // [DH][64 rows] halves
   uint8_t q[BM * DH * 2];
+  uint8_t raw[kAhead][2 * BN * DH];      // records as they are kept
   uint64_t q_full, kv_full[kStages], kv_empty[kStages];
   uint64_t s_full[2], s_free[2], p_full[2], o_full[2];
   float vmax[kThreads / 32];
@@ -55,19 +50,60 @@ __device__ __forceinline__ void mbar_init(uint64_t* b, uint32_t count) {
 __device__ __forceinline__ void mbar_arrive(uint64_t* b) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
 }
-// false when the CTA is giving up (this wait or another one ran out)
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile Ctl* ctl) {
-  const uint32_t b = smem_u32(bar);
-  if (mbar_try(b, parity)) return true;
+// one lane of a whole warp, the same one every time
+__device__ __forceinline__ bool elected() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+__device__ __forceinline__ float lg2(float x) {
+  float r;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// False when the CTA is giving up (this wait or another one ran out).  The clock and the flag are looked at now and then
+// only: eight warps of an SM wait at any time, and what they issue is taken from the others.
+__device__ __forceinline__ bool mbar_tries(uint32_t b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\t"
+      "mov.u32 n, 32;\n"
+      "again:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra done;\n\t"
+      "sub.u32 n, n, 1;\n\t"
+      "setp.ne.u32 q, n, 0;\n\t"
+      "@q bra again;\n"
+      "done:\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(b), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __noinline__ bool mbar_wait_long(uint32_t b, uint32_t parity, volatile Ctl* ctl) {
   const long long t0 = clock64();
   for (;;) {
-    if (mbar_try(b, parity)) return true;
+    if (mbar_tries(b, parity)) return true;
     if (ctl->abort_flag) return false;
     if (clock64() - t0 > ctl->limit) {
       ctl->abort_flag = 1;
       return false;
     }
   }
+}
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile Ctl* ctl) {
+  const uint32_t b = smem_u32(bar);
+  return mbar_tries(b, parity) || mbar_wait_long(b, parity, ctl);
 }
 
 // K-major tile of rows of 32, 64 or 128 bytes: swizzle of that span, groups of eight rows behind one another
@@ -76,6 +112,12 @@ __device__ __forceinline__ uint32_t swizzled(uint32_t row, uint32_t chunk) {   /
   constexpr uint32_t kMask = ROW_BYTES / 16 - 1;
   constexpr uint32_t kShift = ROW_BYTES == 128 ? 0 : ROW_BYTES == 64 ? 1 : 2;
   return row * ROW_BYTES + ((chunk ^ ((row >> kShift) & kMask)) << 4);
+}
+__device__ __forceinline__ void st_shared16(uint32_t at, const uint4& v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ void st_shared4(uint32_t at, uint32_t v) {
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
 }
 template <int ROW_BYTES>
 __device__ __forceinline__ uint64_t tile_desc(uint32_t saddr) {
@@ -154,31 +196,130 @@ __device__ __forceinline__ float2 pk_add(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
-// 2^x on the FMA pipe for x <= 16: the nearest integer n by adding 1.5 * 2^23, a polynomial of degree four for
-// 2^f, f = x - n in [-0.5, 0.5] (relative error 2.6e-6), n into the exponent field.  Below
-// 2^-125 the result is nothing; a NaN stays one.
-__device__ __forceinline__ float2 ex2_fma(float2 x) {
-  const float2 y = make_float2(x.x < -125.0f ? -125.0f : x.x, x.y < -125.0f ? -125.0f : x.y);
-  const float2 r = pk_add(y, make_float2(12582912.0f, 12582912.0f));
-  const float2 n = pk_add(r, make_float2(-12582912.0f, -12582912.0f));
-  const float2 f = pk_fma(n, make_float2(-1.0f, -1.0f), y);
-  float2 p = pk_fma(make_float2(kExp4, kExp4), f, make_float2(kExp3, kExp3));
-  p = pk_fma(p, f, make_float2(kExp2, kExp2));
-  p = pk_fma(p, f, make_float2(kExp1, kExp1));
-  p = pk_fma(p, f, make_float2(kExp0, kExp0));
-  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23)),
-                     __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23)));
+// Tensor memory of a warpgroup: scores, numerators (packed halves), output.
+template <int DH>
+struct Plan {
+  static constexpr bool kAlias = DH == 64;           // numerators in the columns of the scores
+  static constexpr uint32_t kColP = kAlias ? BN / 2 : BN, kColO = kAlias ? BN : BN + BN / 2, kColsWg = kTmemCols / 2;
+};
+
+// Numerators of 32 scores of this thread's row against the reference m: packed halves, and their sum.
+template <bool MASKED>
+__device__ __forceinline__ float numerators(const uint32_t (&r)[32], uint32_t (&pk)[16], float slope, float add, int live) {
+  const float2 sl2 = make_float2(slope, slope), add2 = make_float2(add, add);
+  float2 sums[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+  for (int e = 0; e < 32; e += 2) {
+    float2 y = pk_fma(make_float2(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), sl2, add2);
+    y = make_float2(ex2(y.x), ex2(y.y));
+    if (MASKED) {
+      if (e >= live) y.x = 0.0f;
+      if (e + 1 >= live) y.y = 0.0f;
+    }
+    sums[(e >> 1) & 1] = pk_add(sums[(e >> 1) & 1], y);
+    pk[e >> 1] = h2_bits(__floats2half2_rn(y.x, y.y));
+  }
+  return (sums[0].x + sums[1].x) + (sums[0].y + sums[1].y);
+}
+template <bool MASKED>
+__device__ __forceinline__ float largest(const uint32_t (&r)[32], int live) {
+  float top[4];                                   // four chains: one would wait for itself
+#pragma unroll
+  for (int e = 0; e < 4; ++e) top[e] = -CUDART_INF_F;
+#pragma unroll
+  for (int e = 0; e < 32; ++e)
+    if (!MASKED || e < live) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(r[e]));
+  return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+}
+
+// One block of a warpgroup: scores of this thread's row out of tensor memory, numerators back into it, 32 columns at a
+// time, the upper ones first (where numerators overwrite scores, they overwrite those).  MASKED: the block's last rows
+// are not in use.  False when a wait gave up.
+//
+// The scores are read once: the reference m is a score of the row's first block, and stays until the sum of 32
+// numerators shows that one may have passed the range of halves (2^10 above m).  Then, rarely on ordinary
+// scores, m rises by a whole number k and all that was taken against it shrinks by 2^-k, exactly: sums, the numerators
+// that are in tensor memory, the output.  The result does not depend on m.
+constexpr float kMostSum = 60000.0f;
+template <int DH, bool MASKED>
+__device__ __forceinline__ bool softmax_block(TcSmem<DH>* sm, uint32_t t_row, int wg, int i, float slope, float lift,
+                                              float unlift, int live, float& m, float& l) {
+  constexpr bool kAlias = Plan<DH>::kAlias;
+  constexpr uint32_t kColP = Plan<DH>::kColP, kColO = Plan<DH>::kColO;
+  volatile Ctl* ctl = &sm->ctl;
+  bool ok = true;
+  float sum = 0.0f;
+#pragma unroll 1
+  for (int c = 1; c >= 0; --c) {
+    uint32_t r[32], pk[16];
+    tmem_ld32(t_row + 32 * c, r);
+    wait_ld();
+    const int lv = live - 32 * c;
+    if (i == 0 && c == 1) m = MASKED && lv <= 0 ? m : largest<MASKED>(r, lv) * slope;   // no row of these in use: not yet
+    if (MASKED && i == 0 && c == 0 && live <= 32) m = largest<MASKED>(r, lv) * slope;
+    float part = numerators<MASKED>(r, pk, slope, lift - m, lv);
+    if (c == 1 && i > 0) {                        // the P . V before this one has read P and written O
+      if (!kAlias) ok = __all_sync(0xffffffffu, mbar_wait(&sm->o_full[wg], (i - 1) & 1, ctl));
+      fence_after();
+    }
+    if (__any_sync(0xffffffffu, !(part < kMostSum))) {
+      float k = 0.0f;
+      tmem_ld32(t_row + 32 * c, r);               // again: kept in registers they would cost the common path copies
+      wait_ld();
+      if (!(part < kMostSum)) k = fmaxf(ceilf(largest<MASKED>(r, lv) * slope - m), 0.0f);
+      m += k;
+      const float alpha = ex2(-k);
+      part = numerators<MASKED>(r, pk, slope, lift - m, lv);
+      l *= alpha;
+      sum *= alpha;
+      if (c == 0) {                               // the other half of this block's numerators
+        uint32_t u[16];
+        wait_st();
+        tmem_ld16(t_row + kColP + 16, u);
+        wait_ld();
+        const __half2 al = __float2half2_rn(alpha);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) u[e] = h2_bits(__hmul2(*reinterpret_cast<const __half2*>(&u[e]), al));
+        tmem_st16(t_row + kColP + 16, u);
+      }
+      if (i > 0) {
+#pragma unroll 1
+        for (int d = 0; d < DH; d += 16) {
+          uint32_t o[16];
+          tmem_ld16(t_row + kColO + d, o);
+          wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+          tmem_st16(t_row + kColO + d, o);
+        }
+        wait_st();
+      }
+    }
+    sum += part;
+    if (!kAlias && c == 0) {
+      fence_before();
+      mbar_arrive(&sm->s_free[wg]);
+    }
+    tmem_st16(t_row + kColP + 16 * c, pk);
+  }
+  l = fmaf(sum, unlift, l);
+  wait_st();
+  fence_before();
+  mbar_arrive(&sm->p_full[wg]);
+  return ok;
 }
 
 template <int DH>
 __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnArgs a, long long wait_cycles, int drop_commits) {
-  constexpr bool kAlias = DH == 64;                  // P in the columns of S
-  constexpr uint32_t kColP = kAlias ? 0 : BN, kColO = kAlias ? BN : BN + BN / 2, kColsWg = kTmemCols / 2;
+  constexpr bool kAlias = Plan<DH>::kAlias;
+  constexpr uint32_t kColP = Plan<DH>::kColP, kColO = Plan<DH>::kColO, kColsWg = Plan<DH>::kColsWg;
   constexpr int KS = DH / 16, P = DH + 2, KB = DH * 2;
   extern __shared__ uint8_t smem_raw[];
   using S = TcSmem<DH>;
   S* sm = reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // the warp's number from its first lane: what follows from it is then known to be the same for all lanes, and an MMA takes
+  // its operands from uniform registers as they are
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int rank = (int)(blockIdx.x % a.splits);
   const long unit = blockIdx.x / a.splits;
   const int H = a.c.n_heads, row0 = (int)(unit % a.tiles) * BM, h = (int)(unit / a.tiles % H);
@@ -218,112 +359,138 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  float vmax = 0.0f;                                  // largest value scale of the context
-  for (int i = tid; i < held; i += kThreads) vmax = fmaxf(vmax, scales[i].y);
+  // largest value scale of the context, and whether a scale is not a number (what attends to such a block is not, either)
+  float vmax = 0.0f;
+  bool bad_k = false, bad_v = false;
+  for (int i = tid; i < held; i += kThreads) {
+    const float2 sc = scales[i];
+    vmax = fmaxf(vmax, sc.y);
+    bad_k |= sc.x != sc.x;
+    bad_v |= sc.y != sc.y;
+  }
   vmax = warp_max(vmax);
   if (lane == 0) sm->vmax[warp] = vmax;
   fence_before();
-  __syncthreads();
+  bad_k = __syncthreads_or(bad_k);
+  bad_v = __syncthreads_or(bad_v);
   fence_after();
   const uint32_t tmem = sm->tmem_base;
 
   bool ok = true;
-  float m = -CUDART_INF_F, l = 0.0f, poison = 0.0f;
+  float m = -CUDART_INF_F, l = 0.0f, vref = 0.0f;
   const int wg = warp >> 2, row = tid & (BM - 1);     // softmax threads
   const uint32_t t_row = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (wg & 1) * kColsWg;
   const int steps = wg < 2 ? (nb - wg + 1) / 2 : 0;   // blocks of the warpgroup
 
   if (warp >= 10) {
     // ------------------------------ MMA issuers ------------------------------
+    // The whole warp walks and waits, one lane issues.
     const int w = warp - 10, n = (nb - w + 1) / 2;
-    if (lane == 0 && n > 0) {
-      const uint32_t t_wg = tmem + w * kColsWg, q_addr = smem_u32(sm->q);
-      ok = mbar_wait(&sm->q_full, 0, ctl);
-      const auto scores = [&](int i) {                // S = Q . K^T of step i
-        const int j = 2 * i + w, st = j % kStages;
-        if (!mbar_wait(&sm->kv_full[st], (j / kStages) & 1, ctl)) return false;
-        fence_after();
-        const uint32_t k_addr = smem_u32(sm->k[st]);
+    const uint32_t t_wg = tmem + w * kColsWg, q_addr = smem_u32(sm->q);
+    const auto wait = [&](uint64_t* bar, uint32_t parity) {
+      const bool done = __all_sync(0xffffffffu, mbar_wait(bar, parity, ctl));
+      if (done) fence_after();
+      return done;
+    };
+    const auto scores = [&](int i) {                  // S = Q . K^T of step i
+      const int j = 2 * i + w, st = j % kStages;
+      if (!wait(&sm->kv_full[st], (j / kStages) & 1)) return false;
+      const uint32_t k_addr = smem_u32(sm->k[st]);
+      if (elected()) {
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
           umma_ss(t_wg, tile_desc<KB>(q_addr + 32 * ks), tile_desc<KB>(k_addr + 32 * ks), idesc(BM, BN), ks);
         if (!drop_commits) umma_commit(&sm->s_full[w]);
-        return true;
-      };
-      ok = ok && scores(0);
-      for (int i = 0; ok && i < n; ++i) {
-        const int st = (2 * i + w) % kStages;
-        if (!kAlias && i + 1 < n) {                   // the next scores, as soon as these are in registers
-          ok = mbar_wait(&sm->s_free[w], i & 1, ctl);
-          if (ok) fence_after();
-          ok = ok && scores(i + 1);
-          if (!ok) break;
-        }
-        ok = mbar_wait(&sm->p_full[w], i & 1, ctl);
+      }
+      __syncwarp();
+      return true;
+    };
+    if (n > 0) ok = wait(&sm->q_full, 0) && scores(0);
+    for (int i = 0; ok && i < n; ++i) {
+      const int st = (2 * i + w) % kStages;
+      if (!kAlias && i + 1 < n) {                     // the next scores, as soon as these are in registers
+        ok = wait(&sm->s_free[w], i & 1) && scores(i + 1);
         if (!ok) break;
-        fence_after();
-        const uint32_t v_addr = smem_u32(sm->v[st]);
+      }
+      ok = wait(&sm->p_full[w], i & 1);
+      if (!ok) break;
+      const uint32_t v_addr = smem_u32(sm->v[st]);
+      if (elected()) {
 #pragma unroll
         for (int ks = 0; ks < BN / 16; ++ks)
           umma_ts(t_wg + kColO, t_wg + kColP + 8 * ks, tile_desc<128>(v_addr + 32 * ks), idesc(BM, DH), i > 0 || ks > 0);
         umma_commit(&sm->o_full[w]);
         umma_commit(&sm->kv_empty[st]);
-        if (kAlias && i + 1 < n) {                    // P lies where the next scores go
-          ok = mbar_wait(&sm->o_full[w], i & 1, ctl);
-          if (ok) fence_after();
-          ok = ok && scores(i + 1);
-        }
       }
+      __syncwarp();
+      if (kAlias && i + 1 < n)                        // P lies where the next scores go
+        ok = wait(&sm->o_full[w], i & 1) && scores(i + 1);
     }
-    __syncwarp();
   } else if (warp >= 8) {
     // ------------------------- codes into operand tiles -------------------------
     const int ct = tid - 256;
-    uint4 rk[KS], rv[KS];
-    const auto load = [&](int j) {
-      const uint4* src = reinterpret_cast<const uint4*>(codes + (size_t)(rank + j * a.splits) * (2 * kCacheBlock * DH));
+    uint32_t k_at[KS], v_at[KS];                      // where a thread's pieces begin in a tile
 #pragma unroll
-      for (int i = 0; i < KS; ++i) {
-        rk[i] = src[ct + i * kConvert];
-        rv[i] = src[kCacheBlock * DH / 16 + ct + i * kConvert];
+    for (int i = 0; i < KS; ++i) {
+      const int u = ct + i * kConvert;
+      k_at[i] = swizzled<KB>(u / KS, u % KS * 2);
+      v_at[i] = swizzled<128>(u / 4, 0) + 4 * (u % 4);
+    }
+    // a thread copies the pieces that it turns itself, three blocks ahead: no other thread waits for them
+    const auto fetch = [&](int j) {
+      if (j < nb) {
+        const uint8_t* src = codes + (size_t)(rank + j * a.splits) * (2 * kCacheBlock * DH);
+        const uint32_t dst = smem_u32(sm->raw[j % kAhead]);
+#pragma unroll
+        for (int i = 0; i < 2 * KS; ++i) cache_cp16(dst + (ct + i * kConvert) * 16, src + (ct + i * kConvert) * 16);
       }
+      cp_commit();
     };
-    if (nb > 0) load(0);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) fetch(j);
     for (int j = 0; ok && j < nb; ++j) {
       const int st = j % kStages;
+      cp_wait<kAhead - 1>();
+      uint4 rk[KS], rv[KS];
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        const uint4* from = reinterpret_cast<const uint4*>(sm->raw[j % kAhead]) + ct + i * kConvert;
+        rk[i] = from[0];
+        rv[i] = from[kCacheBlock * DH / 16];
+      }
+      fetch(j + kAhead);
       if (j >= kStages) ok = __all_sync(0xffffffffu, mbar_wait(&sm->kv_empty[st], ((j / kStages) + 1) & 1, ctl));
       if (!ok) break;
+      // the swizzle is an exclusive or of address bits that a tile's base leaves zero
+      const uint32_t k_to = smem_u32(sm->k[st]), v_to = smem_u32(sm->v[st]);
 #pragma unroll
       for (int i = 0; i < KS; ++i) {                  // 16 channels of a key: two chunks
-        const int u = ct + i * kConvert, r = u / KS, c = u % KS * 2;
         const uint32_t w[4] = {rk[i].x, rk[i].y, rk[i].z, rk[i].w};
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          *reinterpret_cast<uint4*>(sm->k[st] + swizzled<KB>(r, c + e)) =
-              make_uint4(codes_to_halves(w[2 * e], false), codes_to_halves(w[2 * e], true),
-                         codes_to_halves(w[2 * e + 1], false), codes_to_halves(w[2 * e + 1], true));
+          st_shared16((k_to + k_at[i]) ^ (16 * e),
+                      make_uint4(codes_to_halves(w[2 * e], false), codes_to_halves(w[2 * e], true),
+                                 codes_to_halves(w[2 * e + 1], false), codes_to_halves(w[2 * e + 1], true)));
       }
 #pragma unroll
       for (int i = 0; i < KS; ++i) {                  // 16 places of a value channel: rows 16 s + 8 h + 2 t + {0, 1}
-        const int u = ct + i * kConvert, d = u / 4, t = u % 4;
         const uint32_t w[4] = {rv[i].x, rv[i].y, rv[i].z, rv[i].w};
 #pragma unroll
         for (int s = 0; s < 4; ++s)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            *reinterpret_cast<uint32_t*>(sm->v[st] + swizzled<128>(d, 2 * s + e) + 4 * t) = codes_to_halves(w[s], e);
+          for (int e = 0; e < 2; ++e) st_shared4((v_to + v_at[i]) ^ (32 * s + 16 * e), codes_to_halves(w[s], e));
       }
-      if (j + 1 < nb) load(j + 1);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(&sm->kv_full[st]);
     }
+    cp_wait<0>();
   } else {
     // --------------------------------- softmax ---------------------------------
     vmax = 0.0f;
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) vmax = fmaxf(vmax, sm->vmax[w]);
-    // a quotient by vmax as a product: both sides lifted where the scale is small
-    const float big = vmax < 1.0f ? 1.152921504606846976e18f : 1.0f, vinv = vmax > 0.0f ? 1.0f / (vmax * big) : 0.0f;
+    const float vinv = fminf(1.0f / vmax, 3e38f);     // relative to vref = 1 / vinv, which is vmax unless that is subnormal
+    vref = 1.0f / vinv;
     float f;
     {
       float x[DH];
@@ -357,79 +524,13 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
       const float2 sc = next;
       if (i + 1 < steps) next = scales[blk + 2 * a.splits];
       const int live = len - blk * kCacheBlock;
-      float ratio = sc.y * big * vinv;
-      if (ratio != ratio) poison = sc.y, ratio = 1.0f;
-      ratio = fmaxf(ratio, kLeastRatio);
-      const float lift = kLiftTc + __log2f(ratio), unlift = __frcp_rn(ratio);
-      const float x = f * sc.x, slope = !(x <= 1e-37f) ? x : 1e-37f;
+      const float ratio = fmaxf(sc.y * vinv, kLeastRatio), lift = kLiftTc + lg2(ratio), unlift = rcp(ratio);
+      const float slope = fmaxf(f * sc.x, 1e-37f);    // never 0: scores that are not finite stay so
       ok = __all_sync(0xffffffffu, mbar_wait(&sm->s_full[wg], i & 1, ctl));
       if (!ok) break;
       fence_after();
-      uint32_t r[32];
-      float top = -CUDART_INF_F;
-#pragma unroll 1
-      for (int c = 0; c < 2; ++c) {
-        tmem_ld32(t_row + 32 * c, r);
-        wait_ld();
-        if (live < BN) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (32 * c + e < live) top = fmaxf(top, __uint_as_float(r[e]));
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) top = fmaxf(top, fmaxf(__uint_as_float(r[e]), __uint_as_float(r[e + 1])));
-        }
-      }
-      top *= slope;
-      const bool raise = !(top <= m + kLag);
-      const float alpha = raise ? ex2(m - top) : 1.0f;
-      if (raise) m = top;
-      const float2 sl2 = make_float2(slope, slope), add2 = make_float2(lift - m, lift - m);
-      float2 sum = make_float2(0.0f, 0.0f);
-#pragma unroll 1
-      for (int c = 0; c < 2; ++c) {
-        uint32_t pk[16];
-        tmem_ld32(t_row + 32 * c, r);
-        wait_ld();
-        if (!kAlias && c == 1) {
-          fence_before();
-          mbar_arrive(&sm->s_free[wg]);
-        }
-#pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          float2 y = pk_fma(make_float2(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), sl2, add2);
-          if (((e >> 1) & 7) < ARTAB_CACHE_POLY_OF_8)
-            y = ex2_fma(y);
-          else
-            y = make_float2(ex2(y.x), ex2(y.y));
-          if (live < BN) {
-            if (32 * c + e >= live) y.x = 0.0f;
-            if (32 * c + e + 1 >= live) y.y = 0.0f;
-          }
-          sum = pk_add(sum, y);
-          pk[e >> 1] = h2_bits(__floats2half2_rn(y.x, y.y));
-        }
-        if (c == 0 && i > 0) {                        // the P . V before this one has read P and written O
-          if (!kAlias) ok = __all_sync(0xffffffffu, mbar_wait(&sm->o_full[wg], (i - 1) & 1, ctl));
-          fence_after();
-          if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll 1
-            for (int d = 0; d < DH; d += 16) {
-              uint32_t o[16];
-              tmem_ld16(t_row + kColO + d, o);
-              wait_ld();
-#pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-              tmem_st16(t_row + kColO + d, o);
-            }
-          }
-        }
-        tmem_st16(t_row + kColP + 16 * c, pk);
-      }
-      l = fmaf(l, alpha, (sum.x + sum.y) * unlift);
-      wait_st();
-      fence_before();
-      mbar_arrive(&sm->p_full[wg]);
+      ok = live < BN ? softmax_block<DH, true>(sm, t_row, wg, i, slope, lift, unlift, live, m, l)
+                     : softmax_block<DH, false>(sm, t_row, wg, i, slope, lift, unlift, BN, m, l);
       if (!ok) break;
     }
     if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sm->o_full[wg], (steps - 1) & 1, ctl));
@@ -458,9 +559,9 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
   if (wg < 2) {
     float* to = part + (wg * BM + row) * P;
 #pragma unroll
-    for (int d = 0; d < DH; ++d) to[d] = __uint_as_float(o[d]) * vmax + poison;
+    for (int d = 0; d < DH; ++d) to[d] = bad_k || bad_v ? CUDART_NAN_F : __uint_as_float(o[d]) * vref;
     to[DH] = m;
-    to[DH + 1] = gave_up ? CUDART_NAN_F : l;
+    to[DH + 1] = gave_up || bad_k ? CUDART_NAN_F : l;
   }
   if (a.splits == 1)
     __syncthreads();

@@ -366,6 +366,29 @@ def test_values_that_are_not_finite_leave_the_weights_sound(dtype, B):
     check_attention(c.context_cache_attention(q, cache), attention(q, cache, 32 ** -0.5), dtype, 32)
 
 
+@pytest.mark.parametrize("D", [16, 32, 64])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_scores_that_rise_from_block_to_block_and_within(dtype, D):
+    """Keys along one direction, longer from row to row, in steps far beyond the range of a half-precision numerator, up, down
+    and in between; half of the queries point the other way."""
+    c = cc()
+    g = gen(36)
+    N, B, H = 700, 200, 4
+    axis = torch.randn(D, device="cuda", generator=g)
+    axis = axis / axis.norm()
+    n = torch.arange(N, device="cuda").float()
+    length = torch.stack([n / 4, 175 - n / 4, 40 * torch.sin(n / 20), torch.where(n % 64 < 32, 0.0, n / 8)])       # [H,N]
+    k = (length[None, :, :, None] * axis + 0.1 * torch.randn(1, H, N, D, device="cuda", generator=g)).to(dtype)
+    v = torch.randn(1, H, N, D, device="cuda", generator=g).to(dtype)
+    sign = torch.where(torch.arange(B, device="cuda") % 2 == 0, 1.0, -1.0)[:, None, None, None]
+    q = (sign * axis * (0.5 + torch.rand(B, H, 1, 1, device="cuda", generator=g)) * D ** 0.5
+         + 0.1 * torch.randn(B, H, 1, D, device="cuda", generator=g)).to(dtype)
+    cache = c.quantize_context(k, v)
+    check_attention(c.context_cache_attention(q, cache), attention(q, cache, D ** -0.5), dtype, D)
+    few = c.context_cache_attention(q[:3], cache)
+    check_attention(few, attention(q[:3], cache, D ** -0.5), dtype, D)
+
+
 @pytest.mark.parametrize("B", [3, 130])
 def test_queries_by_strides_and_odd_addresses(B):
     c = cc()
