@@ -78,7 +78,8 @@ _SIGNATURES = {
     "artab_cache_read": (_i, [_i, _p, _p, _i, _p, _p, _p]),
     "artab_cache_attention": (_i, [_i, _p, _p, _i, _i, _p, _i, C.c_float, _p, _p, _p]),
     "artab_cache_select": (_i, [_i, _p, _p, _i, _i, _p, _i, _i, _p, _p]),
-    "artab_cache_block_attention": (_i, [_i, _p, _p, _i, _i, _p, _p, _i, C.c_float, _p, _p, _p]),
+    "artab_cache_block_workspace": (C.c_int64, [_p, _i, _i, _i]),
+    "artab_cache_block_attention": (_i, [_i, _p, _p, _i, _i, _p, _p, _i, C.c_float, _p, _p, _p, C.c_int64, _p]),
     "artab_embed": (_i, [C.POINTER(Model), _p, _p, _p, _i, _i, _i, _p, _p]),
     "artab_head_logpdf": (_i, [C.POINTER(Model), _p, _p, _i, _p, _p]),
     "artab_head_sample": (_i, [C.POINTER(Model), _p, _p, _p, _i, _p, _p, _p, _p]),

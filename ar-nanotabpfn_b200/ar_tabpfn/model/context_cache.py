@@ -311,7 +311,9 @@ def block_context_attention(q: Tensor, cache: ContextCache, blocks: Tensor,
         blocks = blocks.contiguous()
         q, at, strides = _strided(q)
         with _Launch(device) as (lib, stream):
+            need = lib.artab_cache_block_workspace(cache._ref, B, Lq, shape[3])
+            ws = q.new_empty(need, dtype=torch.uint8) if need else None
             _lib.check(lib.artab_cache_block_attention(code, at, strides, B, Lq, cache._ref, blocks.data_ptr(), shape[3],
                                                        Dh ** -0.5 if scale is None else float(scale), out.data_ptr(),
-                                                       lse.data_ptr(), stream))
+                                                       lse.data_ptr(), _address(ws), need, stream))
     return out, lse

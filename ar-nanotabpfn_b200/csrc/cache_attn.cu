@@ -13,161 +13,15 @@
 // walks blocks of its own with a running maximum; its ring of records is filled by 16-byte asynchronous copies
 // and no warp waits for another until the end, where the warps of a CTA and the CTAs of a cluster (up to eight
 // share the rows of a context) merge maximum, sum and output through shared memory.
-#include "cache_attn.cuh"
+#include "cache_tile.cuh"
 
 namespace artab {
 namespace {
 
 constexpr int kWarps = 8;
 
-// numerators are 2^14 times exp(s - max): halves keep 11 bits of them down to 2^-28 of the largest
-constexpr float kLift = 14.0f;
 // query rows of a group from which the row tiles are taken (fp32: half as many)
 constexpr int kManyRows = 96;
-
-template <int DH, int PARTS>
-struct Tile {
-  static constexpr int KS = DH / 16;      // k steps of a score, 16-channel tiles of the output
-  static constexpr int R = 3 - PARTS;     // query rows of a thread
-  static constexpr int ROWS = 8 / PARTS;
-  uint32_t q[KS][2];
-  float f[R];                             // score units to log2
-  float m[R], l[R], o[KS][2][R];          // o: channels 16 md + g, 16 md + 8 + g of the thread's rows
-
-  __device__ __forceinline__ void reset() {
-#pragma unroll
-    for (int r = 0; r < R; ++r) m[r] = -CUDART_INF_F, l[r] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < KS; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int r = 0; r < R; ++r) o[i][j][r] = 0.0f;
-  }
-
-  // `row`: this thread's row of the query fragment (row g / PARTS of the tile), or null
-  template <typename T>
-  __device__ __forceinline__ void load_queries(const T* row, bool vec, float scale_log2) {
-    constexpr int NE = DH / 4;
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    float x[NE];
-#pragma unroll
-    for (int i = 0; i < NE; ++i) x[i] = 0.0f;
-    if (row) load_elements<T, NE>(row + t * NE, vec, x);
-    float top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NE; ++i) top = fmaxf(top, fabsf(x[i]));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    float to, back;
-    row_scale(top, to, back);
-    back *= scale_log2;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      __half2 p[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float a = x[4 * s + 2 * j] * to, b = x[4 * s + 2 * j + 1] * to;
-        p[j] = __floats2half2_rn(a, b);
-        if (PARTS == 2 && (g & 1)) p[j] = __floats2half2_rn(a - __low2float(p[j]), b - __high2float(p[j]));
-      }
-      q[s][0] = h2_bits(p[0]);
-      q[s][1] = h2_bits(p[1]);
-    }
-#pragma unroll
-    for (int r = 0; r < R; ++r) f[r] = __shfl_sync(0xffffffffu, back, PARTS == 2 ? 8 * t : 8 * t + 4 * r);
-  }
-
-  // one block: record in shared memory, its scales, its rows in use (1 .. 64)
-  __device__ __forceinline__ void block(const uint8_t* rec, float ks, float vs, int live) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    float x[4][2][R];                     // scores of rows 16 mt + g, 16 mt + 8 + g
-    float mx[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) mx[r] = m[r];
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      uint32_t wa[KS], wb[KS];
-      load_codes(rec + (16 * mt + g) * DH + t * (DH / 4), wa);
-      load_codes(rec + (16 * mt + 8 + g) * DH + t * (DH / 4), wb);
-#pragma unroll
-      for (int s = 0; s < KS; ++s)
-        mma_f16(c, codes_to_halves(wa[s], false), codes_to_halves(wb[s], false), codes_to_halves(wa[s], true),
-                codes_to_halves(wb[s], true), q[s][0], q[s][1]);
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          float s = (PARTS == 2 ? c[2 * j] + c[2 * j + 1] : c[2 * j + r]) * (f[r] * ks);
-          if (live < kCacheBlock && 16 * mt + 8 * j + g >= live) s = -CUDART_INF_F;
-          x[mt][j][r] = s;
-          mx[r] = fmaxf(mx[r], s);
-        }
-    }
-    float alpha[R], ref[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], o));
-      const float base = mx[r] == -CUDART_INF_F ? 0.0f : mx[r];
-      alpha[r] = ex2(m[r] - base);
-      m[r] = mx[r];
-      ref[r] = base - kLift;
-      l[r] *= alpha[r];
-    }
-    uint32_t p[4][2];
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float e[R];
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          e[r] = ex2(x[mt][j][r] - ref[r]);
-          l[r] += e[r];
-        }
-        __half2 u;
-        if constexpr (PARTS == 2) {
-          const __half hi = __float2half_rn(e[0]);
-          u = __halves2half2(hi, __float2half_rn(e[0] - __half2float(hi)));
-        } else {
-          u = __floats2half2_rn(e[0], e[R - 1]);
-        }
-        p[mt][j] = transpose_8x8(h2_bits(u));
-      }
-    const uint8_t* vals = rec + kCacheBlock * DH;
-#pragma unroll
-    for (int md = 0; md < KS; ++md) {
-      const uint4 a = *reinterpret_cast<const uint4*>(vals + (16 * md + g) * kCacheBlock + 16 * t);
-      const uint4 b = *reinterpret_cast<const uint4*>(vals + (16 * md + 8 + g) * kCacheBlock + 16 * t);
-      const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};
-      float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-        mma_f16(c, codes_to_halves(wa[s], false), codes_to_halves(wb[s], false), codes_to_halves(wa[s], true),
-                codes_to_halves(wb[s], true), p[s][0], p[s][1]);
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-          o[md][j][r] = fmaf(o[md][j][r], alpha[r], vs * (PARTS == 2 ? c[2 * j] + c[2 * j + 1] : c[2 * j + r]));
-    }
-  }
-
- private:
-  static __device__ __forceinline__ void load_codes(const uint8_t* p, uint32_t (&w)[KS]) {
-    if constexpr (KS == 1) {
-      w[0] = *reinterpret_cast<const uint32_t*>(p);
-    } else if constexpr (KS == 2) {
-      const uint2 v = *reinterpret_cast<const uint2*>(p);
-      w[0] = v.x, w[1] = v.y;
-    } else {
-      const uint4 v = *reinterpret_cast<const uint4*>(p);
-      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-    }
-  }
-};
 
 template <int DH>
 struct Ring {
@@ -687,8 +541,8 @@ int by_form(AttnArgs& a, long blocks, cudaStream_t s) {
 }
 
 int attention(int dtype, const void* q, const int64_t* strides, int n_streams, int n_q, const artab_cache* c,
-              int max_len, const int32_t* list, int n_list, float scale, void* out, float* lse, cudaStream_t s,
-              const char* what) {
+              int max_len, const int32_t* list, int n_list, float scale, void* out, float* lse, void* workspace,
+              cudaStream_t s, const char* what) {
   int rc = check_cache(c, what);
   if (rc) return rc;
   rc = check_queries(dtype, q, n_streams, n_q, c, what);
@@ -708,6 +562,7 @@ int attention(int dtype, const void* q, const int64_t* strides, int n_streams, i
   a.out = out;
   a.lse = lse;
   a.units = list ? (long)n_streams * c->n_heads * n_q : (long)c->n_groups * c->n_heads;
+  if (workspace) return launch_cache_by_block(dtype, a, workspace, s);
   const long blocks = list ? n_list : (max_len + kCacheBlock - 1L) / kCacheBlock;
   a.splits = 1;
   a.per_cta = 1;
@@ -741,16 +596,28 @@ extern "C" {
 
 int artab_cache_attention(int dtype, const void* q, const int64_t* q_strides, int n_streams, int n_q,
                           const artab_cache* c, int max_len, float scale, void* out, float* lse, void* stream) {
-  return attention(dtype, q, q_strides, n_streams, n_q, c, max_len, nullptr, 0, scale, out, lse, (cudaStream_t)stream,
-                   "cache_attention");
+  return attention(dtype, q, q_strides, n_streams, n_q, c, max_len, nullptr, 0, scale, out, lse, nullptr,
+                   (cudaStream_t)stream, "cache_attention");
+}
+
+int64_t artab_cache_block_workspace(const artab_cache* c, int n_streams, int n_q, int n_list) {
+  if (check_cache(c, "cache_block_workspace") || n_streams < 1 || n_q < 1 || n_list < 1) return 0;
+  return by_block_workspace(c, n_streams, n_q, n_list);
 }
 
 int artab_cache_block_attention(int dtype, const void* q, const int64_t* q_strides, int n_streams, int n_q,
                                 const artab_cache* c, const int32_t* blocks, int n_list, float scale, void* out,
-                                float* lse, void* stream) {
+                                float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
   ARTAB_REQUIRE(blocks && n_list >= 1, ARTAB_EINVAL, "cache_block_attention: no blocks");
-  return attention(dtype, q, q_strides, n_streams, n_q, c, 0, blocks, n_list, scale, out, lse, (cudaStream_t)stream,
-                   "cache_block_attention");
+  int rc = check_cache(c, "cache_block_attention");
+  if (rc) return rc;
+  rc = check_queries(dtype, q, n_streams, n_q, c, "cache_block_attention");
+  if (rc) return rc;
+  const int64_t need = by_block_workspace(c, n_streams, n_q, n_list);
+  ARTAB_REQUIRE(!need || !workspace || workspace_bytes >= need, ARTAB_ECAPACITY, "cache_block_attention: workspace too small");
+  ARTAB_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, ARTAB_EINVAL, "cache_block_attention: workspace must be 16-byte aligned");
+  return attention(dtype, q, q_strides, n_streams, n_q, c, 0, blocks, n_list, scale, out, lse, need ? workspace : nullptr,
+                   (cudaStream_t)stream, "cache_block_attention");
 }
 
 }  // extern "C"

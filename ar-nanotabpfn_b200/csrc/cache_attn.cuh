@@ -30,6 +30,8 @@ constexpr int kSms = 148;
 constexpr float kLeastRatio = 9.5367431640625e-7f;
 
 int launch_cache_attn_tc(const AttnArgs& a, cudaStream_t s);
+int64_t by_block_workspace(const artab_cache* c, int n_streams, int n_q, int n_list);
+int launch_cache_by_block(int dtype, const AttnArgs& a, void* workspace, cudaStream_t s);
 
 __device__ __forceinline__ void cluster_meet() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");

@@ -409,10 +409,13 @@ ARTAB_API int artab_cache_select(int dtype, const void* q, const int64_t* q_stri
                                  const artab_cache* c, int max_len, int n_pick, int32_t* index, void* stream);
 
 /* artab_cache_attention over the rows of the blocks that blocks [B][H][Lq][n_list] int32 lists for every query: an index
- * that is no block in use counts for nothing, one that is listed twice counts twice. */
+ * that is no block in use counts for nothing, one that is listed twice counts twice.
+ * artab_cache_block_workspace: bytes of workspace (16-byte aligned) with which many queries of one context are worked
+ * on block by block, 0 where that does not pay; without it (NULL) every query takes its blocks one by one. */
+ARTAB_API int64_t artab_cache_block_workspace(const artab_cache* c, int n_streams, int n_q, int n_list);
 ARTAB_API int artab_cache_block_attention(int dtype, const void* q, const int64_t* q_strides, int n_streams, int n_q,
                                           const artab_cache* c, const int32_t* blocks, int n_list, float scale,
-                                          void* out, float* lse, void* stream);
+                                          void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Embedder: out[r][:] = mean_F(x[r][:]) * wx + bx (+ y[r] * wy + by) + marker[kind] (+ ar_tokens[ar_idx[r]]).
  *   x [rows][F], y [rows] or NULL, ar_idx [rows] or NULL.

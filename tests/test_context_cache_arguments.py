@@ -181,7 +181,8 @@ def test_the_library_refuses_what_does_not_fit_without_a_device():
         assert lib.artab_cache_read(0, r, None, 4, p, p, None) == -1
         assert lib.artab_cache_attention(0, p, st, 2, 1, r, 0, 1.0, p, p, None) == -1
         assert lib.artab_cache_select(0, p, st, 2, 1, r, 0, 1, p, None) == -1
-        assert lib.artab_cache_block_attention(0, p, st, 2, 1, r, p, 1, 1.0, p, p, None) == -1
+        assert lib.artab_cache_block_attention(0, p, st, 2, 1, r, p, 1, 1.0, p, p, None, 0, None) == -1
+        assert lib.artab_cache_block_workspace(r, 4096, 2, 64) == 0
     r = C.byref(good())
     assert lib.artab_cache_write(7, p, st, p, st, 4, None, None, 1, r, None) == -1
     assert lib.artab_cache_write(0, None, st, p, st, 4, None, None, 1, r, None) == -1
@@ -198,6 +199,11 @@ def test_the_library_refuses_what_does_not_fit_without_a_device():
     assert lib.artab_cache_attention(0, p, st, 2, 1, r, 0, 1.0, None, p, None) == -1
     assert lib.artab_cache_select(0, p, st, 2, 1, r, 0, 0, p, None) == -1
     assert lib.artab_cache_select(0, p, st, 2, 1, C.byref(good(n_blocks=3457)), 0, 1, p, None) == -1
-    assert lib.artab_cache_block_attention(0, p, st, 2, 1, r, None, 1, 1.0, p, p, None) == -1
-    assert lib.artab_cache_block_attention(0, p, st, 2, 1, r, p, 0, 1.0, p, p, None) == -1
+    assert lib.artab_cache_block_attention(0, p, st, 2, 1, r, None, 1, 1.0, p, p, None, 0, None) == -1
+    assert lib.artab_cache_block_attention(0, p, st, 2, 1, r, p, 0, 1.0, p, p, None, 0, None) == -1
+    one = C.byref(good(n_groups=1, n_blocks=16))
+    need = lib.artab_cache_block_workspace(one, 4096, 2, 8)
+    assert need == 4096 * 2 * 2 * 8 * (32 * 4 + 8)
+    assert lib.artab_cache_block_attention(0, p, st, 4096, 2, one, p, 8, 1.0, p, p, p, need - 1, None) == -2
+    assert lib.artab_cache_block_attention(0, p, st, 4096, 2, one, p, 8, 1.0, p, p, p + 4, need, None) == -1
     assert b"cache" in lib.artab_last_error()

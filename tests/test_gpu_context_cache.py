@@ -498,7 +498,8 @@ def times_of(blocks, nb):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
 @pytest.mark.parametrize("case", [(True, 1, 1, 16, 1, 1, 1), (False, 4, 2, 32, 640, 2, 5), (True, 3, 3, 64, 2100, 5, 20),
-                                  (True, 200, 6, 32, 3000, 2, 16), (False, 5, 2, 64, 1300, 1, 64), (True, 2, 1, 32, 5000, 1, 1)], ids=str)
+                                  (True, 200, 6, 32, 3000, 2, 16), (False, 5, 2, 64, 1300, 1, 64), (True, 2, 1, 32, 5000, 1, 1),
+                                  (False, 3, 2, 64, 900, 250, 7), (True, 700, 2, 16, 500, 1, 9), (True, 1, 1, 32, 64, 9000, 1)], ids=str)
 def test_attention_over_listed_blocks(case, dtype):
     """Chosen blocks; any list: none (-1), indices that are no block in use, the same one twice."""
     c = cc()
