@@ -7,12 +7,14 @@
 // yet divided, maximum, sum.  cache_join_kernel merges the entries of a query in the order of its list.  The
 // order in which a CTA finds entries varies, what it computes for an entry does not.
 // 1024 queries x 6 heads x 16 of 256 blocks: 75 us one by one, see kLeastShared for the choice.
+#include <type_traits>
+
 #include "cache_tile.cuh"
 
 namespace artab {
 namespace {
 
-constexpr int kWarps = 8, kThreads = 32 * kWarps, kChunk = 8 * kThreads;   // entries looked at between two rounds of work
+constexpr int kWarps = 8, kThreads = 32 * kWarps, kChunk = 16 * kThreads;   // entries looked at between two rounds of work
 
 struct JoinArgs {
   AttnArgs a;
@@ -49,28 +51,31 @@ __global__ void __launch_bounds__(kThreads) cache_by_block_kernel(const JoinArgs
   const auto offer = [&](int index, int p) {
     if (index == blk) found[atomicAdd(&n_found, 1)] = p;
   };
+  // a thread's entries lie `stride` apart: stream and place of the next one follow from those of this one
+  const int wide = by4 ? 4 : 1, stride = kThreads * wide, step_b = stride / per, step_i = stride % per;
+  int b_at = tid * wide / per, i_at = tid * wide % per;
   for (int e0 = 0;; e0 += kChunk) {
     const bool last = e0 + kChunk >= entries;
-    if (by4) {
-#pragma unroll
-      for (int k = 0; k < kChunk / kThreads / 4; ++k) {
-        const int e = e0 + (k * kThreads + tid) * 4;
-        if (e < entries) {
-          const int p = ((first + e / per) * H + h) * per + e % per;
+    const auto look = [&](auto wide_) {
+      constexpr int W = decltype(wide_)::value;
+#pragma unroll 4
+      for (int e = e0 + tid * W; e < min(e0 + kChunk, entries); e += kThreads * W) {
+        const int p = ((first + b_at) * H + h) * per + i_at;
+        if constexpr (W == 4) {
           const int4 v = *reinterpret_cast<const int4*>(a.list + p);
-          offer(v.x, p), offer(v.y, p + 1), offer(v.z, p + 2), offer(v.w, p + 3);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < kChunk / kThreads; ++k) {
-        const int e = e0 + k * kThreads + tid;
-        if (e < entries) {
-          const int p = ((first + e / per) * H + h) * per + e % per;
+          if (v.x == blk || v.y == blk || v.z == blk || v.w == blk)
+            offer(v.x, p), offer(v.y, p + 1), offer(v.z, p + 2), offer(v.w, p + 3);
+        } else {
           offer(a.list[p], p);
         }
+        b_at += step_b, i_at += step_i;
+        if (i_at >= per) i_at -= per, ++b_at;
       }
-    }
+    };
+    if (by4)
+      look(std::integral_constant<int, 4>());
+    else
+      look(std::integral_constant<int, 1>());
     __syncthreads();
     const int n = n_found, full = last ? n : n / (kWarps * Tl::ROWS) * (kWarps * Tl::ROWS);   // whole rounds for all warps
     for (int r0 = warp * Tl::ROWS; r0 < full; r0 += kWarps * Tl::ROWS) {
@@ -122,13 +127,13 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const JoinArgs j) {
   len = len < 0 ? 0 : len > cap ? cap : len;
   const int held = (len + kCacheBlock - 1) / kCacheBlock;
   float top = -CUDART_INF_F, sum = 0.0f, out = 0.0f;
-#pragma unroll 4
+#pragma unroll 8
   for (int s = 0; s < a.n_list; ++s) {
     const long p = u * a.n_list + s;
     const int index = a.list[p];
-    if (index < 0 || index >= held) continue;
-    const float2 ml = j.ml[p];
-    const float o = j.o[p * DH + d];
+    float2 ml = j.ml[p];
+    float o = j.o[p * DH + d];
+    if (index < 0 || index >= held) ml = make_float2(-CUDART_INF_F, 0.0f), o = 0.0f;   // nothing was written for it
     const float m = fmaxf(top, ml.x), base = m == -CUDART_INF_F ? 0.0f : m;
     const float x = ex2(top - base), y = ex2(ml.x - base);
     sum = fmaf(sum, x, ml.y * y);

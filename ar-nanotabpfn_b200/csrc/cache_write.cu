@@ -108,8 +108,10 @@ __device__ __noinline__ typename Four<T>::Raw load_unaligned(const T* p) {
   for (int j = 0; j < 4; ++j) to[j] = p[j];
   return r;
 }
-template <typename T, int DH>
-__global__ void __launch_bounds__(2 * Half<DH>::N, 768 / (2 * Half<DH>::N)) cache_write_kernel(const WriteArgs a) {
+// FRESH: the whole cache is laid out, several neighbouring blocks a CTA, the rows of the next on their way while one is
+// worked on; else one block a CTA and as many CTAs of an SM as there can be, for latencies that follow one another.
+template <typename T, int DH, bool FRESH>
+__global__ void __launch_bounds__(2 * Half<DH>::N, (FRESH ? 1024 : 1280) / (2 * Half<DH>::N)) cache_write_kernel(const WriteArgs a) {
   using F = Half<DH>;
   using Raw = typename Four<T>::Raw;
   constexpr int C4 = F::C4;
@@ -124,8 +126,9 @@ __global__ void __launch_bounds__(2 * Half<DH>::N, 768 / (2 * Half<DH>::N)) cach
   write_range(a, g, start, end);
   if (a.set_lens && blockIdx.x == 0 && h == 0 && threadIdx.x == 0) a.c.lens[g] = end;
   // the blocks of this CTA: `per_cta` neighbours
-  int blk = (a.fresh ? 0 : start / kCacheBlock) + (int)blockIdx.x * a.per_cta;
-  const int last = blk + a.per_cta < a.c.n_blocks ? blk + a.per_cta : a.c.n_blocks;
+  const int per_cta = FRESH ? a.per_cta : 1;
+  int blk = (FRESH ? 0 : start / kCacheBlock) + (int)blockIdx.x * per_cta;
+  const int last = blk + per_cta < a.c.n_blocks ? blk + per_cta : a.c.n_blocks;
   const size_t rec0 = ((size_t)g * a.c.n_heads + h) * a.c.n_blocks;
   const RowView& src = vals ? a.v : a.k;
   // the rows of a thread's four pieces: of keys 16 apart, of values those of a word
@@ -150,19 +153,19 @@ __global__ void __launch_bounds__(2 * Half<DH>::N, 768 / (2 * Half<DH>::N)) cach
     float* scales = a.c.scales + (rec0 + blk) * 2;
     __half* bounds = reinterpret_cast<__half*>(a.c.bounds) + (rec0 + blk) * 2 * DH;
     if (end <= base) {                               // no row of this block
-      if (!a.fresh) return;
+      if (!FRESH) return;
       if (threadIdx.x < 2) scales[threadIdx.x] = 0.0f;
       if (threadIdx.x < 2 * DH) bounds[threadIdx.x] = __float2half(0.0f);
       continue;
     }
     uint32_t* codes = reinterpret_cast<uint32_t*>(a.c.codes + (rec0 + blk) * (size_t)(2 * kCacheBlock * DH)) + (vals ? kCacheBlock * C4 : 0);
-    const int n_old = start > base ? start - base : 0;     // rows that are there already
+    const int n_old = !FRESH && start > base ? start - base : 0;     // rows that are there already
     const int n_live = end - base < kCacheBlock ? end - base : kCacheBlock;
     Raw raw[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) raw[i] = next[i];
     from += kCacheBlock * src.s2;
-    if (blk + 1 < last) load(blk + 1, from, next);
+    if (FRESH && blk + 1 < last) load(blk + 1, from, next);
     const float was = n_old ? scales[vals] : 0.0f;
     const float top = Four<T>::largest(raw);
     const uint32_t warp_top = __reduce_max_sync(0xffffffffu, __float_as_uint(top));   // NaN above all
@@ -182,14 +185,13 @@ __global__ void __launch_bounds__(2 * Half<DH>::N, 768 / (2 * Half<DH>::N)) cach
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float x[4];
-      Four<T>::values(raw[i], x);
-      w[i] = step > 0.0f ? codes_of(x, step, inv) : 0x80808080u;   // rows that are not new are zeros
-    }
-    if (n_old) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (row0 + (i & 1) * d1 + (i >> 1) * d2 >= n_old) continue;
+      const int row = row0 + (i & 1) * d1 + (i >> 1) * d2;
+      w[i] = 0x80808080u;
+      if (FRESH || (row >= n_old && row < n_live)) {   // of a whole cache, rows that are not in use are zeros
+        float x[4];
+        Four<T>::values(raw[i], x);
+        if (step > 0.0f) w[i] = codes_of(x, step, inv);
+      } else if (row < n_old) {
         w[i] = old[i];
         if (step > was) {
           float y[4];
@@ -349,7 +351,10 @@ template <typename T, int DH>
 struct LaunchWrite {
   static int go(const WriteArgs& a, dim3 grid, cudaStream_t s) {
     count_launch();
-    cache_write_kernel<T, DH><<<grid, 2 * Half<DH>::N, 0, s>>>(a);
+    if (a.fresh)
+      cache_write_kernel<T, DH, true><<<grid, 2 * Half<DH>::N, 0, s>>>(a);
+    else
+      cache_write_kernel<T, DH, false><<<grid, 2 * Half<DH>::N, 0, s>>>(a);
     return check_launch("cache_write");
   }
 };
@@ -414,7 +419,7 @@ int artab_cache_write(int dtype, const void* k, const int64_t* k_strides, const 
   if (nb > c->n_blocks) nb = c->n_blocks;
   // several blocks a CTA once there are many: the rows of the next are on their way while one is worked on
   const long all = nb * c->n_heads * c->n_groups;
-  a.per_cta = (int)(all / (148L * 16) < 1 ? 1 : all / (148L * 16) > 8 ? 8 : all / (148L * 16));
+  a.per_cta = !fresh || all / (148L * 16) < 1 ? 1 : all / (148L * 16) > 8 ? 8 : (int)(all / (148L * 16));
   rc = by_type_and_size<LaunchWrite>(dtype, c->head_dim, a,
                                      dim3((unsigned)((nb + a.per_cta - 1) / a.per_cta), c->n_heads, c->n_groups), s);
   if (rc || a.set_lens) return rc;
