@@ -20,9 +20,6 @@ namespace {
 
 constexpr int kWarps = 8;
 
-// query rows of a group from which the row tiles are taken (fp32: half as many)
-constexpr int kManyRows = 96;
-
 template <int DH>
 struct Ring {
   static constexpr int kRecord = 2 * kCacheBlock * DH;
@@ -211,12 +208,12 @@ struct RowTile {
   static constexpr int MT = 2, NW = 4;
   static constexpr int ROWS = NW * MT * 16 / PARTS;
   static constexpr int kBlockBytes = 2 * kCacheBlock * DH * 2;      // keys and values as halves
-  static constexpr int kSmem = 2 * kBlockBytes > ROWS * (DH + 2) * 4 ? 2 * kBlockBytes : ROWS * (DH + 2) * 4;
+  static constexpr int kSmem = 2 * kBlockBytes > ROWS * kPartial<DH> * 4 ? 2 * kBlockBytes : ROWS * kPartial<DH> * 4;
 };
 template <typename T, int DH, int PARTS>
 __global__ void __launch_bounds__(128, DH == 64 ? 2 : 3) cache_attn_rows_kernel(const AttnArgs a) {
   using RT = RowTile<DH, PARTS>;
-  constexpr int MT = RT::MT, NW = RT::NW, KS = DH / 16, ND = DH / 8, P = DH + 2, R = 3 - PARTS;
+  constexpr int MT = RT::MT, NW = RT::NW, KS = DH / 16, ND = DH / 8, P = kPartial<DH>, R = 3 - PARTS;
   constexpr int KN = 8 / NW, VN = ND > NW ? ND / NW : 1;         // key and value tiles that a warp lays out
   constexpr int KQ = KS >= 2 ? KS / 2 : 1;                       // 16-byte pieces of a lane's key fragments
   constexpr size_t kRecord = 2 * kCacheBlock * DH;
@@ -471,9 +468,7 @@ __global__ void __launch_bounds__(128, DH == 64 ? 2 : 3) cache_attn_rows_kernel(
     __syncthreads();
   else
     cluster_meet();
-  const uint32_t base = smem_u32(part);
-  const auto at = [&](int w, int i) { return a.splits == 1 ? part[i] : ld_cluster(base + i * 4, w); };
-  merge_rows<T, DH>(a, at, a.splits, rank * 32 * NW + tid, a.splits * 32 * NW, RT::ROWS, row0, h, group, kLift);
+  merge_rows<T, DH>(a, smem_u32(part), 1, rank * 32 * NW + tid, a.splits * 32 * NW, RT::ROWS, row0, h, group, kLift);
   if (a.splits > 1) cluster_meet();
 }
 
@@ -496,21 +491,32 @@ int plan_splits(long units, long blocks) {
   while (s < 8 && units * s * 2 <= 2 * kSms && blocks >= 2L * s * kWarps) s *= 2;
   return s;
 }
-// the same for the row tiles: the share of the last wave that is idle, and four blocks' worth of work around each share
-int plan_row_splits(long units, long blocks, int per_sm) {
-  int best = 1;
-  double least = 0.0;
-  for (int s = 1; s <= 8; s *= 2) {
-    const double waves = (double)((units * s + (long)kSms * per_sm - 1) / ((long)kSms * per_sm));
-    const double cost = waves * ((double)((blocks + s - 1) / s) + 4.0);
-    if (s == 1 || cost < least) best = s, least = cost;
-  }
-  return best;
+// Which kernel, and how many CTAs share a unit's blocks: the least of the times that these figures give, in us.  Measured
+// (B200) over 16 - 2048 rows, 1 - 384 contexts x heads and 500 - 32768 context rows.
+//   few rows: start and merge, and the whole GPU's time for a block against one tile of 8 (bf16) or 4 (fp32) rows;
+//   row tiles: one CTA's time for a block when it has an SM to itself and when the SM is full; start and merge of a wave.
+struct Cost {
+  double few, alone, full, start;
+  int per_sm;              // row-tile CTAs of an SM
+};
+constexpr double kFewStart = 4.5, kPerSplit = 0.4;
+template <typename T, int DH>
+constexpr Cost cost_of() {
+  if (sizeof(T) == 2) return DH == 16 ? Cost{0.5e-3, 0.56, 0.75, 8.0, 2} : DH == 32 ? Cost{0.85e-3, 0.62, 0.87, 9.0, 2} : Cost{1.8e-3, 0.73, 1.0, 10.0, 2};
+  return DH == 16 ? Cost{0.43e-3, 0.83, 1.7, 4.0, 3} : DH == 32 ? Cost{0.77e-3, 0.96, 2.0, 4.0, 3} : Cost{1.65e-3, 1.3, 2.3, 5.0, 2};
+}
+double row_tiles_time(const Cost& c, long units, long blocks, int s) {
+  const double ctas = (double)units * s, cap = (double)kSms * c.per_sm;
+  const double waves = ctas < cap ? 1.0 : 0.5 * (ctas / cap + (double)(long)((ctas + cap - 1) / cap));   // CTAs end one by one
+  const double crowd = ctas <= kSms ? 0.0 : ctas >= cap ? 1.0 : (ctas / kSms - 1.0) / (c.per_sm - 1);
+  return waves * ((c.alone + (c.full - c.alone) * crowd) * (double)((blocks + s - 1) / s) + c.start + kPerSplit * s);
 }
 
 template <typename T, int DH>
 int by_form(AttnArgs& a, long blocks, cudaStream_t s) {
   constexpr int kParts = sizeof(T) == 2 ? 1 : 2;
+  constexpr int kRows = kParts == 1 ? 128 : RowTile<DH, kParts>::ROWS;
+  constexpr Cost cost = cost_of<T, DH>();
   const auto tiles = [&a](int rows) { a.tiles = (a.rows + rows - 1) / rows, a.units *= a.tiles; };
   if (a.list) {
     // as many warps share a list as leave each two blocks, fewer where the lists alone fill the GPU
@@ -520,15 +526,22 @@ int by_form(AttnArgs& a, long blocks, cudaStream_t s) {
     if (warps == kWarps) a.splits = plan_splits(a.units, blocks);
     return launch<T, DH, 2, true>(a, s);
   }
-  if (kParts == 1 && a.rows >= kManyRows) {
-    tiles(128);
-    a.splits = plan_row_splits(a.units, blocks, 2);
-    return launch_cache_attn_tc(a, s);
-  }
-  if (a.rows >= kManyRows / kParts) {
-    tiles(RowTile<DH, kParts>::ROWS);
-    a.splits = plan_row_splits(a.units, blocks, DH == 64 ? 2 : 3);
-    return launch_rows<T, DH, kParts>(a, s);
+  if (a.rows > 8) {
+    const long units = a.units * ((a.rows + kRows - 1) / kRows);
+    double least = kFewStart + cost.few * (double)(a.units * ((a.rows + 8 / kParts - 1) / (8 / kParts))) * (double)blocks;
+    int splits = 0;
+    for (int n = 1; n <= 8; n *= 2) {
+      const double t = row_tiles_time(cost, units, blocks, n);
+      if (t < least) least = t, splits = n;
+    }
+    if (splits) {
+      tiles(kRows);
+      a.splits = splits;
+      if constexpr (kParts == 1)
+        return launch_cache_attn_tc(a, s);
+      else
+        return launch_rows<T, DH, kParts>(a, s);
+    }
   }
   if (kParts == 1 && a.rows > 4) {
     tiles(8);

@@ -41,29 +41,55 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_rank(addr, rank)) : "memory");
   return v;
 }
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr, uint32_t rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(map_to_rank(addr, rank))
+               : "memory");
+  return v;
+}
 
-// Merges `count` partial results of `rows` query rows (at(w, i): element i of partial result w, [row][DH + 2] = output not
-// yet divided, maximum in log2 units, sum of numerators, which are 2^lift times exp(s - max)) and writes output and
-// log-sum-exp.  The calling thread takes every `step`-th element from `first` on.
-template <typename T, int DH, typename F>
-__device__ __forceinline__ void merge_rows(const AttnArgs& a, F at, int count, int first, int step, int rows, int row0, int h,
-                                           int group, float lift) {
-  constexpr int P = DH + 2;
-  for (int e = first; e < rows * DH; e += step) {
-    const int r = e / DH, d = e % DH, row = row0 + r;
+// A partial result of a query row: output not yet divided, maximum in log2 units, sum of numerators (2^lift times
+// exp(s - maximum)); padded so that four channels are read at once.
+template <int DH>
+constexpr int kPartial = DH + 4;
+
+// Merges the partial results of `rows` query rows and writes output and log-sum-exp: `per_cta` of them lie in every CTA of
+// the cluster, [per_cta][rows][kPartial] from shared-memory address `base` on.  The calling thread takes every `step`-th
+// group of four channels from `first` on.
+template <typename T, int DH>
+__device__ __forceinline__ void merge_rows(const AttnArgs& a, uint32_t base, int per_cta, int first, int step, int rows,
+                                           int row0, int h, int group, float lift) {
+  constexpr int P = kPartial<DH>;
+  const int count = per_cta * a.splits;
+  for (int e = first; e < rows * (DH / 4); e += step) {
+    const int r = e / (DH / 4), d = e % (DH / 4) * 4, row = row0 + r;
     if (row >= a.rows) return;
-    float top = -CUDART_INF_F, sum = 0.0f, out = 0.0f;
-    for (int w = 0; w < count; ++w) top = fmaxf(top, at(w, r * P + DH));
+    const auto at = [&](int w) { return base + (uint32_t)((w % per_cta * rows + r) * P * 4); };
+    float top = -CUDART_INF_F, sum = 0.0f;
+    float4 out = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int w = 0; w < count; ++w) top = fmaxf(top, ld_cluster(at(w) + DH * 4, w / per_cta));
     const float from = top == -CUDART_INF_F ? 0.0f : top;
+#pragma unroll 4
     for (int w = 0; w < count; ++w) {
-      const float x = ex2(at(w, r * P + DH) - from);
-      sum = fmaf(at(w, r * P + DH + 1), x, sum);
-      out = fmaf(at(w, r * P + d), x, out);
+      const float x = ex2(ld_cluster(at(w) + DH * 4, w / per_cta) - from);
+      sum = fmaf(ld_cluster(at(w) + DH * 4 + 4, w / per_cta), x, sum);
+      const float4 o = ld_cluster4(at(w) + d * 4, w / per_cta);
+      out.x = fmaf(o.x, x, out.x), out.y = fmaf(o.y, x, out.y), out.z = fmaf(o.z, x, out.z), out.w = fmaf(o.w, x, out.w);
     }
     const bool one = a.c.n_groups == 1;
     const int b = one ? row / a.n_q : group, l = one ? row % a.n_q : row;
     const size_t to = ((size_t)b * a.c.n_heads + h) * a.n_q + l;
-    reinterpret_cast<T*>(a.out)[to * DH + d] = from_f32<T>(sum == 0.0f ? 0.0f : out / sum);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    T* dst = reinterpret_cast<T*>(a.out) + to * DH + d;
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(dst) = make_float4(out.x * inv, out.y * inv, out.z * inv, out.w * inv);
+    } else {
+      __nv_bfloat162 y[2] = {__floats2bfloat162_rn(out.x * inv, out.y * inv), __floats2bfloat162_rn(out.z * inv, out.w * inv)};
+      *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(y);
+    }
     if (d == 0) a.lse[to] = sum == 0.0f ? -CUDART_INF_F : (top - lift) * kLn2 + logf(sum);
   }
 }

@@ -313,7 +313,7 @@ template <int DH>
 __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnArgs a, long long wait_cycles, int drop_commits) {
   constexpr bool kAlias = Plan<DH>::kAlias;
   constexpr uint32_t kColP = Plan<DH>::kColP, kColO = Plan<DH>::kColO, kColsWg = Plan<DH>::kColsWg;
-  constexpr int KS = DH / 16, P = DH + 2, KB = DH * 2;
+  constexpr int KS = DH / 16, P = kPartial<DH>, KB = DH * 2;
   extern __shared__ uint8_t smem_raw[];
   using S = TcSmem<DH>;
   S* sm = reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -359,6 +359,48 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  // Everything that comes from memory is asked for before the first barrier.
+  const int wg = warp >> 2, row = tid & (BM - 1);     // softmax threads
+  const int ct = tid - 256;                           // converting threads
+  // a converting thread copies the pieces that it turns itself, three blocks ahead: no other thread waits for them
+  const auto fetch = [&](int j) {
+    if (j < nb) {
+      const uint8_t* src = codes + (size_t)(rank + j * a.splits) * (2 * kCacheBlock * DH);
+      const uint32_t dst = smem_u32(sm->raw[j % kAhead]);
+#pragma unroll
+      for (int i = 0; i < 2 * KS; ++i) cache_cp16(dst + (ct + i * kConvert) * 16, src + (ct + i * kConvert) * 16);
+    }
+    cp_commit();
+  };
+  float f = 0.0f;
+  if (wg < 2) {
+    float x[DH];
+#pragma unroll
+    for (int i = 0; i < DH; ++i) x[i] = 0.0f;
+    const int r = row0 + row;
+    if (r < a.rows)
+      load_elements<__nv_bfloat16, DH>(reinterpret_cast<const __nv_bfloat16*>(a.q.p) + stream_of(r) * a.q.s0 + h * a.q.s1 +
+                                           query_of(r) * a.q.s2, a.vec_q, x);
+    float top = 0.0f, to, back;
+#pragma unroll
+    for (int i = 0; i < DH; ++i) top = fmaxf(top, fabsf(x[i]));
+    row_scale(top, to, back);
+    f = back * fabsf(a.scale_log2);
+    to = copysignf(to, a.scale_log2);
+    if (wg == 0) {
+#pragma unroll
+      for (int c = 0; c < DH / 8; ++c) {
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = h2_bits(__floats2half2_rn(x[8 * c + 2 * i] * to, x[8 * c + 2 * i + 1] * to));
+        *reinterpret_cast<uint4*>(sm->q + swizzled<KB>(row, c)) = make_uint4(u[0], u[1], u[2], u[3]);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+  } else if (warp < 10) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) fetch(j);
+  }
   // largest value scale of the context, and whether a scale is not a number (what attends to such a block is not, either)
   float vmax = 0.0f;
   bool bad_k = false, bad_v = false;
@@ -378,7 +420,6 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
 
   bool ok = true;
   float m = -CUDART_INF_F, l = 0.0f, vref = 0.0f;
-  const int wg = warp >> 2, row = tid & (BM - 1);     // softmax threads
   const uint32_t t_row = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (wg & 1) * kColsWg;
   const int steps = wg < 2 ? (nb - wg + 1) / 2 : 0;   // blocks of the warpgroup
 
@@ -428,7 +469,6 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
     }
   } else if (warp >= 8) {
     // ------------------------- codes into operand tiles -------------------------
-    const int ct = tid - 256;
     uint32_t k_at[KS], v_at[KS];                      // where a thread's pieces begin in a tile
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
@@ -436,18 +476,6 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
       k_at[i] = swizzled<KB>(u / KS, u % KS * 2);
       v_at[i] = swizzled<128>(u / 4, 0) + 4 * (u % 4);
     }
-    // a thread copies the pieces that it turns itself, three blocks ahead: no other thread waits for them
-    const auto fetch = [&](int j) {
-      if (j < nb) {
-        const uint8_t* src = codes + (size_t)(rank + j * a.splits) * (2 * kCacheBlock * DH);
-        const uint32_t dst = smem_u32(sm->raw[j % kAhead]);
-#pragma unroll
-        for (int i = 0; i < 2 * KS; ++i) cache_cp16(dst + (ct + i * kConvert) * 16, src + (ct + i * kConvert) * 16);
-      }
-      cp_commit();
-    };
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) fetch(j);
     for (int j = 0; ok && j < nb; ++j) {
       const int st = j % kStages;
       cp_wait<kAhead - 1>();
@@ -491,33 +519,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
     for (int w = 0; w < kThreads / 32; ++w) vmax = fmaxf(vmax, sm->vmax[w]);
     const float vinv = fminf(1.0f / vmax, 3e38f);     // relative to vref = 1 / vinv, which is vmax unless that is subnormal
     vref = 1.0f / vinv;
-    float f;
-    {
-      float x[DH];
-#pragma unroll
-      for (int i = 0; i < DH; ++i) x[i] = 0.0f;
-      const int r = row0 + row;
-      if (r < a.rows)
-        load_elements<__nv_bfloat16, DH>(reinterpret_cast<const __nv_bfloat16*>(a.q.p) + stream_of(r) * a.q.s0 + h * a.q.s1 +
-                                             query_of(r) * a.q.s2, a.vec_q, x);
-      float top = 0.0f, to, back;
-#pragma unroll
-      for (int i = 0; i < DH; ++i) top = fmaxf(top, fabsf(x[i]));
-      row_scale(top, to, back);
-      f = back * fabsf(a.scale_log2);
-      to = copysignf(to, a.scale_log2);
-      if (wg == 0) {
-#pragma unroll
-        for (int c = 0; c < DH / 8; ++c) {
-          uint32_t u[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) u[i] = h2_bits(__floats2half2_rn(x[8 * c + 2 * i] * to, x[8 * c + 2 * i + 1] * to));
-          *reinterpret_cast<uint4*>(sm->q + swizzled<KB>(row, c)) = make_uint4(u[0], u[1], u[2], u[3]);
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_arrive(&sm->q_full);
-      }
-    }
+    if (wg == 0) mbar_arrive(&sm->q_full);
     float2 next = steps > 0 ? scales[rank + wg * a.splits] : make_float2(0.0f, 0.0f);
     for (int i = 0; i < steps; ++i) {
       const int blk = rank + (2 * i + wg) * a.splits;
@@ -537,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
     fence_after();
   }
 
-  // both warpgroups' results where the tiles were: [2][128][DH + 2]
+  // both warpgroups' results where the tiles were: [2][128][kPartial]
   float* part = reinterpret_cast<float*>(sm);
   uint32_t o[DH];
   if (wg < 2) {
@@ -558,8 +560,11 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
   const bool gave_up = ctl->abort_flag != 0;
   if (wg < 2) {
     float* to = part + (wg * BM + row) * P;
+    const float factor = bad_k || bad_v ? CUDART_NAN_F : vref;
 #pragma unroll
-    for (int d = 0; d < DH; ++d) to[d] = bad_k || bad_v ? CUDART_NAN_F : __uint_as_float(o[d]) * vref;
+    for (int d = 0; d < DH; d += 4)
+      *reinterpret_cast<float4*>(to + d) = make_float4(__uint_as_float(o[d]) * factor, __uint_as_float(o[d + 1]) * factor,
+                                                       __uint_as_float(o[d + 2]) * factor, __uint_as_float(o[d + 3]) * factor);
     to[DH] = m;
     to[DH + 1] = gave_up || bad_k ? CUDART_NAN_F : l;
   }
@@ -567,12 +572,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
     __syncthreads();
   else
     cluster_meet();
-  const uint32_t base = smem_u32(part);
-  const auto at = [&](int w, int i) {                 // partial result w: warpgroup w % 2 of CTA w / 2
-    if (a.splits == 1) return part[(w & 1) * BM * P + i];
-    return ld_cluster(base + ((w & 1) * BM * P + i) * 4, w >> 1);
-  };
-  merge_rows<__nv_bfloat16, DH>(a, at, 2 * a.splits, rank * kThreads + tid, a.splits * kThreads, BM, row0, h, group, kLiftTc);
+  merge_rows<__nv_bfloat16, DH>(a, smem_u32(part), 2, rank * kThreads + tid, a.splits * kThreads, BM, row0, h, group, kLiftTc);
   if (a.splits > 1) cluster_meet();
 }
 
@@ -581,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
 template <int DH>
 static int launch_tc(const AttnArgs& a, cudaStream_t s) {
   static SmemConfig config;
-  static_assert(TcSmem<DH>::kFree >= 2 * BM * (DH + 2) * 4, "the merge fits where the tiles were");
+  static_assert(TcSmem<DH>::kFree >= 2 * BM * kPartial<DH> * 4, "the merge fits where the tiles were");
   const long long limit = debug_wait_cycles() ? debug_wait_cycles() : kDefaultWaitCycles;
   return launch_attn(cache_attn_tc_kernel<DH>, config, sizeof(TcSmem<DH>) + 1024, kThreads, a, s, limit, debug_drop_score_commits());
 }
