@@ -33,18 +33,20 @@ constexpr int partial_floats() {
   return Tile<DH, PARTS>::ROWS * (DH + 2);
 }
 
-template <typename T, int DH, int PARTS, bool LIST>
+// FORM 0: every block, a CTA (of a cluster) for a unit; 1: every block, several units a CTA; 2: listed blocks, either way.
+template <typename T, int DH, int PARTS, int FORM>
 __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const AttnArgs a) {
+  constexpr bool LIST = FORM == 2;
   using R = Ring<DH>;
   using Tl = Tile<DH, PARTS>;
   constexpr int ROWS = LIST ? 1 : Tl::ROWS, P = DH + 2;
   extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int rank = (int)(blockIdx.x % a.splits);
-  const int per_cta = LIST ? a.per_cta : 1, warps = kWarps / per_cta;
+  const int per_cta = FORM ? a.per_cta : 1, warps = FORM ? kWarps / per_cta : kWarps;
   long unit = blockIdx.x / a.splits;
-  if (LIST) unit = unit * per_cta + warp / warps;
-  const bool spare = LIST && unit >= a.units;                 // the last CTA may have warps without a unit
+  if (FORM) unit = unit * per_cta + warp / warps;
+  const bool spare = FORM && unit >= a.units;                         // the last CTA may have warps without a unit
   if (spare) unit = a.units - 1;
   const int H = a.c.n_heads;
   int group, h, row0, n_rows;
@@ -76,7 +78,7 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const AttnArgs 
 
   uint8_t* ring = smem + warp * R::kBytes;
   const uint32_t ring_addr = smem_u32(ring);
-  const int first = rank * warps + warp % warps, step = a.splits * warps;
+  const int first = rank * warps + (FORM ? warp % warps : warp), step = a.splits * warps;
   // block to fetch next; -1: nothing there.  Of a list, the lanes keep 32 entries of the warp's share
   int fetched = 0, entries = -1;
   const auto next_block = [&]() {
@@ -172,8 +174,8 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const AttnArgs 
     if (d == 0) a.lse[at] = l == 0.0f ? -CUDART_INF_F : (m - kLift) * kLn2 + logf(l);
   };
   // the threads of a unit's warps write its results
-  const float* of_unit = part + (LIST ? warp / warps * warps : 0) * ROWS * P;
-  for (int e = LIST ? tid % (warps * 32) : tid; e < ROWS * DH; e += warps * 32) {
+  const float* of_unit = part + (FORM ? warp / warps * warps : 0) * ROWS * P;
+  for (int e = FORM ? tid % (warps * 32) : tid; e < ROWS * DH; e += warps * 32) {
     float m, l, o;
     merge([&](int w, int i) { return of_unit[w * ROWS * P + i]; }, warps, e / DH, e % DH, m, l, o);
     if (a.splits == 1) {
@@ -472,12 +474,12 @@ __global__ void __launch_bounds__(128, DH == 64 ? 2 : 3) cache_attn_rows_kernel(
   if (a.splits > 1) cluster_meet();
 }
 
-template <typename T, int DH, int PARTS, bool LIST>
+template <typename T, int DH, int PARTS, int FORM>
 int launch(const AttnArgs& a, cudaStream_t s) {
   static SmemConfig config;
   const size_t part = (size_t)(kWarps + 1) * partial_floats<DH, PARTS>() * sizeof(float);
   const size_t ring = (size_t)kWarps * Ring<DH>::kBytes;
-  return launch_attn(cache_attn_kernel<T, DH, PARTS, LIST>, config, part > ring ? part : ring, kWarps * 32, a, s);
+  return launch_attn(cache_attn_kernel<T, DH, PARTS, FORM>, config, part > ring ? part : ring, kWarps * 32, a, s);
 }
 template <typename T, int DH, int PARTS>
 int launch_rows(const AttnArgs& a, cudaStream_t s) {
@@ -485,11 +487,27 @@ int launch_rows(const AttnArgs& a, cudaStream_t s) {
   return launch_attn(cache_attn_rows_kernel<T, DH, PARTS>, config, RowTile<DH, PARTS>::kSmem, RowTile<DH, PARTS>::NW * 32, a, s);
 }
 
-// CTAs that share the blocks of a unit: as many as fill the GPU twice, none without a block for every warp
-int plan_splits(long units, long blocks) {
-  int s = 1;
-  while (s < 8 && units * s * 2 <= 2 * kSms && blocks >= 2L * s * kWarps) s *= 2;
-  return s;
+// Rounds of work on a GPU that holds `cap` workers at a time: they end one by one, so between the quotient and the whole
+// number above it.
+double rounds(double workers, double cap) {
+  return workers <= cap ? 1.0 : 0.5 * (workers / cap + (double)(long)((workers + cap - 1) / cap));
+}
+// Warps of a unit (fewer than a CTA's: several units a CTA) and CTAs of a unit (a cluster; only whole ones): the least
+// rounds times blocks a warp, start and merge of a round counted as two blocks, each doubling of a cluster as a half, a tenth
+// more for a kernel whose warps and units are not known when it is compiled.
+// 3072 units of 4 blocks: one warp each 20 us, eight 43; 384 of 32: eight or four 18, one 33; 512 of 32 at head size 64: two 29,
+// eight 38.
+void plan_warps(AttnArgs& a, long blocks, int resident_warps) {
+  double least = 0.0;
+  a.splits = 0;
+  for (int warps = 1; warps <= kWarps; warps *= 2)
+    for (int s = 1, extra = 0; s <= (warps == kWarps ? 8 : 1); s *= 2, ++extra) {
+      const long per = (long)warps * s;
+      if (s > 1 && blocks < 2 * per) break;
+      const double t = rounds((double)a.units * per, (double)kSms * resident_warps) *
+                       ((double)((blocks + per - 1) / per) + 2.0 + 0.5 * extra) * (warps < kWarps ? 1.1 : 1.0);
+      if (!a.splits || t <= least) least = t, a.per_cta = kWarps / warps, a.splits = s;
+    }
 }
 // Which kernel, and how many CTAs share a unit's blocks: the least of the times that these figures give, in us.  Measured
 // (B200) over 16 - 2048 rows, 1 - 384 contexts x heads and 500 - 32768 context rows.
@@ -507,9 +525,8 @@ constexpr Cost cost_of() {
 }
 double row_tiles_time(const Cost& c, long units, long blocks, int s) {
   const double ctas = (double)units * s, cap = (double)kSms * c.per_sm;
-  const double waves = ctas < cap ? 1.0 : 0.5 * (ctas / cap + (double)(long)((ctas + cap - 1) / cap));   // CTAs end one by one
   const double crowd = ctas <= kSms ? 0.0 : ctas >= cap ? 1.0 : (ctas / kSms - 1.0) / (c.per_sm - 1);
-  return waves * ((c.alone + (c.full - c.alone) * crowd) * (double)((blocks + s - 1) / s) + c.start + kPerSplit * s);
+  return rounds(ctas, cap) * ((c.alone + (c.full - c.alone) * crowd) * (double)((blocks + s - 1) / s) + c.start + kPerSplit * s);
 }
 
 template <typename T, int DH>
@@ -517,14 +534,11 @@ int by_form(AttnArgs& a, long blocks, cudaStream_t s) {
   constexpr int kParts = sizeof(T) == 2 ? 1 : 2;
   constexpr int kRows = kParts == 1 ? 128 : RowTile<DH, kParts>::ROWS;
   constexpr Cost cost = cost_of<T, DH>();
+  constexpr int kResident = DH == 64 ? 8 : 16;     // warps of an SM, by their rings
   const auto tiles = [&a](int rows) { a.tiles = (a.rows + rows - 1) / rows, a.units *= a.tiles; };
   if (a.list) {
-    // as many warps share a list as leave each two blocks, fewer where the lists alone fill the GPU
-    int warps = kWarps;
-    while (warps > 1 && (2 * warps > a.n_list || a.units * warps > 8L * kWarps * kSms)) warps /= 2;
-    a.per_cta = kWarps / warps;
-    if (warps == kWarps) a.splits = plan_splits(a.units, blocks);
-    return launch<T, DH, 2, true>(a, s);
+    plan_warps(a, blocks, kResident);
+    return launch<T, DH, 2, 2>(a, s);
   }
   if (a.rows > 8) {
     const long units = a.units * ((a.rows + kRows - 1) / kRows);
@@ -543,14 +557,11 @@ int by_form(AttnArgs& a, long blocks, cudaStream_t s) {
         return launch_rows<T, DH, kParts>(a, s);
     }
   }
-  if (kParts == 1 && a.rows > 4) {
-    tiles(8);
-    a.splits = plan_splits(a.units, blocks);
-    return launch<T, DH, kParts, false>(a, s);
-  }
-  tiles(4);
-  a.splits = plan_splits(a.units, blocks);
-  return launch<T, DH, 2, false>(a, s);
+  const bool eight = kParts == 1 && a.rows > 4;
+  tiles(eight ? 8 : 4);
+  plan_warps(a, blocks, kResident);
+  if (a.per_cta == 1) return eight ? launch<T, DH, kParts, 0>(a, s) : launch<T, DH, 2, 0>(a, s);
+  return eight ? launch<T, DH, kParts, 1>(a, s) : launch<T, DH, 2, 1>(a, s);
 }
 
 int attention(int dtype, const void* q, const int64_t* strides, int n_streams, int n_q, const artab_cache* c,
