@@ -138,6 +138,11 @@ __global__ void __launch_bounds__(2 * Half<DH>::N, (FRESH ? 1024 : 1280) / (2 * 
   const int vec = vals ? a.vec_v : a.vec_k;
   const auto load = [&](int b, const T* p, Raw (&raw)[4]) {      // new rows of block b, zeros for the others
     const int lo = start - b * kCacheBlock, hi = end - b * kCacheBlock;
+    if (FRESH && vec && hi >= kCacheBlock) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[i] = *reinterpret_cast<const Raw*>(p + (i & 1) * p1 + (i >> 1) * p2);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = row0 + (i & 1) * d1 + (i >> 1) * d2;
@@ -170,18 +175,24 @@ __global__ void __launch_bounds__(2 * Half<DH>::N, (FRESH ? 1024 : 1280) / (2 * 
     const float top = Four<T>::largest(raw);
     const uint32_t warp_top = __reduce_max_sync(0xffffffffu, __float_as_uint(top));   // NaN above all
     if (lane == 0) s_top[warp] = warp_top;
+    // Codes that are there: of keys all (for the bounds), of values at first only words that new rows go into.
+    const bool mine = row0 < n_live && row0 + d1 + d2 >= n_old;     // may have a new row among its four
     uint32_t old[4] = {0u, 0u, 0u, 0u};
-    if (n_old) {
+    const auto load_old = [&]() {
 #pragma unroll
       for (int i = 0; i < 4; ++i) old[i] = vals ? codes[(c4 * 4 + i) * 16 + word] : codes[(word + 16 * i) * C4 + c4];
       if (vals) turn(old);
-    }
+    };
+    if (n_old && (!vals || mine)) load_old();
     __syncthreads();   // also: every thread has read the old codes and scales
     uint32_t block_top = 0;
 #pragma unroll
     for (int w = 0; w < F::WARPS; ++w) block_top = max(block_top, s_top[(vals ? F::WARPS : 0) + w]);
     // a step of zero (or NaN) has zero codes
     const float step = larger_step(was, step_of(block_top)), inv = 1.0f / step;
+    // rows that stay, at a scale that stays, are not written again
+    const bool stays = !FRESH && n_old > 0 && !(step > was);
+    if (n_old && vals && !mine && !stays) load_old();
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -200,7 +211,13 @@ __global__ void __launch_bounds__(2 * Half<DH>::N, (FRESH ? 1024 : 1280) / (2 * 
         }
       }
     }
-    if (vals) {
+    if (vals && stays) {
+      if (mine) {
+        turn(w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) codes[(c4 * 4 + i) * 16 + word] = w[i];
+      }
+    } else if (vals) {
       turn(w);
 #pragma unroll
       for (int i = 0; i < 4; ++i) s_v[(c4 * 4 + i) * F::VP + word] = w[i];
@@ -211,7 +228,7 @@ __global__ void __launch_bounds__(2 * Half<DH>::N, (FRESH ? 1024 : 1280) / (2 * 
       for (int j = 0; j < 2; ++j) lo[j] = __float2half2_rn(2048.0f), hi[j] = __float2half2_rn(0.0f);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        codes[(word + 16 * i) * C4 + c4] = w[i];
+        if (!stays || row0 + 16 * i >= n_old) codes[(word + 16 * i) * C4 + c4] = w[i];
         if (row0 + 16 * i >= n_live) continue;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -236,6 +253,7 @@ __global__ void __launch_bounds__(2 * Half<DH>::N, (FRESH ? 1024 : 1280) / (2 * 
     if (vals) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
+        if (stays) break;
         const int at = tid + i * F::N;
         codes[at] = s_v[(at / 16) * F::VP + at % 16];
       }
