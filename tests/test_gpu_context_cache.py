@@ -629,3 +629,70 @@ def test_offsets_beyond_32_bits():
     U16 = 2.0 ** -8
     assert bool(((out[-1:] - ref).abs().float() <= 2 * U16 * ref.abs().float().clamp(min=float(v.abs().max()) * 2.0 ** -3)).all())
     assert bool(((lse[-1:] - rlse).abs() <= 1e-4).all())
+
+
+@pytest.mark.parametrize("D", [16, 32, 64])
+def test_a_wait_that_runs_out_gives_nan_and_the_next_call_is_right(D):
+    """The tensor-core form of many bf16 queries with its "scores ready" signal withheld and a limit of 0.1 ms."""
+    from ar_tabpfn import _lib
+    c, lib = cc(), _lib.lib()
+    k, v = rows(80, 1, 6, 6000, D, torch.bfloat16)
+    cache = c.quantize_context(k, v)
+    q = torch.randn(3000, 6, 1, D, device="cuda", generator=gen(81)).bfloat16()   # far beyond the few-row kernel's range
+    want = c.context_cache_attention(q, cache)
+    try:
+        _lib.check(lib.artab_debug_set(_lib.DEBUG_WAIT_CYCLES, 200_000))
+        _lib.check(lib.artab_debug_set(_lib.DEBUG_DROP_SCORE_COMMITS, 1))
+        out, lse = c.context_cache_attention(q, cache)
+        torch.cuda.synchronize()
+    finally:
+        lib.artab_debug_set(_lib.DEBUG_DROP_SCORE_COMMITS, 0)
+        lib.artab_debug_set(_lib.DEBUG_WAIT_CYCLES, 0)
+    assert bool(torch.isnan(out).all()) and bool(torch.isnan(lse).all())
+    assert all(torch.equal(a, b) for a, b in zip(want, c.context_cache_attention(q, cache)))
+
+
+def test_two_graphs_with_workspaces_replayed_in_turn():
+    """Attention over listed blocks by block, captured for two caches: each graph has its own partial results."""
+    c = cc()
+    outs, wants, graphs = [], [], []
+    for seed in (90, 91):
+        k, v = rows(seed, 1, 2, 1000, 32, torch.float32)
+        cache = c.quantize_context(k, v)
+        q = torch.randn(600, 2, 1, 32, device="cuda", generator=gen(seed))
+        blocks = c.select_context_blocks(q, cache, 8)
+        from ar_tabpfn import _lib
+        assert _lib.lib().artab_cache_block_workspace(cache._ref, 600, 1, 8) > 0
+        wants.append((blocks, c.block_context_attention(q, cache, blocks)))
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append((c.select_context_blocks(q, cache, 8), c.block_context_attention(q, cache, blocks), (cache, q)))
+        graphs.append(g)
+    for i in (0, 1, 1, 0, 1, 0):
+        outs[i][1][0].zero_()
+        graphs[i].replay()
+        if i:
+            graphs[0].replay()
+        assert torch.equal(outs[i][0], wants[i][0]) and all(torch.equal(a, b) for a, b in zip(outs[i][1], wants[i][1]))
+
+
+def test_many_rows_again_and_on_another_stream():
+    """The forms of many queries: the same bits twice, and on a side stream while another call runs."""
+    c = cc()
+    for dtype in (torch.float32, torch.bfloat16):
+        k, v = rows(95, 1, 3, 2500, 32, dtype)
+        cache = c.quantize_context(k, v)
+        q = torch.randn(700, 3, 2, 32, device="cuda", generator=gen(96)).to(dtype)
+        want = c.context_cache_attention(q, cache)
+        blocks = c.select_context_blocks(q, cache, 6)
+        listed = c.block_context_attention(q, cache, blocks)
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        got = []
+        for s in streams * 3:
+            with torch.cuda.stream(s):
+                got.append((c.context_cache_attention(q, cache), c.block_context_attention(q, cache, blocks)))
+        torch.cuda.synchronize()
+        for a, b in got:
+            assert all(torch.equal(x, y) for x, y in zip(a, want)) and all(torch.equal(x, y) for x, y in zip(b, listed))
