@@ -249,12 +249,16 @@ __device__ __forceinline__ bool softmax_block(TcSmem<DH>* sm, uint32_t t_row, in
   volatile Ctl* ctl = &sm->ctl;
   bool ok = true;
   float sum = 0.0f;
-#pragma unroll 1
+#pragma unroll
   for (int c = 1; c >= 0; --c) {
     uint32_t r[32], pk[16];
     tmem_ld32(t_row + 32 * c, r);
     wait_ld();
     const int lv = live - 32 * c;
+    if (!kAlias && c == 0) {                      // the next scores may come
+      fence_before();
+      mbar_arrive(&sm->s_free[wg]);
+    }
     if (i == 0 && c == 1) m = MASKED && lv <= 0 ? m : largest<MASKED>(r, lv) * slope;   // no row of these in use: not yet
     if (MASKED && i == 0 && c == 0 && live <= 32) m = largest<MASKED>(r, lv) * slope;
     float part = numerators<MASKED>(r, pk, slope, lift - m, lv);
@@ -264,8 +268,10 @@ __device__ __forceinline__ bool softmax_block(TcSmem<DH>* sm, uint32_t t_row, in
     }
     if (__any_sync(0xffffffffu, !(part < kMostSum))) {
       float k = 0.0f;
-      tmem_ld32(t_row + 32 * c, r);               // again: kept in registers they would cost the common path copies
-      wait_ld();
+      if (kAlias || c == 1) {   // still there: scores kept in registers for this cost the common path a copy each
+        tmem_ld32(t_row + 32 * c, r);
+        wait_ld();
+      }
       if (!(part < kMostSum)) k = fmaxf(ceilf(largest<MASKED>(r, lv) * slope - m), 0.0f);
       m += k;
       const float alpha = ex2(-k);
@@ -296,10 +302,6 @@ __device__ __forceinline__ bool softmax_block(TcSmem<DH>* sm, uint32_t t_row, in
       }
     }
     sum += part;
-    if (!kAlias && c == 0) {
-      fence_before();
-      mbar_arrive(&sm->s_free[wg]);
-    }
     tmem_st16(t_row + kColP + 16 * c, pk);
   }
   l = fmaf(sum, unlift, l);
