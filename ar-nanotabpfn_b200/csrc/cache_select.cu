@@ -7,7 +7,7 @@
 // depend on tiling, and ties (broken by the lowest index) are real ties.
 //
 // One CTA = 16 queries of a (group, head): scores of all blocks into shared memory as ordered keys (products of
-// 16 queries x 8 blocks a warp), then a warp takes two queries at a time, finds their n-th largest keys bit by bit
+// 16 queries x 8 blocks a warp), then a warp takes two queries at a time, finds their n-th largest keys by bisection
 // and writes the chosen indices in ascending order.
 #include "cache8.cuh"
 
@@ -27,12 +27,15 @@ struct SelectArgs {
 
 constexpr int kHeld = 8;   // keys of a lane that are kept in registers: contexts of up to 16384 rows
 
-// Finds the n-th largest of `held` keys (n < held; lanes i, i + 32, ... hold key i) and writes the n indices chosen.
+// Finds the n-th largest of `held` keys (n < held; lanes i, i + 32, ... hold key i) by bisection between two values, `lo` with
+// at least n keys from it on and `hi` with fewer, and writes the n indices chosen.  It ends when exactly n keys lie from lo
+// on, or when lo is a key that is there several times.  A first lower value comes from the largest keys of the 32 lanes alone, at
+// a vote a step: from their n-th on there are n keys, and few more.
 struct Pick {
   uint32_t key[kHeld];
   const uint32_t* row;
-  uint32_t nth, bit;
-  int at_least;
+  uint32_t lo, hi;
+  int at_least;            // keys from lo on
 
   template <typename F>
   __device__ __forceinline__ int count(int held, F f) const {
@@ -45,49 +48,71 @@ struct Pick {
     }
     return __reduce_add_sync(0xffffffffu, n);
   }
-  __device__ __forceinline__ void start(const uint32_t* r, int held) {
+  __device__ __forceinline__ void start(const uint32_t* r, int held, int n) {
     const int lane = threadIdx.x & 31;
     row = r;
-    uint32_t lo = 0xffffffffu, hi = 0;
+    uint32_t top = 0, least = 0xffffffffu;
     if (held <= 32 * kHeld) {
 #pragma unroll
       for (int i = 0; i < kHeld; ++i) {
-        const bool in = i * 32 + lane < held;
-        key[i] = in ? r[i * 32 + lane] : 0u;       // below every key
-        lo = in ? min(lo, key[i]) : lo, hi = max(hi, key[i]);
+        key[i] = i * 32 + lane < held ? r[i * 32 + lane] : 0u;       // 0: below every key
+        top = max(top, key[i]);
       }
+      least = lane < held ? top : 0xffffffffu;
     } else {
-      for (int i = lane; i < held; i += 32) lo = min(lo, r[i]), hi = max(hi, r[i]);
+      for (int i = lane; i < held; i += 32) top = max(top, r[i]), least = min(least, r[i]);
+      if (n <= 32) least = top;
     }
-    lo = __reduce_min_sync(0xffffffffu, lo);
-    hi = __reduce_max_sync(0xffffffffu, hi);
-    // bits that all keys share need no search
-    bit = lo == hi ? 0u : 0x80000000u >> __clz(lo ^ hi);
-    nth = bit ? hi & ~(2u * bit - 1u) : hi;
-    at_least = held;
+    hi = __reduce_max_sync(0xffffffffu, top) + 1u;
+    lo = __reduce_min_sync(0xffffffffu, least);
+    if (n > 32) {                                    // the lanes' own maxima tell nothing
+      if (held <= 32 * kHeld) lo = 1u;
+    } else {
+      uint32_t above = hi;
+      int lanes = min(held, 32);
+      while (lanes > n && above - lo > 1u) {
+        const uint32_t mid = lo + (above - lo) / 2;
+        const int c = __popc(__ballot_sync(0xffffffffu, top >= mid));
+        if (c >= n)
+          lo = mid, lanes = c;
+        else
+          above = mid;
+      }
+    }
+    const uint32_t from = lo;
+    at_least = count(held, [from](uint32_t k) { return k >= from ? 1 : 0; });
   }
+  __device__ __forceinline__ bool done(int n) const { return at_least == n || hi - lo == 1u; }
   __device__ __forceinline__ void narrow(int held, int n) {
-    const uint32_t trial = nth | bit;
-    const int c = count(held, [trial](uint32_t k) { return k >= trial ? 1 : 0; });
-    if (c >= n) nth = trial, at_least = c;
-    bit = at_least > n ? bit >> 1 : 0u;
+    const uint32_t mid = lo + (hi - lo) / 2;
+    const int c = count(held, [mid](uint32_t k) { return k >= mid ? 1 : 0; });
+    if (c >= n)
+      lo = mid, at_least = c;
+    else
+      hi = mid;
   }
   __device__ __forceinline__ void write(int held, int n, int32_t* out) const {
     const int lane = threadIdx.x & 31;
-    const uint32_t last = nth;
-    // every key above the n-th, and the first of those equal to it
-    int ties = n;
-    if (at_least > n) ties -= count(held, [last](uint32_t k) { return k > last ? 1 : 0; });
-    const bool exact = at_least == n;                // every key from nth on is taken
+    const uint32_t below = (1u << lane) - 1u, last = lo;
     int done = 0;
+    if (at_least == n) {                             // every key from lo on
+      for (int i0 = 0; i0 < held && done < n; i0 += 32) {
+        const bool take = i0 + lane < held && row[i0 + lane] >= last;
+        const uint32_t taken = __ballot_sync(0xffffffffu, take);
+        if (take) out[done + __popc(taken & below)] = i0 + lane;
+        done += __popc(taken);
+      }
+      return;
+    }
+    // every key above lo, and the first of those equal to it
+    int ties = n - count(held, [last](uint32_t k) { return k > last ? 1 : 0; });
     for (int i0 = 0; i0 < held && done < n; i0 += 32) {
       const bool there = i0 + lane < held;
       const uint32_t k = there ? row[i0 + lane] : 0u;
-      const bool tie = there && !exact && k == last;
-      const uint32_t tied = __ballot_sync(0xffffffffu, tie);
-      const bool take = (there && (exact ? k >= last : k > last)) || (tie && __popc(tied & ((1u << lane) - 1u)) < ties);
+      const uint32_t tied = __ballot_sync(0xffffffffu, there && k == last);
+      const bool take = there && (k > last || (k == last && __popc(tied & below) < ties));
       const uint32_t taken = __ballot_sync(0xffffffffu, take);
-      if (take) out[done + __popc(taken & ((1u << lane) - 1u))] = i0 + lane;
+      if (take) out[done + __popc(taken & below)] = i0 + lane;
       ties -= min(ties, __popc(tied));
       done += __popc(taken);
     }
@@ -110,6 +135,21 @@ __global__ void __launch_bounds__(kThreads) cache_select_kernel(const SelectArgs
   const int held = (len + kCacheBlock - 1) / kCacheBlock;
   const size_t gh = (size_t)group * H + h;
 
+  // bounds and scales of a warp's eight blocks, asked for while those before them (at first: the queries) are worked on
+  constexpr int kStep = kThreads / 32 * 8;
+  const uint4* bounds = reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(a.c.bounds) + gh * a.c.n_blocks * 2 * DH + t * NE);
+  const float* scales = a.c.scales + gh * a.c.n_blocks * 2;
+  uint4 next[NE / 8];
+  float next_ks[2];
+  const auto load = [&](int j) {
+    if (j >= held) return;
+    const uint4* src = bounds + (size_t)min(j + g, held - 1) * (2 * DH / 8);
+#pragma unroll
+    for (int i = 0; i < NE / 8; ++i) next[i] = src[i];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) next_ks[e] = scales[(size_t)min(j + 2 * t + e, held - 1) * 2];
+  };
+  load(warp * 8);
   // the queries as whole numbers, four channels a thread
   constexpr int C4 = DH / 4;
   __shared__ __align__(16) __half s_q[kRows][DH];
@@ -142,18 +182,13 @@ __global__ void __launch_bounds__(kThreads) cache_select_kernel(const SelectArgs
       qa[s][half] = h2_bits(t < 2 ? __hmin2(x, zero) : __hmax2(x, zero));
       qa[s][2 + half] = h2_bits(t < 2 ? __hmin2(y, zero) : __hmax2(y, zero));
     }
-  const __half* bounds = reinterpret_cast<const __half*>(a.c.bounds) + gh * a.c.n_blocks * 2 * DH;
-  const float* scales = a.c.scales + gh * a.c.n_blocks * 2;
-  for (int j = warp * 8; j < held; j += kThreads / 32 * 8) {
-    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    const int blk = j + g < held ? j + g : held - 1;
-    const uint4* src = reinterpret_cast<const uint4*>(bounds + (size_t)blk * 2 * DH + t * NE);
+  for (int j = warp * 8; j < held; j += kStep) {
+    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f}, ks[2] = {next_ks[0], next_ks[1]};
     uint32_t w[KS][2];
 #pragma unroll
-    for (int i = 0; i < NE / 8; ++i) {
-      const uint4 v = src[i];
-      w[2 * i][0] = v.x, w[2 * i][1] = v.y, w[2 * i + 1][0] = v.z, w[2 * i + 1][1] = v.w;
-    }
+    for (int i = 0; i < NE / 8; ++i)
+      w[2 * i][0] = next[i].x, w[2 * i][1] = next[i].y, w[2 * i + 1][0] = next[i].z, w[2 * i + 1][1] = next[i].w;
+    load(j + kStep);
 #pragma unroll
     for (int s = 0; s < KS; ++s) mma_f16(c, qa[s][0], qa[s][1], qa[s][2], qa[s][3], w[s][0], w[s][1]);
     __syncwarp();
@@ -161,11 +196,10 @@ __global__ void __launch_bounds__(kThreads) cache_select_kernel(const SelectArgs
     for (int e = 0; e < 2; ++e) {
       const int col = j + 2 * t + e;
       if (col >= held) continue;
-      const float ks = scales[(size_t)col * 2];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         // a block whose scale is not a number ranks first: what is wrong with it shows in the output
-        const float v = ks == ks ? c[2 * half + e] * ks : __uint_as_float(0x7f800000u);
+        const float v = ks[e] == ks[e] ? c[2 * half + e] * ks[e] : __uint_as_float(0x7f800000u);
         const uint32_t bits = __float_as_uint(v + 0.0f);   // -0 -> 0: equal scores have equal keys
         s_key[(g + 8 * half) * a.pitch + col] = bits & 0x80000000u ? ~bits : bits | 0x80000000u;
       }
@@ -185,11 +219,11 @@ __global__ void __launch_bounds__(kThreads) cache_select_kernel(const SelectArgs
   if (!out[0]) return;
   if (held > n) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) pick[i].start(s_key + (2 * warp + i) * a.pitch, held);   // the scores of a row of zeros, if need be
-    while (pick[0].bit | pick[1].bit) {
+    for (int i = 0; i < 2; ++i) pick[i].start(s_key + (2 * warp + i) * a.pitch, held, n);   // of a row of zeros, if need be
+    while (!pick[0].done(n) || !pick[1].done(n)) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        if (pick[i].bit) pick[i].narrow(held, n);
+        if (!pick[i].done(n)) pick[i].narrow(held, n);
     }
   }
 #pragma unroll
