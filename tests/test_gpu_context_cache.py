@@ -269,6 +269,35 @@ def test_rows_appended_step_by_step(shape, dtype):
         assert int(state[3].max()) <= cache.length
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(1, 1, 16), (7, 3, 32), (5, 2, 64)], ids=str)
+def test_single_rows_one_after_another(shape, dtype):
+    """The step of a decode over more than two blocks: scales that rise and stay, contexts that take no row, rows that
+    are taken back, rows of zeros, from strided tensors; the last rows one beyond the capacity."""
+    c = cc()
+    G, H, D = shape
+    cap = 192
+    k, v = rows(100, G, H, 50, D, dtype)
+    lens = torch.arange(G, device="cuda").int() * 13 % 50
+    cache = c.quantize_context(k, v, lens=lens, capacity=cap)
+    ck, cv, s, _ = quantized(k, v, lens, cap // BLOCK)
+    state = (ck, cv, s, lens.long())
+    kn, vn = rows(101, G, H, 150, D, dtype)
+    grow = (1 + torch.arange(150, device="cuda") / 60)[:, None]
+    kn, vn = (kn * grow).to(dtype), (vn / grow).to(dtype)
+    kn[:, :, 20] = 0
+    g = torch.Generator().manual_seed(3)
+    for i in range(150):
+        counts = torch.randint(0, 4, (G,), generator=g).clamp(max=1).cuda() if i % 5 == 3 else torch.ones(G, dtype=torch.long, device="cuda")
+        start = (state[3] - 2).clamp(min=0) if i % 17 == 16 else None
+        if int((state[3] if start is None else start).max()) + 1 > cap:
+            start = state[3] if i % 2 else state[3] // 3
+        c.append_context(cache, kn[:, :, i:i + 1], vn[:, :, i:i + 1], counts=counts, start=start)
+        state = _append_reference(state, kn[:, :, i:i + 1], vn[:, :, i:i + 1], state[3] if start is None else start, counts, cap)
+        if i % 7 == 0 or i > 120 or start is not None:
+            check_fields(cache, *state)
+
+
 def test_a_full_cache_refuses_rows_and_looks_its_lengths_up_before():
     c = cc()
     k, v = rows(7, 2, 2, 100, 32, torch.float32)
