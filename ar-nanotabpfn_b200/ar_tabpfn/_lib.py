@@ -14,7 +14,7 @@ import torch
 
 F32, BF16 = 0, 1
 ETIMEOUT = -5
-DEBUG_WAIT_CYCLES, DEBUG_DROP_SCORE_COMMITS = 0, 1
+DEBUG_WAIT_CYCLES, DEBUG_DROP_SCORE_COMMITS, DEBUG_CACHE_FORM = 0, 1, 2
 MARK_TARGET, MARK_CONTEXT, MARK_BUFFER = 0, 1, 2
 MAX_SPLITS = 16
 

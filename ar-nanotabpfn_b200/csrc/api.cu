@@ -47,6 +47,8 @@ static int dependent_launch_default() {
 static std::atomic<int> g_dependent_launch{dependent_launch_default()};
 static std::atomic<long long> g_debug_wait_cycles{0};
 static std::atomic<int> g_debug_drop_score_commits{0};
+static std::atomic<int> g_debug_cache_form{0};
+int debug_cache_form() { return g_debug_cache_form.load(std::memory_order_relaxed); }
 long long debug_wait_cycles() { return g_debug_wait_cycles.load(std::memory_order_relaxed); }
 int debug_drop_score_commits() { return g_debug_drop_score_commits.load(std::memory_order_relaxed); }
 
@@ -405,6 +407,10 @@ int artab_debug_set(int key, long long value) {
       return ARTAB_OK;
     case ARTAB_DEBUG_DROP_SCORE_COMMITS:
       g_debug_drop_score_commits.store(value != 0, std::memory_order_relaxed);
+      return ARTAB_OK;
+    case ARTAB_DEBUG_CACHE_FORM:
+      ARTAB_REQUIRE(value >= 0 && value <= 2, ARTAB_EINVAL, "debug_set: the form must be 0, 1 or 2");
+      g_debug_cache_form.store((int)value, std::memory_order_relaxed);
       return ARTAB_OK;
     default:
       set_error("debug_set: unknown key %d", key);

@@ -540,13 +540,14 @@ int by_form(AttnArgs& a, long blocks, cudaStream_t s) {
     plan_warps(a, blocks, kResident);
     return launch<T, DH, 2, 2>(a, s);
   }
-  if (a.rows > 8) {
+  const int form = debug_cache_form();
+  if (form == 2 || (form == 0 && a.rows > 8)) {
     const long units = a.units * ((a.rows + kRows - 1) / kRows);
     double least = kFewStart + cost.few * (double)(a.units * ((a.rows + 8 / kParts - 1) / (8 / kParts))) * (double)blocks;
     int splits = 0;
     for (int n = 1; n <= 8; n *= 2) {
       const double t = row_tiles_time(cost, units, blocks, n);
-      if (t < least) least = t, splits = n;
+      if (t < least || (form == 2 && !splits)) least = t, splits = n;
     }
     if (splits) {
       tiles(kRows);
@@ -572,6 +573,7 @@ int attention(int dtype, const void* q, const int64_t* strides, int n_streams, i
   rc = check_queries(dtype, q, n_streams, n_q, c, what);
   if (rc) return rc;
   ARTAB_REQUIRE(out && lse, ARTAB_EINVAL, "%s: null pointer", what);
+  ARTAB_REQUIRE(reinterpret_cast<uintptr_t>(out) % 16 == 0, ARTAB_EINVAL, "%s: the output must be 16-byte aligned", what);
   AttnArgs a;
   a.c = *c;
   a.q = row_view(q, strides, c->n_heads, n_q, c->head_dim);

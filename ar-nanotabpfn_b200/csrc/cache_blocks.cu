@@ -159,15 +159,18 @@ int launch_by_block(const JoinArgs& j, cudaStream_t s) {
 }  // namespace
 
 // Going through the blocks pays from so many entries a block on (in the mean), as long as looking an entry up in every
-// block does not cost more than the records that are read once less.
+// block does not cost more than the records that are read once less, and the partial results stay below a gigabyte.
 constexpr int kLeastShared = 8;
+constexpr int64_t kMostWorkspace = 1LL << 30;
 int64_t by_block_workspace(const artab_cache* c, int n_streams, int n_q, int n_list) {
   const int64_t rows = c->n_groups == 1 ? (int64_t)n_streams * n_q : n_q;
   const int64_t entries = (int64_t)n_streams * c->n_heads * n_q * n_list;
-  if (rows * n_list < (int64_t)kLeastShared * c->n_blocks || c->n_blocks * 4 > 64 * c->head_dim || entries < 8192 ||
-      entries > (1 << 27))
+  const int64_t bytes = entries * (c->head_dim * 4 + 8);
+  const int form = debug_cache_form();
+  if (form == 1 || entries > (1 << 27) || bytes > kMostWorkspace) return 0;
+  if (form == 0 && (rows * n_list < (int64_t)kLeastShared * c->n_blocks || c->n_blocks * 4 > 64 * c->head_dim || entries < 8192))
     return 0;
-  return entries * (c->head_dim * 4 + 8);
+  return bytes;
 }
 
 int launch_cache_by_block(int dtype, const AttnArgs& a, void* workspace, cudaStream_t s) {

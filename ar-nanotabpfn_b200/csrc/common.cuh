@@ -103,6 +103,7 @@ bool dependent_launch_enabled();
 long long debug_wait_cycles();
 constexpr long long kDefaultWaitCycles = 2000000000LL;   // about one second
 int debug_drop_score_commits();
+int debug_cache_form();
 
 // While one of these lives on the calling thread, launch_dependent* issue plain launches.
 struct PlainLaunchScope {

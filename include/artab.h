@@ -396,7 +396,7 @@ ARTAB_API int artab_cache_read(int dtype, const artab_cache* c, const int32_t* s
                                void* stream);
 
 /* Attention of q [B][H][Lq][Dh] (HOST array of three strides: stream, head, query; NULL: contiguous) over the rows in use:
- * out [B][H][Lq][Dh] of `dtype`, lse [B][H][Lq] (natural log).  A context of no rows gives 0 and -inf.
+ * out [B][H][Lq][Dh] of `dtype` (16-byte aligned), lse [B][H][Lq] (natural log).  A context of no rows gives 0 and -inf.
  * max_len: a bound of lens known to the host, for the choice of launch only (results do not depend on its truth). */
 ARTAB_API int artab_cache_attention(int dtype, const void* q, const int64_t* q_strides, int n_streams, int n_q,
                                     const artab_cache* c, int max_len, float scale, void* out, float* lse,
@@ -466,9 +466,13 @@ ARTAB_API void artab_set_dependent_launch(int on);
  *   ARTAB_DEBUG_DROP_SCORE_COMMITS value != 0: the context contraction's MMA thread never signals
  *                                  "scores ready", so its softmax threads' waits run out.  This is how
  *                                  the tests exercise the give-up path without faulting anything:
- *                                  the kernel returns normally, status is non-zero, `out` untouched. */
+ *                                  the kernel returns normally, status is non-zero, `out` untouched.
+ *   ARTAB_DEBUG_CACHE_FORM         which kernels serve the 8-bit context cache: 0 by their cost; 1 attention a few rows at
+ *                                  a time and listed blocks one by one; 2 attention in tiles of many rows and listed
+ *                                  blocks block by block (as far as a workspace is handed over).  Results are the same up to rounding. */
 #define ARTAB_DEBUG_WAIT_CYCLES 0
 #define ARTAB_DEBUG_DROP_SCORE_COMMITS 1
+#define ARTAB_DEBUG_CACHE_FORM 2
 ARTAB_API int artab_debug_set(int key, long long value);
 
 /* Kernels launched by this library on the calling thread since the last reset

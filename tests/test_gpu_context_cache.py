@@ -23,6 +23,16 @@ def cc():
     return context_cache
 
 
+@pytest.fixture(params=["by_cost", "few_rows", "row_tiles"])
+def form(request):
+    """Attention by the kernels that their cost picks, and by either kind whatever the sizes."""
+    from ar_tabpfn import _lib
+    lib = _lib.lib()
+    _lib.check(lib.artab_debug_set(_lib.DEBUG_CACHE_FORM, ("by_cost", "few_rows", "row_tiles").index(request.param)))
+    yield request.param
+    lib.artab_debug_set(_lib.DEBUG_CACHE_FORM, 0)
+
+
 def gen(seed):
     return torch.Generator(device="cuda").manual_seed(seed)
 
@@ -342,12 +352,13 @@ def test_rows_read_from_anywhere():
 ATTENTION = [(True, 1, 1, 16, 1, 1), (True, 3, 2, 32, 63, 1), (False, 3, 2, 32, 64, 2), (True, 2, 3, 64, 65, 5),
              (False, 5, 2, 16, 200, 1), (False, 9, 1, 64, 333, 9), (True, 17, 2, 32, 1000, 1), (True, 1, 2, 32, 5003, 1),
              (False, 2, 1, 64, 4100, 3), (True, 40, 6, 32, 700, 2), (True, 300, 2, 32, 450, 1), (True, 70, 1, 64, 1500, 3),
-             (True, 1, 2, 64, 20000, 300), (True, 257, 1, 16, 130, 2), (False, 3, 2, 32, 900, 150)]
+             (True, 1, 2, 64, 20000, 300), (True, 257, 1, 16, 130, 2), (False, 3, 2, 32, 900, 150),
+             (True, 1100, 2, 32, 1500, 2), (False, 6, 3, 16, 1700, 500), (True, 900, 1, 64, 4100, 3)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
 @pytest.mark.parametrize("case", ATTENTION, ids=str)
-def test_attention_over_the_cache(case, dtype):
+def test_attention_over_the_cache(case, dtype, form):
     shared, B, H, D, N, L = case
     G = 1 if shared else B
     k, v = rows(20, G, H, N, D, dtype)
@@ -359,7 +370,7 @@ def test_attention_over_the_cache(case, dtype):
 
 @pytest.mark.parametrize("B", [2, 200])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
-def test_scales_of_scores_and_magnitudes(dtype, B):
+def test_scales_of_scores_and_magnitudes(dtype, B, form):
     """Any factor of the scores, negative and zero too; scores far apart between blocks; values and queries of extreme size."""
     c = cc()
     k, v = rows(22, 1, 2, 500, 32, dtype)
@@ -376,7 +387,7 @@ def test_scales_of_scores_and_magnitudes(dtype, B):
 
 @pytest.mark.parametrize("B", [2, 100])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
-def test_values_that_are_not_finite_leave_the_weights_sound(dtype, B):
+def test_values_that_are_not_finite_leave_the_weights_sound(dtype, B, form):
     c = cc()
     k, v = rows(28, 1, 3, 300, 32, dtype)
     q = torch.randn(B, 3, 1, 32, device="cuda", generator=gen(29)).to(dtype)
@@ -397,7 +408,7 @@ def test_values_that_are_not_finite_leave_the_weights_sound(dtype, B):
 
 @pytest.mark.parametrize("D", [16, 32, 64])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
-def test_scores_that_rise_from_block_to_block_and_within(dtype, D):
+def test_scores_that_rise_from_block_to_block_and_within(dtype, D, form):
     """Keys along one direction, longer from row to row, in steps far beyond the range of a half-precision numerator, up, down
     and in between; half of the queries point the other way."""
     c = cc()
@@ -419,7 +430,7 @@ def test_scores_that_rise_from_block_to_block_and_within(dtype, D):
 
 
 @pytest.mark.parametrize("B", [3, 130])
-def test_queries_by_strides_and_odd_addresses(B):
+def test_queries_by_strides_and_odd_addresses(B, form):
     c = cc()
     for dtype in (torch.float32, torch.bfloat16):
         k, v = rows(24, 1, 2, 300, 32, dtype)
@@ -434,7 +445,7 @@ def test_queries_by_strides_and_odd_addresses(B):
             assert all(torch.equal(a, b) for a, b in zip(c.block_context_attention(x, cache, blocks), c.block_context_attention(y, cache, blocks)))
 
 
-def test_a_query_that_is_not_finite_stays_in_its_row():
+def test_a_query_that_is_not_finite_stays_in_its_row(form):
     c = cc()
     for B in (4, 200):
         for dtype in (torch.float32, torch.bfloat16):
@@ -529,7 +540,7 @@ def times_of(blocks, nb):
 @pytest.mark.parametrize("case", [(True, 1, 1, 16, 1, 1, 1), (False, 4, 2, 32, 640, 2, 5), (True, 3, 3, 64, 2100, 5, 20),
                                   (True, 200, 6, 32, 3000, 2, 16), (False, 5, 2, 64, 1300, 1, 64), (True, 2, 1, 32, 5000, 1, 1),
                                   (False, 3, 2, 64, 900, 250, 7), (True, 700, 2, 16, 500, 1, 9), (True, 1, 1, 32, 64, 9000, 1)], ids=str)
-def test_attention_over_listed_blocks(case, dtype):
+def test_attention_over_listed_blocks(case, dtype, form):
     """Chosen blocks; any list: none (-1), indices that are no block in use, the same one twice."""
     c = cc()
     shared, B, H, D, N, L, S = case
@@ -553,7 +564,7 @@ def test_attention_over_listed_blocks(case, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
 @pytest.mark.parametrize("shared", [True, False])
-def test_a_decode_step_on_a_growing_context(dtype, shared):
+def test_a_decode_step_on_a_growing_context(dtype, shared, form):
     """A cache is written, grows, its blocks are chosen, attended to and merged with private buffers: the attention
     over [listed rows of the cache, buffer rows] together."""
     from ar_tabpfn.model.triton_kernels import merge_attention_outputs, pytorch_buffer_attention
@@ -585,7 +596,7 @@ def test_a_decode_step_on_a_growing_context(dtype, shared):
     check_attention(full, attention(q, cache, D ** -0.5), dtype, D)
 
 
-def test_the_same_bits_again_on_another_stream_and_in_a_graph():
+def test_the_same_bits_again_on_another_stream_and_in_a_graph(form):
     """A decode step captured once and replayed: lengths grow on the device, the launches stay."""
     c = cc()
     B, H, D = 5, 2, 32
@@ -706,7 +717,7 @@ def test_two_graphs_with_workspaces_replayed_in_turn():
         assert torch.equal(outs[i][0], wants[i][0]) and all(torch.equal(a, b) for a, b in zip(outs[i][1], wants[i][1]))
 
 
-def test_many_rows_again_and_on_another_stream():
+def test_many_rows_again_and_on_another_stream(form):
     """The forms of many queries: the same bits twice, and on a side stream while another call runs."""
     c = cc()
     for dtype in (torch.float32, torch.bfloat16):
