@@ -45,6 +45,7 @@ class ContextCache:
       bounds  float16 [G,H,blocks,2,Dh]: smallest and largest key code (less 128) of each channel over a block's rows
       lens    int32 [G]: rows in use.  Kernels read it on the device
 
+    They are worked on in place, where they are now: another tensor put in a field's place is not seen.
     ``length``: a bound of ``lens`` known to the host (default: the capacity)."""
 
     __slots__ = ("codes", "scales", "bounds", "lens", "length", "n_groups", "n_heads", "head_dim", "capacity", "_c", "_ref")
@@ -279,7 +280,7 @@ def select_context_blocks(q: Tensor, cache: ContextCache, n_blocks: int) -> Tens
 
     The bound of a block is sum_d max(q_d lo_d, q_d hi_d) over the extreme keys of its channels, with the query rounded
     to whole numbers (largest magnitude 127): whole-number arithmetic, so the choice is reproducible to the bit; equal
-    bounds go to the lower index.  A query that is not finite gets the first blocks."""
+    bounds go to the lower index.  A query that is not finite gets the first blocks.  Capacities of up to 221184 rows."""
     (B, H, Lq, _), code, device = _queries(q, cache, "select_context_blocks")
     n = int(n_blocks)
     if n < 1:

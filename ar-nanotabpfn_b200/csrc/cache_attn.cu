@@ -11,8 +11,12 @@
 // 2 r + p is part p of query r, and a thread holds both parts of a score of its own query t.  PARTS = 1: eight
 // queries.  Numerators become the second product's columns by one 8 x 8 transposition per 8 rows.  Each warp
 // walks blocks of its own with a running maximum; its ring of records is filled by 16-byte asynchronous copies
-// and no warp waits for another until the end, where the warps of a CTA and the CTAs of a cluster (up to eight
+// and no warp waits for another until the end, where the warps of a unit and the CTAs of a cluster (up to eight
 // share the rows of a context) merge maximum, sum and output through shared memory.
+// Measured (B200), queries of one row each: 8 contexts x 65536 rows x 8 heads of size 64, 90 us for 537 MB (5.95 TB/s, 0.91
+// of a copy's rate; half of the issue slots busy, three ring stages instead of two 102 us: one CTA an SM either way), size 32
+// 50 us (5.4 TB/s), size 16 35 us (3.9 TB/s: 16 codes a lane between two shuffles); 64 x 2048 x 6 of size 32 16 us and one
+// context of 16384 rows 8.6 us: a chain of loads, products and merges.
 #include "cache_tile.cuh"
 
 namespace artab {
@@ -198,24 +202,27 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const AttnArgs 
   cluster_meet();
 }
 
-// ---- many rows on one context ------------------------------------------------------------------------------
-// cache_attn_rows_kernel: the queries are the 16-row operand.  A CTA of four warps owns 64 rows a part (PARTS = 1: 128
-// rows; PARTS = 2: 64, part p of query g of a tile in row g + 8 p) and walks the blocks of its share together: each
-// warp turns a quarter of a block's codes into half-precision fragments in shared memory, in the order in which a
-// lane reads them with 16-byte loads, while the block before is worked on; the numerators go from the accumulators
-// of one product straight into the operand registers of the next.  The value scale of a block is folded into the
-// exponent, relative to the largest of the context, so that one accumulator serves all blocks.
-template <int DH, int PARTS>
+// ---- many fp32 rows on one context -----------------------------------------------------------------------------
+// cache_attn_rows_kernel: the queries are the 16-row operand, part p of query g of a tile in row g + 8 p.  A CTA of four
+// warps owns 64 queries and walks the blocks of its share together: each warp turns a quarter of a block's codes into
+// half-precision fragments in shared memory, in the order in which a lane reads them with 16-byte loads, while the
+// block before is worked on; the numerators go from the accumulators of one product straight into the operand
+// registers of the next.  The value scale of a block is folded into the exponent, relative to the largest of the
+// context, so that one accumulator serves all blocks.  (bf16 queries, exact in one part: cache_attn_tc.cu.)
+// 1024 queries x 8192 rows x 6 heads (B200): size 32 65 us, 100 TFLOP/s, 200 with both parts of either product: the tensor
+// pipe 40 % busy, issue slots 40 %; size 64 130 us.  Two CTAs (size 64) or three of 168 registers an SM: what is left
+// is latency of a block's chain (scores, maximum, exponentials, second product) with twelve warps to hide it.
+template <int DH>
 struct RowTile {
-  static constexpr int MT = 2, NW = 4;
-  static constexpr int ROWS = NW * MT * 16 / PARTS;
+  static constexpr int MT = 2, NW = 4;                              // tiles of 8 queries a warp, warps
+  static constexpr int ROWS = NW * MT * 8;
   static constexpr int kBlockBytes = 2 * kCacheBlock * DH * 2;      // keys and values as halves
   static constexpr int kSmem = 2 * kBlockBytes > ROWS * kPartial<DH> * 4 ? 2 * kBlockBytes : ROWS * kPartial<DH> * 4;
 };
-template <typename T, int DH, int PARTS>
+template <int DH>
 __global__ void __launch_bounds__(128, DH == 64 ? 2 : 3) cache_attn_rows_kernel(const AttnArgs a) {
-  using RT = RowTile<DH, PARTS>;
-  constexpr int MT = RT::MT, NW = RT::NW, KS = DH / 16, ND = DH / 8, P = kPartial<DH>, R = 3 - PARTS;
+  using RT = RowTile<DH>;
+  constexpr int MT = RT::MT, NW = RT::NW, KS = DH / 16, ND = DH / 8, P = kPartial<DH>;
   constexpr int KN = 8 / NW, VN = ND > NW ? ND / NW : 1;         // key and value tiles that a warp lays out
   constexpr int KQ = KS >= 2 ? KS / 2 : 1;                       // 16-byte pieces of a lane's key fragments
   constexpr size_t kRecord = 2 * kCacheBlock * DH;
@@ -294,44 +301,40 @@ __global__ void __launch_bounds__(128, DH == 64 ? 2 : 3) cache_attn_rows_kernel(
 
   // queries: fragments a0 .. a3 of every k step
   uint32_t q[MT][KS][4];
-  float f[MT][R];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      constexpr int NE = DH / 4;
-      const int row = row0 + (warp * MT + mt) * (16 / PARTS) + g + 8 * r;
-      float x[NE];
-#pragma unroll
-      for (int i = 0; i < NE; ++i) x[i] = 0.0f;
-      if (row < a.rows)
-        load_elements<T, NE>(reinterpret_cast<const T*>(a.q.p) + stream_of(row) * a.q.s0 + h * a.q.s1 +
-                                 query_of(row) * a.q.s2 + t * NE, a.vec_q, x);
-      float top = 0.0f;
-#pragma unroll
-      for (int i = 0; i < NE; ++i) top = fmaxf(top, fabsf(x[i]));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      float to, back;
-      row_scale(top, to, back);
-      f[mt][r] = back * fabsf(a.scale_log2);
-      to = copysignf(to, a.scale_log2);
-#pragma unroll
-      for (int s = 0; s < KS; ++s)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float u = x[4 * s + 2 * j] * to, w = x[4 * s + 2 * j + 1] * to;
-          const __half2 hi = __floats2half2_rn(u, w);
-          q[mt][s][2 * j + r] = h2_bits(hi);
-          if constexpr (PARTS == 2)
-            q[mt][s][2 * j + 1] = h2_bits(__floats2half2_rn(u - __low2float(hi), w - __high2float(hi)));
-        }
-    }
-  float m[MT][R], l[MT][R], o[MT][ND][4];
+  float f[MT];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
+    constexpr int NE = DH / 4;
+    const int row = row0 + (warp * MT + mt) * 8 + g;
+    float x[NE];
 #pragma unroll
-    for (int r = 0; r < R; ++r) m[mt][r] = -CUDART_INF_F, l[mt][r] = 0.0f;
+    for (int i = 0; i < NE; ++i) x[i] = 0.0f;
+    if (row < a.rows)
+      load_elements<float, NE>(reinterpret_cast<const float*>(a.q.p) + stream_of(row) * a.q.s0 + h * a.q.s1 +
+                               query_of(row) * a.q.s2 + t * NE, a.vec_q, x);
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) top = fmaxf(top, fabsf(x[i]));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    float to, back;
+    row_scale(top, to, back);
+    f[mt] = back * fabsf(a.scale_log2);
+    to = copysignf(to, a.scale_log2);
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float u = x[4 * s + 2 * j] * to, w = x[4 * s + 2 * j + 1] * to;
+        const __half2 hi = __floats2half2_rn(u, w);
+        q[mt][s][2 * j] = h2_bits(hi);
+        q[mt][s][2 * j + 1] = h2_bits(__floats2half2_rn(u - __low2float(hi), w - __high2float(hi)));
+      }
+    }
+  float m[MT], l[MT], o[MT][ND][4];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    m[mt] = -CUDART_INF_F, l[mt] = 0.0f;
 #pragma unroll
     for (int j = 0; j < ND; ++j)
 #pragma unroll
@@ -380,55 +383,39 @@ __global__ void __launch_bounds__(128, DH == 64 ? 2 : 3) cache_attn_rows_kernel(
     uint32_t p[MT][4][4];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      if constexpr (PARTS == 2)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) c[mt][j][0] += c[mt][j][2], c[mt][j][1] += c[mt][j][3];
+      for (int j = 0; j < 8; ++j) c[mt][j][0] += c[mt][j][2], c[mt][j][1] += c[mt][j][3];
       if (live < kCacheBlock)
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
-          for (int e = 0; e < 2 * R; ++e)
-            if (8 * j + 2 * t + (e & 1) >= live) c[mt][j][e] = -CUDART_INF_F;
-      float alpha[R], sl[R], add[R];
+          for (int e = 0; e < 2; ++e)
+            if (8 * j + 2 * t + e >= live) c[mt][j][e] = -CUDART_INF_F;
+      float mx = c[mt][0][0];
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        float mx = c[mt][0][2 * r];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fmaxf(c[mt][j][2 * r], c[mt][j][2 * r + 1]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float x = f[mt][r] * sc.x;
-        sl[r] = !(x <= 1e-37f) ? x : 1e-37f;      // never 0 (a masked score stays -inf), NaN as it is
-        mx = fmaxf(m[mt][r], mx * sl[r]);
-        const float base = mx == -CUDART_INF_F ? 0.0f : mx;
-        alpha[r] = ex2(m[mt][r] - base);
-        m[mt][r] = mx;
-        add[r] = lift - base;
-      }
-      bool moved = alpha[0] != 1.0f;
-      if (R == 2) moved |= alpha[R - 1] != 1.0f;
-      if (__any_sync(0xffffffffu, moved)) {
+      for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fmaxf(c[mt][j][0], c[mt][j][1]));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float x = f[mt] * sc.x, slope = !(x <= 1e-37f) ? x : 1e-37f;      // never 0 (a masked score stays -inf), NaN as it is
+      mx = fmaxf(m[mt], mx * slope);
+      const float base = mx == -CUDART_INF_F ? 0.0f : mx, alpha = ex2(m[mt] - base), add = lift - base;
+      m[mt] = mx;
+      if (__any_sync(0xffffffffu, alpha != 1.0f)) {
 #pragma unroll
         for (int j = 0; j < ND; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[mt][j][e] *= alpha[PARTS == 2 ? 0 : e >> 1];
+          for (int e = 0; e < 4; ++e) o[mt][j][e] *= alpha;
       }
-      float sum[R];
+      float sum = 0.0f;
 #pragma unroll
-      for (int r = 0; r < R; ++r) sum[r] = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const float x = ex2(fmaf(c[mt][j][2 * r], sl[r], add[r])), y = ex2(fmaf(c[mt][j][2 * r + 1], sl[r], add[r]));
-          sum[r] += x + y;
-          const __half2 hi = __floats2half2_rn(x, y);
-          p[mt][j >> 1][2 * (j & 1) + r] = h2_bits(hi);
-          if constexpr (PARTS == 2)
-            p[mt][j >> 1][2 * (j & 1) + 1] = h2_bits(__floats2half2_rn(x - __low2float(hi), y - __high2float(hi)));
-        }
-#pragma unroll
-      for (int r = 0; r < R; ++r) l[mt][r] = fmaf(l[mt][r], alpha[r], sum[r] * unlift);
+      for (int j = 0; j < 8; ++j) {
+        const float y = ex2(fmaf(c[mt][j][0], slope, add)), z = ex2(fmaf(c[mt][j][1], slope, add));
+        sum += y + z;
+        const __half2 hi = __floats2half2_rn(y, z);
+        p[mt][j >> 1][2 * (j & 1)] = h2_bits(hi);
+        p[mt][j >> 1][2 * (j & 1) + 1] = h2_bits(__floats2half2_rn(y - __low2float(hi), z - __high2float(hi)));
+      }
+      l[mt] = fmaf(l[mt], alpha, sum * unlift);
     }
     const uint4* v = reinterpret_cast<const uint4*>(kv + 2 * kCacheBlock * DH);
 #pragma unroll
@@ -452,25 +439,22 @@ __global__ void __launch_bounds__(128, DH == 64 ? 2 : 3) cache_attn_rows_kernel(
 
   float* part = reinterpret_cast<float*>(smem);
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  for (int mt = 0; mt < MT; ++mt) {
+    const int row = (warp * MT + mt) * 8 + g;
+    float s = l[mt];
+    s += __shfl_xor_sync(0xffffffffu, s, 1);
+    s += __shfl_xor_sync(0xffffffffu, s, 2);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int row = (warp * MT + mt) * (16 / PARTS) + g + 8 * r;
-      float s = l[mt][r];
-      s += __shfl_xor_sync(0xffffffffu, s, 1);
-      s += __shfl_xor_sync(0xffffffffu, s, 2);
+    for (int j = 0; j < ND; ++j)
 #pragma unroll
-      for (int j = 0; j < ND; ++j)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          part[row * P + 8 * j + 2 * t + e] = (PARTS == 2 ? o[mt][j][e] + o[mt][j][2 + e] : o[mt][j][2 * r + e]) * vmax + poison;
-      if (t == 0) part[row * P + DH] = m[mt][r], part[row * P + DH + 1] = s;
-    }
+      for (int e = 0; e < 2; ++e) part[row * P + 8 * j + 2 * t + e] = (o[mt][j][e] + o[mt][j][2 + e]) * vmax + poison;
+    if (t == 0) part[row * P + DH] = m[mt], part[row * P + DH + 1] = s;
+  }
   if (a.splits == 1)
     __syncthreads();
   else
     cluster_meet();
-  merge_rows<T, DH>(a, smem_u32(part), 1, rank * 32 * NW + tid, a.splits * 32 * NW, RT::ROWS, row0, h, group, kLift);
+  merge_rows<float, DH>(a, smem_u32(part), 1, rank * 32 * NW + tid, a.splits * 32 * NW, RT::ROWS, row0, h, group, kLift);
   if (a.splits > 1) cluster_meet();
 }
 
@@ -481,10 +465,10 @@ int launch(const AttnArgs& a, cudaStream_t s) {
   const size_t ring = (size_t)kWarps * Ring<DH>::kBytes;
   return launch_attn(cache_attn_kernel<T, DH, PARTS, FORM>, config, part > ring ? part : ring, kWarps * 32, a, s);
 }
-template <typename T, int DH, int PARTS>
+template <int DH>
 int launch_rows(const AttnArgs& a, cudaStream_t s) {
   static SmemConfig config;
-  return launch_attn(cache_attn_rows_kernel<T, DH, PARTS>, config, RowTile<DH, PARTS>::kSmem, RowTile<DH, PARTS>::NW * 32, a, s);
+  return launch_attn(cache_attn_rows_kernel<DH>, config, RowTile<DH>::kSmem, RowTile<DH>::NW * 32, a, s);
 }
 
 // Rounds of work on a GPU that holds `cap` workers at a time: they end one by one, so between the quotient and the whole
@@ -532,7 +516,7 @@ double row_tiles_time(const Cost& c, long units, long blocks, int s) {
 template <typename T, int DH>
 int by_form(AttnArgs& a, long blocks, cudaStream_t s) {
   constexpr int kParts = sizeof(T) == 2 ? 1 : 2;
-  constexpr int kRows = kParts == 1 ? 128 : RowTile<DH, kParts>::ROWS;
+  constexpr int kRows = kParts == 1 ? 128 : RowTile<DH>::ROWS;
   constexpr Cost cost = cost_of<T, DH>();
   constexpr int kResident = DH == 64 ? 8 : 16;     // warps of an SM, by their rings
   const auto tiles = [&a](int rows) { a.tiles = (a.rows + rows - 1) / rows, a.units *= a.tiles; };
@@ -555,7 +539,7 @@ int by_form(AttnArgs& a, long blocks, cudaStream_t s) {
       if constexpr (kParts == 1)
         return launch_cache_attn_tc(a, s);
       else
-        return launch_rows<T, DH, kParts>(a, s);
+        return launch_rows<DH>(a, s);
     }
   }
   const bool eight = kParts == 1 && a.rows > 4;

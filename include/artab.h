@@ -397,7 +397,8 @@ ARTAB_API int artab_cache_read(int dtype, const artab_cache* c, const int32_t* s
 
 /* Attention of q [B][H][Lq][Dh] (HOST array of three strides: stream, head, query; NULL: contiguous) over the rows in use:
  * out [B][H][Lq][Dh] of `dtype` (16-byte aligned), lse [B][H][Lq] (natural log).  A context of no rows gives 0 and -inf.
- * max_len: a bound of lens known to the host, for the choice of launch only (results do not depend on its truth). */
+ * max_len: a bound of lens known to the host, for the choice of kernel and launch only (any value gives a right result).
+ * A bounded wait that gives up shows as NaN in the rows of out and lse that it concerns. */
 ARTAB_API int artab_cache_attention(int dtype, const void* q, const int64_t* q_strides, int n_streams, int n_q,
                                     const artab_cache* c, int max_len, float scale, void* out, float* lse,
                                     void* stream);
@@ -460,13 +461,14 @@ ARTAB_API void artab_set_dependent_launch(int on);
  * the reference).  Every mbarrier wait inside the kernels gives up after a limit, the CTA then waits for
  * what it has in flight, frees what it holds, sets the status word and returns; results of the call are void.
  *   ARTAB_DEBUG_WAIT_CYCLES        value = limit in SM clock cycles for the waits of the context contraction, the
- *                                  whole-sequence decode and the register-tiled chain (0 restores the
+ *                                  whole-sequence decode, the register-tiled chain and artab_cache_attention (0 restores the
  *                                  built-in limit of about one second; the other dense chains always have
  *                                  that, except that the few-row chain gives up at once with a limit of 1)
  *   ARTAB_DEBUG_DROP_SCORE_COMMITS value != 0: the context contraction's MMA thread never signals
  *                                  "scores ready", so its softmax threads' waits run out.  This is how
  *                                  the tests exercise the give-up path without faulting anything:
- *                                  the kernel returns normally, status is non-zero, `out` untouched.
+ *                                  the kernel returns normally, status is non-zero, `out` untouched.  The same in
+ *                                  artab_cache_attention's tensor-core form, which writes NaN to out and lse instead.
  *   ARTAB_DEBUG_CACHE_FORM         which kernels serve the 8-bit context cache: 0 by their cost; 1 attention a few rows at
  *                                  a time and listed blocks one by one; 2 attention in tiles of many rows and listed
  *                                  blocks block by block (as far as a workspace is handed over).  Results are the same up to rounding. */
