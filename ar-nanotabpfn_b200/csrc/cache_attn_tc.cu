@@ -15,9 +15,9 @@
 // no room for P beside S: it overwrites the scores it came from, and the next scores wait for P . V.
 // Measured (B200), 8192 queries x 8192 rows x 6 heads: head size 32 176 us (292 TFLOP/s, 2.28e12 exponentials a second),
 // 16 162 us, 64 213 us (484 TFLOP/s); 87 us is what the special-function units need for the exponentials.  They are 63 % busy,
-// issue slots 57 % (of some 440 instructions a warp and block 160 are the 64 numerators' own), the tensor pipe 15 %.  One
-// warpgroup alone takes 1500 - 2500 cycles a block, four on an SM 3600 for one block each: latency of a chain of loads,
-// exponentials, stores and barriers with four warps a scheduler.  What was measured on the way at head size 32: masked blocks in
+// issue slots 57 % (of some 440 instructions a warp and block 160 are the 64 numerators' own), the tensor pipe 15 %.  Two
+// warpgroups alone on an SM take 2200 cycles a block each, four 3400: latency of a chain of loads, exponentials, stores and
+// barriers with four warps a scheduler.  What was measured on the way at head size 32: masked blocks in
 // code of their own 261 -> 226 us; MMAs issued by an elected lane instead of lane 0 of a divergent warp, scores read again
 // (not kept) where the reference rises, waits in a tight loop 226 -> 208; all memory asked for before the first barrier,
 // both halves of a block unrolled, the next scores as soon as these are read 208 -> 176.  A share of the exponentials on the FMA
