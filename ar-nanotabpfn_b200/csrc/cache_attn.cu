@@ -22,7 +22,7 @@
 namespace artab {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 8;         // of a unit, at most
 
 template <int DH>
 struct Ring {
@@ -37,9 +37,10 @@ constexpr int partial_floats() {
   return Tile<DH, PARTS>::ROWS * (DH + 2);
 }
 
-// FORM 0: every block, a CTA (of a cluster) for a unit; 1: every block, several units a CTA; 2: listed blocks, either way.
-template <typename T, int DH, int PARTS, int FORM>
-__global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const AttnArgs a) {
+// W warps a CTA.  FORM 0: every block, a CTA (of a cluster) for a unit; 1: every block, several units a CTA; 2: listed blocks,
+// either way.
+template <typename T, int DH, int PARTS, int FORM, int W>
+__global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnArgs a) {
   constexpr bool LIST = FORM == 2;
   using R = Ring<DH>;
   using Tl = Tile<DH, PARTS>;
@@ -47,7 +48,7 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const AttnArgs 
   extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int rank = (int)(blockIdx.x % a.splits);
-  const int per_cta = FORM ? a.per_cta : 1, warps = FORM ? kWarps / per_cta : kWarps;
+  const int per_cta = FORM ? a.per_cta : 1, warps = FORM ? W / per_cta : W;
   long unit = blockIdx.x / a.splits;
   if (FORM) unit = unit * per_cta + warp / warps;
   const bool spare = FORM && unit >= a.units;                         // the last CTA may have warps without a unit
@@ -158,7 +159,7 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const AttnArgs 
     }
   }
   __syncthreads();
-  float* mine = part + kWarps * ROWS * P;
+  float* mine = part + W * ROWS * P;
   const auto merge = [&](auto at, int count, int row, int d, float& m, float& l, float& o) {
     m = -CUDART_INF_F;
     for (int w = 0; w < count; ++w) m = fmaxf(m, at(w, row * P + DH));
@@ -192,7 +193,7 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const AttnArgs 
   if (a.splits == 1) return;
   cluster_meet();
   const uint32_t base = smem_u32(mine);
-  for (int e = rank * kWarps * 32 + tid; e < ROWS * DH; e += a.splits * kWarps * 32) {
+  for (int e = rank * W * 32 + tid; e < ROWS * DH; e += a.splits * W * 32) {
     float m, l, o;
     merge([&](int w, int i) {
       return ld_cluster(base + i * 4, w);
@@ -458,12 +459,21 @@ __global__ void __launch_bounds__(128, DH == 64 ? 2 : 3) cache_attn_rows_kernel(
   if (a.splits > 1) cluster_meet();
 }
 
-template <typename T, int DH, int PARTS, int FORM>
+template <typename T, int DH, int PARTS, int FORM, int W>
 int launch(const AttnArgs& a, cudaStream_t s) {
   static SmemConfig config;
-  const size_t part = (size_t)(kWarps + 1) * partial_floats<DH, PARTS>() * sizeof(float);
-  const size_t ring = (size_t)kWarps * Ring<DH>::kBytes;
-  return launch_attn(cache_attn_kernel<T, DH, PARTS, FORM>, config, part > ring ? part : ring, kWarps * 32, a, s);
+  const size_t part = (size_t)(W + 1) * partial_floats<DH, PARTS>() * sizeof(float);
+  const size_t ring = (size_t)W * Ring<DH>::kBytes;
+  return launch_attn(cache_attn_kernel<T, DH, PARTS, FORM, W>, config, part > ring ? part : ring, W * 32, a, s);
+}
+// By plan_warps' choice: eight warps a unit are a CTA (of a cluster); fewer are CTAs of four, which leave sooner: 64 contexts of
+// 2048 rows 15.7 us with eight, 14.0 with four; 800 units of 11 blocks 16.5 and 14.0.
+template <typename T, int DH, int PARTS>
+int launch_few(AttnArgs& a, int warps, cudaStream_t s) {
+  if (warps == kWarps) return a.list ? launch<T, DH, PARTS, 2, kWarps>(a, s) : launch<T, DH, PARTS, 0, kWarps>(a, s);
+  a.per_cta = 4 / warps;
+  if (a.list) return launch<T, DH, PARTS, 2, 4>(a, s);
+  return a.per_cta == 1 ? launch<T, DH, PARTS, 0, 4>(a, s) : launch<T, DH, PARTS, 1, 4>(a, s);
 }
 template <int DH>
 int launch_rows(const AttnArgs& a, cudaStream_t s) {
@@ -476,22 +486,24 @@ int launch_rows(const AttnArgs& a, cudaStream_t s) {
 double rounds(double workers, double cap) {
   return workers <= cap ? 1.0 : 0.5 * (workers / cap + (double)(long)((workers + cap - 1) / cap));
 }
-// Warps of a unit (fewer than a CTA's: several units a CTA) and CTAs of a unit (a cluster; only whole ones): the least
+// Warps of a unit and CTAs of a unit (a cluster; only whole ones): the least
 // rounds times blocks a warp, start and merge of a round counted as two blocks, each doubling of a cluster as a half, a tenth
-// more for a kernel whose warps and units are not known when it is compiled.
+// more where a CTA has several units (head sizes 16 and 32), a twentieth where it has eight warps.
 // 3072 units of 4 blocks: one warp each 20 us, eight 43; 384 of 32: eight or four 18, one 33; 512 of 32 at head size 64: two 29,
 // eight 38.
-void plan_warps(AttnArgs& a, long blocks, int resident_warps) {
+int plan_warps(AttnArgs& a, long blocks, int resident_warps) {
+  const double few = a.c.head_dim == 64 ? 1.0 : 1.1;
   double least = 0.0;
-  a.splits = 0;
+  int best = 0;
   for (int warps = 1; warps <= kWarps; warps *= 2)
     for (int s = 1, extra = 0; s <= (warps == kWarps ? 8 : 1); s *= 2, ++extra) {
       const long per = (long)warps * s;
       if (s > 1 && blocks < 2 * per) break;
       const double t = rounds((double)a.units * per, (double)kSms * resident_warps) *
-                       ((double)((blocks + per - 1) / per) + 2.0 + 0.5 * extra) * (warps < kWarps ? 1.1 : 1.0);
-      if (!a.splits || t <= least) least = t, a.per_cta = kWarps / warps, a.splits = s;
+                       ((double)((blocks + per - 1) / per) + 2.0 + 0.5 * extra) * (warps == kWarps ? 1.05 : warps < 4 ? few : 1.0);
+      if (!best || t < least) least = t, best = warps, a.splits = s;
     }
+  return best;
 }
 // Which kernel, and how many CTAs share a unit's blocks: the least of the times that these figures give, in us.  Measured
 // (B200) over 16 - 2048 rows, 1 - 384 contexts x heads and 500 - 32768 context rows.
@@ -521,8 +533,7 @@ int by_form(AttnArgs& a, long blocks, cudaStream_t s) {
   constexpr int kResident = DH == 64 ? 8 : 16;     // warps of an SM, by their rings
   const auto tiles = [&a](int rows) { a.tiles = (a.rows + rows - 1) / rows, a.units *= a.tiles; };
   if (a.list) {
-    plan_warps(a, blocks, kResident);
-    return launch<T, DH, 2, 2>(a, s);
+    return launch_few<T, DH, 2>(a, plan_warps(a, blocks, kResident), s);
   }
   const int form = debug_cache_form();
   if (form == 2 || (form == 0 && a.rows > 8)) {
@@ -544,9 +555,8 @@ int by_form(AttnArgs& a, long blocks, cudaStream_t s) {
   }
   const bool eight = kParts == 1 && a.rows > 4;
   tiles(eight ? 8 : 4);
-  plan_warps(a, blocks, kResident);
-  if (a.per_cta == 1) return eight ? launch<T, DH, kParts, 0>(a, s) : launch<T, DH, 2, 0>(a, s);
-  return eight ? launch<T, DH, kParts, 1>(a, s) : launch<T, DH, 2, 1>(a, s);
+  const int warps = plan_warps(a, blocks, kResident);
+  return eight ? launch_few<T, DH, kParts>(a, warps, s) : launch_few<T, DH, 2>(a, warps, s);
 }
 
 int attention(int dtype, const void* q, const int64_t* strides, int n_streams, int n_q, const artab_cache* c,
