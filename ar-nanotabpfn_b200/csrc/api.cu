@@ -409,7 +409,7 @@ int artab_debug_set(int key, long long value) {
       g_debug_drop_score_commits.store(value != 0, std::memory_order_relaxed);
       return ARTAB_OK;
     case ARTAB_DEBUG_CACHE_FORM:
-      ARTAB_REQUIRE(value >= 0 && value <= 2, ARTAB_EINVAL, "debug_set: the form must be 0, 1 or 2");
+      ARTAB_REQUIRE(value >= 0 && value <= 3, ARTAB_EINVAL, "debug_set: the form must be 0, 1, 2 or 3");
       g_debug_cache_form.store((int)value, std::memory_order_relaxed);
       return ARTAB_OK;
     default:

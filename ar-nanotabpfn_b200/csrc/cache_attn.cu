@@ -15,7 +15,7 @@
 // share the rows of a context) merge maximum, sum and output through shared memory.
 // Measured (B200), queries of one row each: 8 contexts x 65536 rows x 8 heads of size 64, 90 us for 537 MB (5.95 TB/s, 0.91
 // of a copy's rate; half of the issue slots busy, three ring stages instead of two 102 us: one CTA an SM either way), size 32
-// 50 us (5.4 TB/s), size 16 35 us (3.9 TB/s: 16 codes a lane between two shuffles); 64 x 2048 x 6 of size 32 16 us and one
+// 50 us (5.4 TB/s), size 16 35 us (3.9 TB/s: 16 codes a lane between two shuffles); 64 x 2048 x 6 of size 32 14 us and one
 // context of 16384 rows 8.6 us: a chain of loads, products and merges.
 #include "cache_tile.cuh"
 
@@ -203,16 +203,16 @@ __global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnArgs a) {
   cluster_meet();
 }
 
-// ---- many fp32 rows on one context -----------------------------------------------------------------------------
+// ---- fp32 rows, some hundreds --------------------------------------------------------------------------------
 // cache_attn_rows_kernel: the queries are the 16-row operand, part p of query g of a tile in row g + 8 p.  A CTA of four
 // warps owns 64 queries and walks the blocks of its share together: each warp turns a quarter of a block's codes into
 // half-precision fragments in shared memory, in the order in which a lane reads them with 16-byte loads, while the
 // block before is worked on; the numerators go from the accumulators of one product straight into the operand
 // registers of the next.  The value scale of a block is folded into the exponent, relative to the largest of the
-// context, so that one accumulator serves all blocks.  (bf16 queries, exact in one part: cache_attn_tc.cu.)
-// 1024 queries x 8192 rows x 6 heads (B200): size 32 65 us, 100 TFLOP/s, 200 with both parts of either product: the tensor
-// pipe 40 % busy, issue slots 40 %; size 64 130 us.  Two CTAs (size 64) or three of 168 registers an SM: what is left
-// is latency of a block's chain (scores, maximum, exponentials, second product) with twelve warps to hide it.
+// context, so that one accumulator serves all blocks.  (bf16 queries and larger jobs: cache_attn_tc.cu.)
+// B200, 6 heads of size 32: 512 queries x 2000 rows 14.3 us, 512 x 8192 34 us.  Two CTAs (size 64) or three of 168 registers an
+// SM; with 1024 queries x 8192 rows (64 us) the tensor pipe is 40 % busy, issue slots 40 %: latency of a block's chain (scores,
+// maximum, exponentials, second product) with twelve warps to hide it.
 template <int DH>
 struct RowTile {
   static constexpr int MT = 2, NW = 4;                              // tiles of 8 queries a warp, warps
@@ -489,7 +489,7 @@ double rounds(double workers, double cap) {
 // Warps of a unit and CTAs of a unit (a cluster; only whole ones): the least
 // rounds times blocks a warp, start and merge of a round counted as two blocks, each doubling of a cluster as a half, a tenth
 // more where a CTA has several units (head sizes 16 and 32), a twentieth where it has eight warps.
-// 3072 units of 4 blocks: one warp each 20 us, eight 43; 384 of 32: eight or four 18, one 33; 512 of 32 at head size 64: two 29,
+// 512 contexts x 6 heads of 4 blocks: one warp each 20 us, eight 43; 384 of 32: eight or four 18, one 33; 512 of 32 at head size 64: two 29,
 // eight 38.
 int plan_warps(AttnArgs& a, long blocks, int resident_warps) {
   const double few = a.c.head_dim == 64 ? 1.0 : 1.1;
@@ -506,51 +506,72 @@ int plan_warps(AttnArgs& a, long blocks, int resident_warps) {
   return best;
 }
 // Which kernel, and how many CTAs share a unit's blocks: the least of the times that these figures give, in us.  Measured
-// (B200) over 16 - 2048 rows, 1 - 384 contexts x heads and 500 - 32768 context rows.
+// (B200) over 16 - 4096 rows, 1 - 384 contexts x heads and 500 - 32768 context rows.
 //   few rows: start and merge, and the whole GPU's time for a block against one tile of 8 (bf16) or 4 (fp32) rows;
-//   row tiles: one CTA's time for a block when it has an SM to itself and when the SM is full; start and merge of a wave.
-struct Cost {
-  double few, alone, full, start;
-  int per_sm;              // row-tile CTAs of an SM
+//   tiles of many rows: one CTA's time for a block when it has an SM to itself and when the SM is full; start and merge of a
+//   wave; CTAs of an SM; rows of a tile.
+struct TileCost {
+  double alone, full, start;
+  int per_sm, rows;
 };
 constexpr double kFewStart = 4.5, kPerSplit = 0.4;
 template <typename T, int DH>
-constexpr Cost cost_of() {
-  if (sizeof(T) == 2) return DH == 16 ? Cost{0.5e-3, 0.56, 0.75, 8.0, 2} : DH == 32 ? Cost{0.85e-3, 0.62, 0.87, 9.0, 2} : Cost{1.8e-3, 0.73, 1.0, 10.0, 2};
-  return DH == 16 ? Cost{0.43e-3, 0.83, 1.7, 4.0, 3} : DH == 32 ? Cost{0.77e-3, 0.96, 2.0, 4.0, 3} : Cost{1.65e-3, 1.3, 2.3, 5.0, 2};
+constexpr double few_cost() {
+  if (sizeof(T) == 2) return DH == 16 ? 0.5e-3 : DH == 32 ? 0.85e-3 : 1.8e-3;
+  return DH == 16 ? 0.43e-3 : DH == 32 ? 0.77e-3 : 1.65e-3;
 }
-double row_tiles_time(const Cost& c, long units, long blocks, int s) {
-  const double ctas = (double)units * s, cap = (double)kSms * c.per_sm;
-  const double crowd = ctas <= kSms ? 0.0 : ctas >= cap ? 1.0 : (ctas / kSms - 1.0) / (c.per_sm - 1);
-  return rounds(ctas, cap) * ((c.alone + (c.full - c.alone) * crowd) * (double)((blocks + s - 1) / s) + c.start + kPerSplit * s);
+// cache_attn_tc_kernel
+template <typename T, int DH>
+constexpr TileCost tc_cost() {
+  if (sizeof(T) == 2) return DH == 16 ? TileCost{0.56, 0.75, 8.0, 2, 128} : DH == 32 ? TileCost{0.62, 0.87, 9.0, 2, 128} : TileCost{0.73, 1.0, 10.0, 2, 128};
+  return DH == 16 ? TileCost{0.75, 1.3, 9.0, 2, 128} : DH == 32 ? TileCost{0.75, 1.3, 9.5, 2, 128} : TileCost{0.82, 1.75, 11.5, 2, 128};
+}
+// cache_attn_rows_kernel.  It starts sooner and has half the rows a tile, tcgen05 is faster once it runs (6 heads x 2000 rows of size
+// 32: 512 queries 14.5 and 22.4 us; 8192 rows: 1024 queries 64 and 49, 4096 queries 227 and 149).
+template <int DH>
+constexpr TileCost rows_cost() {
+  constexpr int rows = RowTile<DH>::ROWS;
+  return DH == 16 ? TileCost{0.83, 1.7, 4.0, 3, rows} : DH == 32 ? TileCost{0.96, 2.0, 4.0, 3, rows} : TileCost{1.3, 2.3, 5.0, 2, rows};
+}
+// least time over the splits of a unit, and those splits
+double tiles_time(const TileCost& c, const AttnArgs& a, long blocks, int& splits) {
+  const double units = (double)a.units * (double)((a.rows + c.rows - 1) / c.rows), cap = (double)kSms * c.per_sm;
+  double least = 0.0;
+  for (int s = 1; s <= 8; s *= 2) {
+    const double ctas = units * s;
+    const double crowd = ctas <= kSms ? 0.0 : ctas >= cap ? 1.0 : (ctas / kSms - 1.0) / (c.per_sm - 1);
+    const double t = rounds(ctas, cap) * ((c.alone + (c.full - c.alone) * crowd) * (double)((blocks + s - 1) / s) + c.start + kPerSplit * s);
+    if (s == 1 || t < least) least = t, splits = s;
+  }
+  return least;
 }
 
 template <typename T, int DH>
 int by_form(AttnArgs& a, long blocks, cudaStream_t s) {
   constexpr int kParts = sizeof(T) == 2 ? 1 : 2;
-  constexpr int kRows = kParts == 1 ? 128 : RowTile<DH>::ROWS;
-  constexpr Cost cost = cost_of<T, DH>();
   constexpr int kResident = DH == 64 ? 8 : 16;     // warps of an SM, by their rings
   const auto tiles = [&a](int rows) { a.tiles = (a.rows + rows - 1) / rows, a.units *= a.tiles; };
-  if (a.list) {
-    return launch_few<T, DH, 2>(a, plan_warps(a, blocks, kResident), s);
-  }
+  if (a.list) return launch_few<T, DH, 2>(a, plan_warps(a, blocks, kResident), s);
   const int form = debug_cache_form();
-  if (form == 2 || (form == 0 && a.rows > 8)) {
-    const long units = a.units * ((a.rows + kRows - 1) / kRows);
-    double least = kFewStart + cost.few * (double)(a.units * ((a.rows + 8 / kParts - 1) / (8 / kParts))) * (double)blocks;
-    int splits = 0;
-    for (int n = 1; n <= 8; n *= 2) {
-      const double t = row_tiles_time(cost, units, blocks, n);
-      if (t < least || (form == 2 && !splits)) least = t, splits = n;
-    }
-    if (splits) {
-      tiles(kRows);
-      a.splits = splits;
-      if constexpr (kParts == 1)
-        return launch_cache_attn_tc(a, s);
-      else
+  if (form >= 2 || (form == 0 && a.rows > 8)) {
+    const double few = kFewStart + few_cost<T, DH>() * (double)(a.units * ((a.rows + 8 / kParts - 1) / (8 / kParts))) * (double)blocks;
+    constexpr TileCost tc = tc_cost<T, DH>();
+    int tc_splits = 1;
+    const double tc_time = tiles_time(tc, a, blocks, tc_splits);
+    if constexpr (kParts == 2) {
+      constexpr TileCost rows = rows_cost<DH>();
+      int splits = 1;
+      const double time = tiles_time(rows, a, blocks, splits);
+      if (form == 2 || (form == 0 && time < tc_time && time < few)) {
+        tiles(rows.rows);
+        a.splits = splits;
         return launch_rows<DH>(a, s);
+      }
+    }
+    if (form >= 2 || tc_time < few) {
+      tiles(tc.rows);
+      a.splits = tc_splits;
+      return launch_cache_attn_tc<T>(a, s);
     }
   }
   const bool eight = kParts == 1 && a.rows > 4;

@@ -29,6 +29,7 @@ constexpr int kSms = 148;
 // numerators: below it codes count as much as they would at it, an error of 2^-20 of the largest value.
 constexpr float kLeastRatio = 9.5367431640625e-7f;
 
+template <typename T>
 int launch_cache_attn_tc(const AttnArgs& a, cudaStream_t s);
 int64_t by_block_workspace(const artab_cache* c, int n_streams, int n_q, int n_list);
 int launch_cache_by_block(int dtype, const AttnArgs& a, void* workspace, cudaStream_t s);

@@ -1,19 +1,19 @@
-// Attention over the 8-bit context cache for many query rows of bf16, on the 5th-generation tensor cores.
+// Attention over the 8-bit context cache for many query rows, on the 5th-generation tensor cores.
 //
 // The formulas are those of cache_attn.cu.  One CTA = 128 query rows of a (group, head) and a share of its blocks of 64 rows,
 // 384 threads:
 //   warps 0-3, 4-7   two softmax warpgroups; a thread owns one query row (TMEM lane).  Each warpgroup takes every other
 //                    block, with scores, numerators and an output accumulator of its own in tensor memory, a running
 //                    reference and sum in registers: the two meet only at the end, like two key splits
-//   warps 8, 9       turn codes into half-precision tiles (K-major, swizzled) of a ring of four blocks
+//   warps 8, 9       turn codes into half-precision tiles (K-major, swizzled) of a ring of four blocks (three where four do not fit)
 //   warps 10, 11     issue the MMAs of one warpgroup each, by an elected lane of a warp that walks and waits as a whole
 // S = Q . codes^T is M 128, N 64; O += P . codes is M 128, N = Dh with P from tensor memory.  All operands are halves:
 // queries of bf16 are exact in them (scaled by a power of two per row), codes are whole numbers, numerators keep
-// 11 bits.  Scales of keys go into the exponent's factor, scales of values into its offset (relative to the largest of the
+// 11 bits.  fp32: queries and numerators in two parts of 11 bits, each product once per part into the same accumulator.  Scales of keys go into the exponent's factor, scales of values into its offset (relative to the largest of the
 // context, taken out of the row sum again), so O accumulates over all blocks.
-// Two CTAs share an SM (256 TMEM columns each), so four warpgroups are in different phases of their blocks.  head_dim 64 has
-// no room for P beside S: it overwrites the scores it came from, and the next scores wait for P . V.
-// Measured (B200), 8192 queries x 8192 rows x 6 heads: head size 32 176 us (292 TFLOP/s, 2.28e12 exponentials a second),
+// Two CTAs share an SM (256 TMEM columns each), so four warpgroups are in different phases of their blocks.  Head size 64
+// and two parts have no room for P beside S: it overwrites the scores it came from, and the next scores wait for P . V.
+// Measured (B200), bf16, 8192 queries x 8192 rows x 6 heads: head size 32 176 us (292 TFLOP/s, 2.28e12 exponentials a second),
 // 16 162 us, 64 213 us (484 TFLOP/s); 87 us is what the special-function units need for the exponentials.  They are 63 % busy,
 // issue slots 57 % (of some 440 instructions a warp and block 160 are the 64 numerators' own), the tensor pipe 15 %.  Two
 // warpgroups alone on an SM take 2200 cycles a block each, four 3400: latency of a chain of loads, exponentials, stores and
@@ -23,13 +23,14 @@
 // both halves of a block unrolled, the next scores as soon as these are read 208 -> 176.  A share of the exponentials on the FMA
 // pipe (degree four, packed pairs) cost more issue slots than it freed at every share: 242 us with none, 246 with an eighth,
 // 255 with a quarter of them.
+// fp32, 4096 queries x 8192 rows x 6 heads: size 32 149 us (register tiles of cache_attn.cu 227), 16 144 (164), 64 162 (380).
 // Every wait is bounded; a CTA that gives up writes NaN for its rows.
 #include "cache_attn.cuh"
 
 namespace artab {
 namespace {
 
-constexpr int BM = 128, BN = kCacheBlock, kStages = 4, kAhead = 3, kThreads = 384, kConvert = 64;
+constexpr int BM = 128, BN = kCacheBlock, kAhead = 3, kThreads = 384, kConvert = 64;
 constexpr uint32_t kTmemCols = 256;
 // numerators are 2^6 times exp(s - reference)
 constexpr float kLiftTc = 6.0f;
@@ -38,18 +39,31 @@ struct Ctl {
   int abort_flag, pad;
   long long limit;
 };
-template <int DH>
+// Tensor memory of a warpgroup: scores, numerators (packed halves), output.  One part of the numerators has columns of its own
+// where there is room; else numerators overwrite scores, those of 32 scores the columns of these: one part of both halves the
+// upper 32, two parts (fp32) the 16 + 16 columns of their own half.
+template <typename T, int DH>
+struct Plan {
+  static constexpr int kParts = sizeof(T) == 4 ? 2 : 1;
+  static constexpr bool kAlias = DH == 64 || kParts == 2;
+  static constexpr uint32_t kColO = kAlias ? BN : BN + BN / 2, kColsWg = kTmemCols / 2;
+  static constexpr int kStages = DH == 64 && kParts == 2 ? 3 : 4;     // two CTAs in 227 KB
+  // column of part `part` of the numerators of scores 32 c ..
+  static constexpr uint32_t col_p(int c, int part) { return kParts == 2 ? 32 * c + 16 * part : (kAlias ? BN / 2 : BN) + 16 * c; }
+};
+template <typename T, int DH>
 struct __align__(1024) TcSmem {
-  uint8_t k[kStages][BN * DH * 2];       // [64 rows][DH] halves
-  uint8_t v[kStages][DH * 128];          // [DH][64 rows] halves
-  uint8_t q[BM * DH * 2];
-  uint8_t raw[kAhead][2 * BN * DH];      // records as they are kept
-  uint64_t q_full, kv_full[kStages], kv_empty[kStages];
+  using Pl = Plan<T, DH>;
+  uint8_t k[Pl::kStages][BN * DH * 2];       // [64 rows][DH] halves
+  uint8_t v[Pl::kStages][DH * 128];          // [DH][64 rows] halves
+  uint8_t q[Pl::kParts][BM * DH * 2];
+  uint8_t raw[kAhead][2 * BN * DH];          // records as they are kept
+  uint64_t q_full, kv_full[Pl::kStages], kv_empty[Pl::kStages];
   uint64_t s_full[2], s_free[2], p_full[2], o_full[2];
   float vmax[kThreads / 32];
   uint32_t tmem_base;
   Ctl ctl;
-  static constexpr int kFree = kStages * (BN * DH * 2 + DH * 128) + BM * DH * 2;   // bytes that the merge may use
+  static constexpr int kFree = Pl::kStages * (BN * DH * 2 + DH * 128) + Pl::kParts * BM * DH * 2;   // bytes that the merge may use
 };
 
 __device__ __forceinline__ void mbar_init(uint64_t* b, uint32_t count) {
@@ -204,16 +218,9 @@ __device__ __forceinline__ float2 pk_add(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
-// Tensor memory of a warpgroup: scores, numerators (packed halves), output.
-template <int DH>
-struct Plan {
-  static constexpr bool kAlias = DH == 64;           // numerators in the columns of the scores
-  static constexpr uint32_t kColP = kAlias ? BN / 2 : BN, kColO = kAlias ? BN : BN + BN / 2, kColsWg = kTmemCols / 2;
-};
-
-// Numerators of 32 scores of this thread's row against the reference m: packed halves, and their sum.
-template <bool MASKED>
-__device__ __forceinline__ float numerators(const uint32_t (&r)[32], uint32_t (&pk)[16], float slope, float add, int live) {
+// Numerators of 32 scores of this thread's row against the reference m: packed halves (in one part or two), and their sum.
+template <bool MASKED, int PARTS>
+__device__ __forceinline__ float numerators(const uint32_t (&r)[32], uint32_t (&pk)[PARTS][16], float slope, float add, int live) {
   const float2 sl2 = make_float2(slope, slope), add2 = make_float2(add, add);
   float2 sums[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
@@ -225,7 +232,9 @@ __device__ __forceinline__ float numerators(const uint32_t (&r)[32], uint32_t (&
       if (e + 1 >= live) y.y = 0.0f;
     }
     sums[(e >> 1) & 1] = pk_add(sums[(e >> 1) & 1], y);
-    pk[e >> 1] = h2_bits(__floats2half2_rn(y.x, y.y));
+    const __half2 hi = __floats2half2_rn(y.x, y.y);
+    pk[0][e >> 1] = h2_bits(hi);
+    if constexpr (PARTS == 2) pk[1][e >> 1] = h2_bits(__floats2half2_rn(y.x - __low2float(hi), y.y - __high2float(hi)));
   }
   return (sums[0].x + sums[1].x) + (sums[0].y + sums[1].y);
 }
@@ -249,17 +258,18 @@ __device__ __forceinline__ float largest(const uint32_t (&r)[32], int live) {
 // scores, m rises by a whole number k and all that was taken against it shrinks by 2^-k, exactly: sums, the numerators
 // that are in tensor memory, the output.  The result does not depend on m.
 constexpr float kMostSum = 60000.0f;
-template <int DH, bool MASKED>
-__device__ __forceinline__ bool softmax_block(TcSmem<DH>* sm, uint32_t t_row, int wg, int i, float slope, float lift,
+template <typename T, int DH, bool MASKED>
+__device__ __forceinline__ bool softmax_block(TcSmem<T, DH>* sm, uint32_t t_row, int wg, int i, float slope, float lift,
                                               float unlift, int live, float& m, float& l) {
-  constexpr bool kAlias = Plan<DH>::kAlias;
-  constexpr uint32_t kColP = Plan<DH>::kColP, kColO = Plan<DH>::kColO;
+  using Pl = Plan<T, DH>;
+  constexpr bool kAlias = Pl::kAlias;
+  constexpr uint32_t kColO = Pl::kColO;
   volatile Ctl* ctl = &sm->ctl;
   bool ok = true;
   float sum = 0.0f;
 #pragma unroll
   for (int c = 1; c >= 0; --c) {
-    uint32_t r[32], pk[16];
+    uint32_t r[32], pk[Pl::kParts][16];
     tmem_ld32(t_row + 32 * c, r);
     wait_ld();
     const int lv = live - 32 * c;
@@ -269,7 +279,7 @@ __device__ __forceinline__ bool softmax_block(TcSmem<DH>* sm, uint32_t t_row, in
     }
     if (i == 0 && c == 1) m = MASKED && lv <= 0 ? m : largest<MASKED>(r, lv) * slope;   // no row of these in use: not yet
     if (MASKED && i == 0 && c == 0 && live <= 32) m = largest<MASKED>(r, lv) * slope;
-    float part = numerators<MASKED>(r, pk, slope, lift - m, lv);
+    float part = numerators<MASKED, Pl::kParts>(r, pk, slope, lift - m, lv);
     if (c == 1 && i > 0) {                        // the P . V before this one has read P and written O
       if (!kAlias) ok = __all_sync(0xffffffffu, mbar_wait(&sm->o_full[wg], (i - 1) & 1, ctl));
       fence_after();
@@ -283,18 +293,21 @@ __device__ __forceinline__ bool softmax_block(TcSmem<DH>* sm, uint32_t t_row, in
       if (!(part < kMostSum)) k = fmaxf(ceilf(largest<MASKED>(r, lv) * slope - m), 0.0f);
       m += k;
       const float alpha = ex2(-k);
-      part = numerators<MASKED>(r, pk, slope, lift - m, lv);
+      part = numerators<MASKED, Pl::kParts>(r, pk, slope, lift - m, lv);
       l *= alpha;
       sum *= alpha;
       if (c == 0) {                               // the other half of this block's numerators
-        uint32_t u[16];
-        wait_st();
-        tmem_ld16(t_row + kColP + 16, u);
-        wait_ld();
         const __half2 al = __float2half2_rn(alpha);
+        wait_st();
+#pragma unroll 1
+        for (int part = 0; part < Pl::kParts; ++part) {
+          uint32_t u[16];
+          tmem_ld16(t_row + Pl::col_p(1, part), u);
+          wait_ld();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) u[e] = h2_bits(__hmul2(*reinterpret_cast<const __half2*>(&u[e]), al));
-        tmem_st16(t_row + kColP + 16, u);
+          for (int e = 0; e < 16; ++e) u[e] = h2_bits(__hmul2(*reinterpret_cast<const __half2*>(&u[e]), al));
+          tmem_st16(t_row + Pl::col_p(1, part), u);
+        }
       }
       if (i > 0) {
 #pragma unroll 1
@@ -310,7 +323,8 @@ __device__ __forceinline__ bool softmax_block(TcSmem<DH>* sm, uint32_t t_row, in
       }
     }
     sum += part;
-    tmem_st16(t_row + kColP + 16 * c, pk);
+#pragma unroll
+    for (int part = 0; part < Pl::kParts; ++part) tmem_st16(t_row + Pl::col_p(c, part), pk[part]);
   }
   l = fmaf(sum, unlift, l);
   wait_st();
@@ -319,13 +333,15 @@ __device__ __forceinline__ bool softmax_block(TcSmem<DH>* sm, uint32_t t_row, in
   return ok;
 }
 
-template <int DH>
+template <typename T, int DH>
 __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnArgs a, long long wait_cycles, int drop_commits) {
-  constexpr bool kAlias = Plan<DH>::kAlias;
-  constexpr uint32_t kColP = Plan<DH>::kColP, kColO = Plan<DH>::kColO, kColsWg = Plan<DH>::kColsWg;
+  using Pl = Plan<T, DH>;
+  constexpr bool kAlias = Pl::kAlias;
+  constexpr int kStages = Pl::kStages;
+  constexpr uint32_t kColO = Pl::kColO, kColsWg = Pl::kColsWg;
   constexpr int KS = DH / 16, P = kPartial<DH>, KB = DH * 2;
   extern __shared__ uint8_t smem_raw[];
-  using S = TcSmem<DH>;
+  using S = TcSmem<T, DH>;
   S* sm = reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   // the warp's number from its first lane: what follows from it is then known to be the same for all lanes, and an MMA takes
   // its operands from uniform registers as they are
@@ -389,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
     for (int i = 0; i < DH; ++i) x[i] = 0.0f;
     const int r = row0 + row;
     if (r < a.rows)
-      load_elements<__nv_bfloat16, DH>(reinterpret_cast<const __nv_bfloat16*>(a.q.p) + stream_of(r) * a.q.s0 + h * a.q.s1 +
+      load_elements<T, DH>(reinterpret_cast<const T*>(a.q.p) + stream_of(r) * a.q.s0 + h * a.q.s1 +
                                            query_of(r) * a.q.s2, a.vec_q, x);
     float top = 0.0f, to, back;
 #pragma unroll
@@ -400,10 +416,17 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
     if (wg == 0) {
 #pragma unroll
       for (int c = 0; c < DH / 8; ++c) {
-        uint32_t u[4];
+        uint32_t u[Pl::kParts][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = h2_bits(__floats2half2_rn(x[8 * c + 2 * i] * to, x[8 * c + 2 * i + 1] * to));
-        *reinterpret_cast<uint4*>(sm->q + swizzled<KB>(row, c)) = make_uint4(u[0], u[1], u[2], u[3]);
+        for (int i = 0; i < 4; ++i) {
+          const float y = x[8 * c + 2 * i] * to, z = x[8 * c + 2 * i + 1] * to;
+          const __half2 hi = __floats2half2_rn(y, z);
+          u[0][i] = h2_bits(hi);
+          if constexpr (Pl::kParts == 2) u[1][i] = h2_bits(__floats2half2_rn(y - __low2float(hi), z - __high2float(hi)));
+        }
+#pragma unroll
+        for (int part = 0; part < Pl::kParts; ++part)
+          *reinterpret_cast<uint4*>(sm->q[part] + swizzled<KB>(row, c)) = make_uint4(u[part][0], u[part][1], u[part][2], u[part][3]);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -437,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
     // ------------------------------ MMA issuers ------------------------------
     // The whole warp walks and waits, one lane issues.
     const int w = warp - 10, n = (nb - w + 1) / 2;
-    const uint32_t t_wg = tmem + w * kColsWg, q_addr = smem_u32(sm->q);
+    const uint32_t t_wg = tmem + w * kColsWg, q_addr = smem_u32(sm->q[0]);
     const auto wait = [&](uint64_t* bar, uint32_t parity) {
       const bool done = __all_sync(0xffffffffu, mbar_wait(bar, parity, ctl));
       if (done) fence_after();
@@ -449,8 +472,11 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
       const uint32_t k_addr = smem_u32(sm->k[st]);
       if (elected()) {
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-          umma_ss(t_wg, tile_desc<KB>(q_addr + 32 * ks), tile_desc<KB>(k_addr + 32 * ks), idesc(BM, BN), ks);
+        for (int part = 0; part < Pl::kParts; ++part)
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks)
+            umma_ss(t_wg, tile_desc<KB>(q_addr + part * BM * KB + 32 * ks), tile_desc<KB>(k_addr + 32 * ks), idesc(BM, BN),
+                    part + ks);
         if (!drop_commits) umma_commit(&sm->s_full[w]);
       }
       __syncwarp();
@@ -468,8 +494,11 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
       const uint32_t v_addr = smem_u32(sm->v[st]);
       if (elected()) {
 #pragma unroll
-        for (int ks = 0; ks < BN / 16; ++ks)
-          umma_ts(t_wg + kColO, t_wg + kColP + 8 * ks, tile_desc<128>(v_addr + 32 * ks), idesc(BM, DH), i > 0 || ks > 0);
+        for (int part = 0; part < Pl::kParts; ++part)
+#pragma unroll
+          for (int ks = 0; ks < BN / 16; ++ks)
+            umma_ts(t_wg + kColO, t_wg + Pl::col_p(ks >> 1, part) + 8 * (ks & 1), tile_desc<128>(v_addr + 32 * ks), idesc(BM, DH),
+                    i > 0 || part + ks > 0);
         umma_commit(&sm->o_full[w]);
         umma_commit(&sm->kv_empty[st]);
       }
@@ -541,8 +570,8 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
       ok = __all_sync(0xffffffffu, mbar_wait(&sm->s_full[wg], i & 1, ctl));
       if (!ok) break;
       fence_after();
-      ok = live < BN ? softmax_block<DH, true>(sm, t_row, wg, i, slope, lift, unlift, live, m, l)
-                     : softmax_block<DH, false>(sm, t_row, wg, i, slope, lift, unlift, BN, m, l);
+      ok = live < BN ? softmax_block<T, DH, true>(sm, t_row, wg, i, slope, lift, unlift, live, m, l)
+                     : softmax_block<T, DH, false>(sm, t_row, wg, i, slope, lift, unlift, BN, m, l);
       if (!ok) break;
     }
     if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sm->o_full[wg], (steps - 1) & 1, ctl));
@@ -582,22 +611,25 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
     __syncthreads();
   else
     cluster_meet();
-  merge_rows<__nv_bfloat16, DH>(a, smem_u32(part), 2, rank * kThreads + tid, a.splits * kThreads, BM, row0, h, group, kLiftTc);
+  merge_rows<T, DH>(a, smem_u32(part), 2, rank * kThreads + tid, a.splits * kThreads, BM, row0, h, group, kLiftTc);
   if (a.splits > 1) cluster_meet();
 }
 
 }  // namespace
 
-template <int DH>
+template <typename T, int DH>
 static int launch_tc(const AttnArgs& a, cudaStream_t s) {
   static SmemConfig config;
-  static_assert(TcSmem<DH>::kFree >= 2 * BM * kPartial<DH> * 4, "the merge fits where the tiles were");
+  static_assert(TcSmem<T, DH>::kFree >= 2 * BM * kPartial<DH> * 4, "the merge fits where the tiles were");
   const long long limit = debug_wait_cycles() ? debug_wait_cycles() : kDefaultWaitCycles;
-  return launch_attn(cache_attn_tc_kernel<DH>, config, sizeof(TcSmem<DH>) + 1024, kThreads, a, s, limit, debug_drop_score_commits());
+  return launch_attn(cache_attn_tc_kernel<T, DH>, config, sizeof(TcSmem<T, DH>) + 1024, kThreads, a, s, limit, debug_drop_score_commits());
 }
 
+template <typename T>
 int launch_cache_attn_tc(const AttnArgs& a, cudaStream_t s) {
-  return a.c.head_dim == 16 ? launch_tc<16>(a, s) : a.c.head_dim == 32 ? launch_tc<32>(a, s) : launch_tc<64>(a, s);
+  return a.c.head_dim == 16 ? launch_tc<T, 16>(a, s) : a.c.head_dim == 32 ? launch_tc<T, 32>(a, s) : launch_tc<T, 64>(a, s);
 }
+template int launch_cache_attn_tc<float>(const AttnArgs&, cudaStream_t);
+template int launch_cache_attn_tc<__nv_bfloat16>(const AttnArgs&, cudaStream_t);
 
 }  // namespace artab

@@ -470,8 +470,9 @@ ARTAB_API void artab_set_dependent_launch(int on);
  *                                  the kernel returns normally, status is non-zero, `out` untouched.  The same in
  *                                  artab_cache_attention's tensor-core form, which writes NaN to out and lse instead.
  *   ARTAB_DEBUG_CACHE_FORM         which kernels serve the 8-bit context cache: 0 by their cost; 1 attention a few rows at
- *                                  a time and listed blocks one by one; 2 attention in tiles of many rows and listed
- *                                  blocks block by block (as far as a workspace is handed over).  Results are the same up to rounding. */
+ *                                  a time and listed blocks one by one; 2 attention in tiles of many rows (fp32: register
+ *                                  tiles) and listed blocks block by block (as far as a workspace is handed over); 3 as 2,
+ *                                  the tiles on tcgen05 for fp32 too.  Results are the same up to rounding. */
 #define ARTAB_DEBUG_WAIT_CYCLES 0
 #define ARTAB_DEBUG_DROP_SCORE_COMMITS 1
 #define ARTAB_DEBUG_CACHE_FORM 2

@@ -23,12 +23,12 @@ def cc():
     return context_cache
 
 
-@pytest.fixture(params=["by_cost", "few_rows", "row_tiles"])
+@pytest.fixture(params=["by_cost", "few_rows", "row_tiles", "tensor_tiles"])
 def form(request):
-    """Attention by the kernels that their cost picks, and by either kind whatever the sizes."""
+    """Attention by the kernels that their cost picks, and by each kind whatever the sizes."""
     from ar_tabpfn import _lib
     lib = _lib.lib()
-    _lib.check(lib.artab_debug_set(_lib.DEBUG_CACHE_FORM, ("by_cost", "few_rows", "row_tiles").index(request.param)))
+    _lib.check(lib.artab_debug_set(_lib.DEBUG_CACHE_FORM, ("by_cost", "few_rows", "row_tiles", "tensor_tiles").index(request.param)))
     yield request.param
     lib.artab_debug_set(_lib.DEBUG_CACHE_FORM, 0)
 
@@ -671,14 +671,15 @@ def test_offsets_beyond_32_bits():
     assert bool(((lse[-1:] - rlse).abs() <= 1e-4).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
 @pytest.mark.parametrize("D", [16, 32, 64])
-def test_a_wait_that_runs_out_gives_nan_and_the_next_call_is_right(D):
-    """The tensor-core form of many bf16 queries with its "scores ready" signal withheld and a limit of 0.1 ms."""
+def test_a_wait_that_runs_out_gives_nan_and_the_next_call_is_right(D, dtype):
+    """The tensor-core form of many queries with its "scores ready" signal withheld and a limit of 0.1 ms."""
     from ar_tabpfn import _lib
     c, lib = cc(), _lib.lib()
-    k, v = rows(80, 1, 6, 6000, D, torch.bfloat16)
+    k, v = rows(80, 1, 6, 6000, D, dtype)
     cache = c.quantize_context(k, v)
-    q = torch.randn(3000, 6, 1, D, device="cuda", generator=gen(81)).bfloat16()   # far beyond the few-row kernel's range
+    q = torch.randn(3000, 6, 1, D, device="cuda", generator=gen(81)).to(dtype)   # far beyond the few-row kernel's range
     want = c.context_cache_attention(q, cache)
     try:
         _lib.check(lib.artab_debug_set(_lib.DEBUG_WAIT_CYCLES, 200_000))
