@@ -46,9 +46,10 @@ class ContextCache:
       lens    int32 [G]: rows in use.  Kernels read it on the device
 
     They are worked on in place, where they are now: another tensor put in a field's place is not seen.
-    ``length``: a bound of ``lens`` known to the host (default: the capacity)."""
+    ``length``: a bound of ``lens`` known to the host (default: the capacity).  A captured ``append_context`` counts once
+    in it, however often it is replayed; appending and reading outside a capture then look ``lens`` up."""
 
-    __slots__ = ("codes", "scales", "bounds", "lens", "length", "n_groups", "n_heads", "head_dim", "capacity", "_c", "_ref")
+    __slots__ = ("codes", "scales", "bounds", "lens", "length", "n_groups", "n_heads", "head_dim", "capacity", "captured", "_c", "_ref")
 
     def __init__(self, codes: Tensor, scales: Tensor, bounds: Tensor, lens: Tensor, length: Optional[int] = None):
         shape = codes.shape
@@ -73,6 +74,7 @@ class ContextCache:
         self.codes, self.scales, self.bounds, self.lens = codes, scales, bounds, lens
         self.n_groups, self.n_heads, self.head_dim, self.capacity = G, H, Dh, blocks * CONTEXT_BLOCK
         self.length = self.capacity if length is None else min(int(length), self.capacity)
+        self.captured = False      # a graph may have moved lens since `length` was set
         self._c = _lib.Cache(G, H, Dh, blocks, codes.data_ptr(), scales.data_ptr(), bounds.data_ptr(), lens.data_ptr())
         self._ref = C.byref(self._c)
 
@@ -193,6 +195,10 @@ def quantize_context(k_ctx: Tensor, v_ctx: Tensor, lens: Optional[Lengths] = Non
     return cache
 
 
+def _look_up(cache: ContextCache) -> None:
+    cache.length = min(max(int(cache.lens.max()), 0), cache.capacity)
+
+
 def append_context(cache: ContextCache, k_new: Tensor, v_new: Tensor, counts: Optional[Lengths] = None,
                    start: Optional[Lengths] = None) -> None:
     """Put rows k_new / v_new [G,H,n,Dh] ([H,n,Dh] for a shared context) behind those in use, in place.
@@ -213,19 +219,23 @@ def append_context(cache: ContextCache, k_new: Tensor, v_new: Tensor, counts: Op
     if n == 0 and start is None:
         return
     with _Launch(k.get_device()) as (lib, stream):
+        capturing = torch.cuda.is_current_stream_capturing()
+        if cache.captured and not capturing:
+            _look_up(cache)
         if start is None and cache.length + n > cache.capacity:
             # the bound that the host keeps may be too high: contexts that took fewer rows, a cache put together from tensors
-            if torch.cuda.is_current_stream_capturing():
+            if capturing:
                 raise ValueError("append_context: the cache may be full, and its lengths cannot be looked up during capture")
             room = cache.lens if counts is None else cache.lens + counts.clamp(0, n)
-            cache.length = min(int(cache.lens.max()), cache.capacity)
+            _look_up(cache)
             if int(room.max()) + (n if counts is None else 0) > cache.capacity:
                 raise ValueError("append_context: context cache exceeded; increase its capacity")
         if n == 0:
             k = v = cache.scales.new_empty(G, H, 1, Dh)      # nothing is read from it: start alone takes effect
             counts = torch.zeros(G, dtype=torch.int32, device=k.device)
         _write(lib, stream, cache, code, k, v, start, counts, 0)
-    cache.length = min(cache.length + n, cache.capacity)
+        cache.length = min(cache.length + n, cache.capacity)
+        cache.captured = cache.captured or capturing
 
 
 def read_context(cache: ContextCache, start: Optional[Lengths] = None, n: Optional[int] = None,
@@ -234,7 +244,13 @@ def read_context(cache: ContextCache, start: Optional[Lengths] = None, n: Option
     ``cache.length``).  Rows that are not in use are zero."""
     code = _lib.dtype_code(dtype)
     G, H, Dh = cache.n_groups, cache.n_heads, cache.head_dim
-    n = cache.length if n is None else int(n)
+    if n is None:
+        if cache.captured:
+            with _Launch(cache.codes.get_device()):
+                if not torch.cuda.is_current_stream_capturing():
+                    _look_up(cache)
+        n = cache.length
+    n = int(n)
     if n < 0:
         raise ValueError(f"read_context: {n} rows")
     start = _lengths(start, G, cache.device, "start")

@@ -207,3 +207,22 @@ def test_the_library_refuses_what_does_not_fit_without_a_device():
     assert lib.artab_cache_block_attention(0, p, st, 4096, 2, one, p, 8, 1.0, p, p, p, need - 1, None) == -2
     assert lib.artab_cache_block_attention(0, p, st, 4096, 2, one, p, 8, 1.0, p, p, p + 4, need, None) == -1
     assert b"cache" in lib.artab_last_error()
+
+
+def test_replayed_rows_are_counted_too(fake, monkeypatch):
+    """A graph that appends moves lens, not what the host knows of it."""
+    c = cc.ContextCache(**tensors(), length=80)
+    x = torch.zeros(G, H, 10, D)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    cc.append_context(c, x, x)
+    cc.append_context(c, x, x)                              # two steps of one graph
+    assert c.length == 100 and len(fake.calls) == 2
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    c.lens.fill_(125)                                       # what replays have left
+    with pytest.raises(ValueError, match="capacity"):
+        cc.append_context(c, x, x)
+    assert len(fake.calls) == 2
+    assert cc.read_context(c)[0].shape[2] == 125
+    c.lens.fill_(118)
+    cc.append_context(c, x, x)
+    assert c.length == 128 and len(fake.calls) == 4
