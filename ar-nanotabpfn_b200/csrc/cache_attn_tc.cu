@@ -24,7 +24,7 @@
 // pipe (degree four, packed pairs) cost more issue slots than it freed at every share: 242 us with none, 246 with an eighth,
 // 255 with a quarter of them.
 // fp32, 4096 queries x 8192 rows x 6 heads: size 32 149 us (register tiles of cache_attn.cu 227), 16 144 (164), 64 162 (380).
-// Every wait is bounded; a CTA that gives up writes NaN for its rows.
+// Every wait is bounded; a CTA that gives up lets its MMAs end, frees its tensor memory and writes NaN for its rows.
 #include "cache_attn.cuh"
 
 namespace artab {
@@ -59,7 +59,7 @@ struct __align__(1024) TcSmem {
   uint8_t q[Pl::kParts][BM * DH * 2];
   uint8_t raw[kAhead][2 * BN * DH];          // records as they are kept
   uint64_t q_full, kv_full[Pl::kStages], kv_empty[Pl::kStages];
-  uint64_t s_full[2], s_free[2], p_full[2], o_full[2];
+  uint64_t s_full[2], s_free[2], p_full[2], o_full[2], drained[2];
   float vmax[kThreads / 32];
   uint32_t tmem_base;
   Ctl ctl;
@@ -374,6 +374,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
       mbar_init(&sm->s_free[w], BM);
       mbar_init(&sm->p_full[w], BM);
       mbar_init(&sm->o_full[w], 1);
+      mbar_init(&sm->drained[w], 1);
     }
     sm->ctl.abort_flag = 0;
     sm->ctl.limit = wait_cycles;
@@ -505,6 +506,12 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
       __syncwarp();
       if (kAlias && i + 1 < n)                        // P lies where the next scores go
         ok = wait(&sm->o_full[w], i & 1) && scores(i + 1);
+    }
+    // no MMA outlives its operands and its tensor memory, whether or not the CTA is giving up
+    if (elected()) umma_commit(&sm->drained[w]);
+    __syncwarp();
+    const uint32_t drained = smem_u32(&sm->drained[w]);
+    for (const long long t0 = clock64(); !mbar_tries(drained, 0) && clock64() - t0 < kDefaultWaitCycles;) {
     }
   } else if (warp >= 8) {
     // ------------------------- codes into operand tiles -------------------------
