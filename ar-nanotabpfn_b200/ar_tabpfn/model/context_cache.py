@@ -31,6 +31,8 @@ from torch import Tensor
 from .. import _lib
 
 CONTEXT_BLOCK = 64
+_MOST_ROWS = 1 << 30          # of a cache; also of a call
+_MOST_LISTED = (1 << 31) - 1
 _Strides = C.c_int64 * 3
 Lengths = Union[Tensor, Sequence[int]]
 
@@ -141,6 +143,8 @@ def _lengths(x: Optional[Lengths], G: int, device: torch.device, what: str) -> O
         raise ValueError(f"{what} must be whole numbers")
     if x.shape != (G,):
         raise ValueError(f"{what} must have one entry per context: ({G},), not {tuple(x.shape)}")
+    if x.dtype is torch.int64:
+        x = x.clamp(-1, _MOST_LISTED)                        # what does not fit 32 bits stays out of range
     if x.dtype is not torch.int32 or x.device != device or not x.is_contiguous():
         x = x.to(device=device, dtype=torch.int32).contiguous()
     return x
@@ -152,6 +156,8 @@ def _rows_of(k: Tensor, v: Tensor, what: str) -> Tuple[Tensor, Tensor, int]:
         k, v = k.unsqueeze(0), v.unsqueeze(0)
     if k.dim() != 4 or v.shape != k.shape:
         raise ValueError(f"{what}: keys {tuple(k.shape)} and values {tuple(v.shape)} must both be [H,N,Dh] or [G,H,N,Dh]")
+    if k.shape[2] > _MOST_ROWS:
+        raise ValueError(f"{what}: {k.shape[2]} rows at once")
     if v.dtype is not k.dtype:
         raise ValueError(f"{what}: keys are {k.dtype}, values {v.dtype}")
     code = _lib.dtype_code(k.dtype)
@@ -181,7 +187,7 @@ def quantize_context(k_ctx: Tensor, v_ctx: Tensor, lens: Optional[Lengths] = Non
     if Dh not in (16, 32, 64):
         raise ValueError(f"quantize_context: head_dim {Dh} not supported (16, 32, 64)")
     capacity = N if capacity is None else int(capacity)
-    if capacity < max(N, 1) or G < 1 or H < 1:
+    if not max(N, 1) <= capacity <= _MOST_ROWS or G < 1 or H < 1:
         raise ValueError(f"quantize_context: no room for {N} rows of {G} x {H} heads in a capacity of {capacity}")
     counts = _lengths(lens, G, k.device, "lens")
     blocks = (capacity + CONTEXT_BLOCK - 1) // CONTEXT_BLOCK
@@ -251,7 +257,7 @@ def read_context(cache: ContextCache, start: Optional[Lengths] = None, n: Option
                     _look_up(cache)
         n = cache.length
     n = int(n)
-    if n < 0:
+    if not 0 <= n <= _MOST_ROWS:
         raise ValueError(f"read_context: {n} rows")
     start = _lengths(start, G, cache.device, "start")
     k = cache.scales.new_empty((G, H, n, Dh), dtype=dtype)
@@ -299,7 +305,7 @@ def select_context_blocks(q: Tensor, cache: ContextCache, n_blocks: int) -> Tens
     bounds go to the lower index.  A query that is not finite gets the first blocks.  Capacities of up to 221184 rows."""
     (B, H, Lq, _), code, device = _queries(q, cache, "select_context_blocks")
     n = int(n_blocks)
-    if n < 1:
+    if not 1 <= n <= _MOST_LISTED:
         raise ValueError(f"select_context_blocks: {n} blocks")
     index = q.new_empty((B, H, Lq, n), dtype=torch.int32)
     if B and Lq:
@@ -319,6 +325,8 @@ def block_context_attention(q: Tensor, cache: ContextCache, blocks: Tensor,
     shape = blocks.shape
     if len(shape) != 4 or shape[:3] != (B, H, Lq) or blocks.dtype is not torch.int32:
         raise ValueError(f"block_context_attention: blocks must be int32 [{B},{H},{Lq},S]")
+    if shape[3] > _MOST_LISTED:
+        raise ValueError(f"block_context_attention: {shape[3]} blocks a query")
     if blocks.get_device() != device:
         raise ValueError("block_context_attention: blocks must live on the device of the queries")
     out, lse = q.new_empty((B, H, Lq, Dh)), q.new_empty((B, H, Lq), dtype=torch.float32)

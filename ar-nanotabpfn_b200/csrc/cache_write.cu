@@ -13,6 +13,8 @@
 namespace artab {
 namespace {
 
+constexpr int kMostRows = 1 << 30;   // of a cache, or to write or read at once
+
 struct WriteArgs {
   artab_cache c;
   RowView k, v;
@@ -540,7 +542,7 @@ int check_cache(const artab_cache* c, const char* what) {
   ARTAB_REQUIRE(c->head_dim == 16 || c->head_dim == 32 || c->head_dim == 64, ARTAB_EINVAL,
                 "%s: head_dim %d not supported (16, 32, 64)", what, c->head_dim);
   ARTAB_REQUIRE(c->n_groups >= 1 && c->n_groups <= 65535 && c->n_heads >= 1 && c->n_heads <= 65535 && c->n_blocks >= 1 &&
-                    c->n_blocks <= (1 << 24),
+                    c->n_blocks <= kMostRows / kCacheBlock,
                 ARTAB_EINVAL, "%s: bad cache sizes", what);
   const uintptr_t bits = reinterpret_cast<uintptr_t>(c->codes) | reinterpret_cast<uintptr_t>(c->bounds);
   ARTAB_REQUIRE(bits % 16 == 0 && reinterpret_cast<uintptr_t>(c->scales) % 8 == 0, ARTAB_EINVAL,
@@ -560,7 +562,7 @@ int artab_cache_write(int dtype, const void* k, const int64_t* k_strides, const 
   int rc = check_cache(c, "cache_write");
   if (rc) return rc;
   ARTAB_REQUIRE(dtype == ARTAB_F32 || dtype == ARTAB_BF16, ARTAB_EINVAL, "cache_write: bad dtype %d", dtype);
-  ARTAB_REQUIRE(k && v && n_rows >= 1, ARTAB_EINVAL, "cache_write: no rows");
+  ARTAB_REQUIRE(k && v && n_rows >= 1 && n_rows <= kMostRows, ARTAB_EINVAL, "cache_write: bad number of rows");
   ARTAB_REQUIRE(!(fresh && start), ARTAB_EINVAL, "cache_write: a fresh cache starts at row 0");
   ARTAB_REQUIRE(!fresh || (n_rows + kCacheBlock - 1) / kCacheBlock <= c->n_blocks, ARTAB_ECAPACITY,
                 "cache_write: %d rows in a cache of %d", n_rows, c->n_blocks * kCacheBlock);
@@ -601,7 +603,7 @@ int artab_cache_read(int dtype, const artab_cache* c, const int32_t* start, int 
   int rc = check_cache(c, "cache_read");
   if (rc) return rc;
   ARTAB_REQUIRE(dtype == ARTAB_F32 || dtype == ARTAB_BF16, ARTAB_EINVAL, "cache_read: bad dtype %d", dtype);
-  ARTAB_REQUIRE(k && v && n_rows >= 1, ARTAB_EINVAL, "cache_read: no rows");
+  ARTAB_REQUIRE(k && v && n_rows >= 1 && n_rows <= kMostRows, ARTAB_EINVAL, "cache_read: bad number of rows");
   ARTAB_REQUIRE((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 == 0, ARTAB_EINVAL,
                 "cache_read: outputs must be 16-byte aligned");
   ReadArgs a;

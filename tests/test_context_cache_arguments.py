@@ -226,3 +226,22 @@ def test_replayed_rows_are_counted_too(fake, monkeypatch):
     c.lens.fill_(118)
     cc.append_context(c, x, x)
     assert c.length == 128 and len(fake.calls) == 4
+
+
+def test_sizes_beyond_32_bits_are_refused(fake):
+    c = cc.ContextCache(**tensors(), length=0)
+    x = torch.zeros(1).expand(G, H, 2 ** 32 + 5, D)
+    start = torch.zeros(G, dtype=torch.int32)
+    q = torch.zeros(G, H, 1, D)
+    listed = torch.zeros(1, dtype=torch.int32).expand(G, H, 1, 2 ** 32 + 1)
+    for match, call in (("rows at once", lambda: cc.append_context(c, x, x, start=start)),
+                        ("rows at once", lambda: cc.quantize_context(x, x)),
+                        ("no room", lambda: cc.quantize_context(x[:, :, :4], x[:, :, :4], capacity=2 ** 32 + 64)),
+                        ("4294967297 rows", lambda: cc.read_context(c, n=2 ** 32 + 1)),
+                        ("4294967297 blocks", lambda: cc.select_context_blocks(q, c, 2 ** 32 + 1)),
+                        ("4294967297 blocks", lambda: cc.block_context_attention(q, c, listed))):
+        with pytest.raises(ValueError, match=match):
+            call()
+    assert not fake.calls
+    counts = cc._lengths(torch.tensor([2 ** 32, -2 ** 40, 7]), G, q.device, "counts")
+    assert counts.dtype is torch.int32 and counts[0] >= 2 ** 30 and counts[1] < 0 and counts[2] == 7
