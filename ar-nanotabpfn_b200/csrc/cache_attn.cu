@@ -13,16 +13,13 @@
 // walks blocks of its own with a running maximum; its ring of records is filled by 16-byte asynchronous copies
 // and no warp waits for another until the end, where the warps of a unit and the CTAs of a cluster (up to eight
 // share the rows of a context) merge maximum, sum and output through shared memory.
-// Measured (B200), queries of one row each: 8 contexts x 65536 rows x 8 heads of size 64, 90 us for 537 MB (5.95 TB/s, 0.91
-// of a copy's rate; half of the issue slots busy, three ring stages instead of two 102 us: one CTA an SM either way), size 32
-// 50 us (5.4 TB/s), size 16 35 us (3.9 TB/s: 16 codes a lane between two shuffles); 64 x 2048 x 6 of size 32 14 us and one
-// context of 16384 rows 8.6 us: a chain of loads, products and merges.
+// Measured (B200), queries of one row each: 8 contexts x 65536 rows x 8 heads of size 64, 82.5 us for 537 MB (6.5 TB/s, 0.99
+// of a copy's rate; half of the issue slots busy), size 32 51 us (5.3 TB/s), size 16 36 us (3.8 TB/s: 16 codes a lane between two
+// shuffles); 64 x 2048 x 6 of size 32 14 us and one context of 8192 rows 7 us: a chain of loads, products and merges.
 #include "cache_tile.cuh"
 
 namespace artab {
 namespace {
-
-constexpr int kWarps = 8;         // of a unit, at most
 
 template <int DH>
 struct Ring {
@@ -37,22 +34,16 @@ constexpr int partial_floats() {
   return Tile<DH, PARTS>::ROWS * (DH + 2);
 }
 
-// W warps a CTA.  FORM 0: every block, a CTA (of a cluster) for a unit; 1: every block, several units a CTA; 2: listed blocks,
-// either way.
-template <typename T, int DH, int PARTS, int FORM, int W>
+// A unit is a tile of query rows of a (group, head), or (LIST) one query with its listed blocks: a CTA of W warps, or a cluster.
+template <typename T, int DH, int PARTS, bool LIST, int W>
 __global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnArgs a) {
-  constexpr bool LIST = FORM == 2;
   using R = Ring<DH>;
   using Tl = Tile<DH, PARTS>;
   constexpr int ROWS = LIST ? 1 : Tl::ROWS, P = DH + 2;
   extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int rank = (int)(blockIdx.x % a.splits);
-  const int per_cta = FORM ? a.per_cta : 1, warps = FORM ? W / per_cta : W;
-  long unit = blockIdx.x / a.splits;
-  if (FORM) unit = unit * per_cta + warp / warps;
-  const bool spare = FORM && unit >= a.units;                         // the last CTA may have warps without a unit
-  if (spare) unit = a.units - 1;
+  const long unit = blockIdx.x / a.splits;
   const int H = a.c.n_heads;
   int group, h, row0, n_rows;
   if (LIST) {
@@ -75,7 +66,7 @@ __global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnArgs a) {
   const int cap = a.c.n_blocks * kCacheBlock;
   len = len < 0 ? 0 : len > cap ? cap : len;
   const int held = (len + kCacheBlock - 1) / kCacheBlock;
-  const int n = spare ? 0 : LIST ? a.n_list : held;           // blocks of the unit
+  const int n = LIST ? a.n_list : held;                       // blocks of the unit
   const int32_t* list = LIST ? a.list + unit * a.n_list : nullptr;
   const size_t gh = (size_t)group * H + h;
   const uint8_t* codes = a.c.codes + gh * a.c.n_blocks * (size_t)R::kRecord;
@@ -83,7 +74,7 @@ __global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnArgs a) {
 
   uint8_t* ring = smem + warp * R::kBytes;
   const uint32_t ring_addr = smem_u32(ring);
-  const int first = rank * warps + (FORM ? warp % warps : warp), step = a.splits * warps;
+  const int first = rank * W + warp, step = a.splits * W;
   // block to fetch next; -1: nothing there.  Of a list, the lanes keep 32 entries of the warp's share
   int fetched = 0, entries = -1;
   const auto next_block = [&]() {
@@ -173,16 +164,14 @@ __global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnArgs a) {
   };
   const auto store = [&](int r, int d, float m, float l, float o) {
     const int row = row0 + r;
-    if (row >= n_rows || spare) return;
+    if (row >= n_rows) return;
     const size_t at = ((size_t)stream_of(row) * H + h) * a.n_q + query_of(row);
     reinterpret_cast<T*>(a.out)[at * DH + d] = from_f32<T>(l == 0.0f ? 0.0f : o / l);
     if (d == 0) a.lse[at] = l == 0.0f ? -CUDART_INF_F : (m - kLift) * kLn2 + logf(l);
   };
-  // the threads of a unit's warps write its results
-  const float* of_unit = part + (FORM ? warp / warps * warps : 0) * ROWS * P;
-  for (int e = FORM ? tid % (warps * 32) : tid; e < ROWS * DH; e += warps * 32) {
+  for (int e = tid; e < ROWS * DH; e += W * 32) {
     float m, l, o;
-    merge([&](int w, int i) { return of_unit[w * ROWS * P + i]; }, warps, e / DH, e % DH, m, l, o);
+    merge([&](int w, int i) { return part[w * ROWS * P + i]; }, W, e / DH, e % DH, m, l, o);
     if (a.splits == 1) {
       store(e / DH, e % DH, m, l, o);
     } else {
@@ -459,21 +448,54 @@ __global__ void __launch_bounds__(128, DH == 64 ? 2 : 3) cache_attn_rows_kernel(
   if (a.splits > 1) cluster_meet();
 }
 
-template <typename T, int DH, int PARTS, int FORM, int W>
+// Rounds of work on a GPU that holds `cap` workers at a time: they end one by one, so between the quotient and the whole
+// number above it.
+double rounds(double workers, double cap) {
+  return workers <= cap ? 1.0 : 0.5 * (workers / cap + (double)(long)((workers + cap - 1) / cap));
+}
+// Warps of a CTA and CTAs of a unit, the few-row kernel: the least of the times, in us, that a warp's blocks take on the SM with the
+// most warps.  A block takes a warp `alone` + `shared` times the warps of its SM (measured, B200, 4 - 32 warps an SM; CTAs of one
+// warp a fifth more); start and merge of a round 2.5, of clusters 4; these have to fit into a part of the GPU of some
+// 18 SMs, and many are slow to find their places.
+// Small CTAs spread better, larger ones need fewer partial results.  64 contexts x heads of 65536 rows of size 64: 2 CTAs of eight
+// warps 86 us, 8 of two 82; 160 of 8192: 46 and, 4 of two, 33; 384 of 8192 of size 32: 4 of four 43, one of four 41; 240 of 4096 of
+// size 16: 8 of two 16, one of eight 12; 512 contexts x 6 heads of 256 rows of size 32: one of eight 43, one of one 13.
+template <int DH>
+int plan_warps(AttnArgs& a, long blocks) {
+  constexpr double alone = DH == 16 ? 0.2 : DH == 32 ? 0.36 : 0.5, shared = DH == 16 ? 0.047 : DH == 32 ? 0.062 : 0.09;
+  constexpr int kRegisters = 72, kShared = 227 * 1024;
+  double least = 0.0;
+  int best = 0;
+  for (int warps = 1; warps <= 8; warps *= 2) {
+    const int by_shared = kShared / (warps * Ring<DH>::kBytes + 1024), by_registers = 65536 / (32 * kRegisters * warps);
+    const int fit = by_shared < by_registers ? by_shared : by_registers;
+    for (int s = 1; s <= (warps == 1 ? 1 : 8); s *= 2) {
+      const long ctas = a.units * s, per_sm = (ctas + kSms - 1) / kSms, per = (long)warps * s;
+      const double full = s == 1 ? kSms * fit : 8 * (18 * fit / s * s), quotient = (double)ctas / full;
+      const double rounds = ctas <= full ? 1.0 : 0.25 * quotient + 0.75 * (double)(long)(quotient + 0.999);
+      const double block = alone + shared * (warps == 1 ? 1.2 : warps) * (per_sm < fit ? per_sm : fit);
+      const double t = rounds * ((double)((blocks + per - 1) / per) * block + (s > 1 ? 4.0 : 2.5)) + (s > 1 && ctas > 600 ? 0.007 * (ctas - 600) : 0.0);
+      if (!best || t < least) least = t, best = warps, a.splits = s;
+    }
+  }
+  return best;
+}
+
+template <typename T, int DH, int PARTS, bool LIST, int W>
 int launch(const AttnArgs& a, cudaStream_t s) {
   static SmemConfig config;
   const size_t part = (size_t)(W + 1) * partial_floats<DH, PARTS>() * sizeof(float);
   const size_t ring = (size_t)W * Ring<DH>::kBytes;
-  return launch_attn(cache_attn_kernel<T, DH, PARTS, FORM, W>, config, part > ring ? part : ring, W * 32, a, s);
+  return launch_attn(cache_attn_kernel<T, DH, PARTS, LIST, W>, config, part > ring ? part : ring, W * 32, a, s);
 }
-// By plan_warps' choice: eight warps a unit are a CTA (of a cluster); fewer are CTAs of four, which leave sooner: 64 contexts of
-// 2048 rows 15.7 us with eight, 14.0 with four; 800 units of 11 blocks 16.5 and 14.0.
-template <typename T, int DH, int PARTS>
-int launch_few(AttnArgs& a, int warps, cudaStream_t s) {
-  if (warps == kWarps) return a.list ? launch<T, DH, PARTS, 2, kWarps>(a, s) : launch<T, DH, PARTS, 0, kWarps>(a, s);
-  a.per_cta = 4 / warps;
-  if (a.list) return launch<T, DH, PARTS, 2, 4>(a, s);
-  return a.per_cta == 1 ? launch<T, DH, PARTS, 0, 4>(a, s) : launch<T, DH, PARTS, 1, 4>(a, s);
+template <typename T, int DH, int PARTS, bool LIST>
+int launch_few(AttnArgs& a, long blocks, cudaStream_t s) {
+  switch (plan_warps<DH>(a, blocks)) {
+    case 1: return launch<T, DH, PARTS, LIST, 1>(a, s);
+    case 2: return launch<T, DH, PARTS, LIST, 2>(a, s);
+    case 4: return launch<T, DH, PARTS, LIST, 4>(a, s);
+    default: return launch<T, DH, PARTS, LIST, 8>(a, s);
+  }
 }
 template <int DH>
 int launch_rows(const AttnArgs& a, cudaStream_t s) {
@@ -481,30 +503,6 @@ int launch_rows(const AttnArgs& a, cudaStream_t s) {
   return launch_attn(cache_attn_rows_kernel<DH>, config, RowTile<DH>::kSmem, RowTile<DH>::NW * 32, a, s);
 }
 
-// Rounds of work on a GPU that holds `cap` workers at a time: they end one by one, so between the quotient and the whole
-// number above it.
-double rounds(double workers, double cap) {
-  return workers <= cap ? 1.0 : 0.5 * (workers / cap + (double)(long)((workers + cap - 1) / cap));
-}
-// Warps of a unit and CTAs of a unit (a cluster; only whole ones): the least
-// rounds times blocks a warp, start and merge of a round counted as two blocks, each doubling of a cluster as a half, a tenth
-// more where a CTA has several units (head sizes 16 and 32), a twentieth where it has eight warps.
-// 512 contexts x 6 heads of 4 blocks: one warp each 20 us, eight 43; 384 of 32: eight or four 18, one 33; 512 of 32 at head size 64: two 29,
-// eight 38.
-int plan_warps(AttnArgs& a, long blocks, int resident_warps) {
-  const double few = a.c.head_dim == 64 ? 1.0 : 1.1;
-  double least = 0.0;
-  int best = 0;
-  for (int warps = 1; warps <= kWarps; warps *= 2)
-    for (int s = 1, extra = 0; s <= (warps == kWarps ? 8 : 1); s *= 2, ++extra) {
-      const long per = (long)warps * s;
-      if (s > 1 && blocks < 2 * per) break;
-      const double t = rounds((double)a.units * per, (double)kSms * resident_warps) *
-                       ((double)((blocks + per - 1) / per) + 2.0 + 0.5 * extra) * (warps == kWarps ? 1.05 : warps < 4 ? few : 1.0);
-      if (!best || t < least) least = t, best = warps, a.splits = s;
-    }
-  return best;
-}
 // Which kernel, and how many CTAs share a unit's blocks: the least of the times that these figures give, in us.  Measured
 // (B200) over 16 - 4096 rows, 1 - 384 contexts x heads and 500 - 32768 context rows.
 //   few rows: start and merge, and the whole GPU's time for a block against one tile of 8 (bf16) or 4 (fp32) rows;
@@ -549,9 +547,8 @@ double tiles_time(const TileCost& c, const AttnArgs& a, long blocks, int& splits
 template <typename T, int DH>
 int by_form(AttnArgs& a, long blocks, cudaStream_t s) {
   constexpr int kParts = sizeof(T) == 2 ? 1 : 2;
-  constexpr int kResident = DH == 64 ? 8 : 16;     // warps of an SM, by their rings
   const auto tiles = [&a](int rows) { a.tiles = (a.rows + rows - 1) / rows, a.units *= a.tiles; };
-  if (a.list) return launch_few<T, DH, 2>(a, plan_warps(a, blocks, kResident), s);
+  if (a.list) return launch_few<T, DH, 2, true>(a, blocks, s);
   const int form = debug_cache_form();
   if (form >= 2 || (form == 0 && a.rows > 8)) {
     const double few = kFewStart + few_cost<T, DH>() * (double)(a.units * ((a.rows + 8 / kParts - 1) / (8 / kParts))) * (double)blocks;
@@ -576,8 +573,7 @@ int by_form(AttnArgs& a, long blocks, cudaStream_t s) {
   }
   const bool eight = kParts == 1 && a.rows > 4;
   tiles(eight ? 8 : 4);
-  const int warps = plan_warps(a, blocks, kResident);
-  return eight ? launch_few<T, DH, kParts>(a, warps, s) : launch_few<T, DH, 2>(a, warps, s);
+  return eight ? launch_few<T, DH, kParts, false>(a, blocks, s) : launch_few<T, DH, 2, false>(a, blocks, s);
 }
 
 int attention(int dtype, const void* q, const int64_t* strides, int n_streams, int n_q, const artab_cache* c,
@@ -606,7 +602,6 @@ int attention(int dtype, const void* q, const int64_t* strides, int n_streams, i
   if (workspace) return launch_cache_by_block(dtype, a, workspace, s);
   const long blocks = list ? n_list : (max_len + kCacheBlock - 1L) / kCacheBlock;
   a.splits = 1;
-  a.per_cta = 1;
   if (dtype == ARTAB_F32) {
     if (c->head_dim == 16) return by_form<float, 16>(a, blocks, s);
     if (c->head_dim == 32) return by_form<float, 32>(a, blocks, s);

@@ -15,7 +15,6 @@ struct AttnArgs {
   int tiles;              // tiles of a group's rows
   long units;             // (group, head, tile) or (stream, head, query)
   int splits;             // CTAs of a cluster, which share the blocks of a unit
-  int per_cta;            // units of a CTA (lists; else 1)
   const int32_t* list;    // [B][H][Lq][n_list], or null: every block
   int n_list;
   float scale_log2;       // scale * log2 e
@@ -95,12 +94,12 @@ __device__ __forceinline__ void merge_rows(const AttnArgs& a, uint32_t base, int
   }
 }
 
-// One launch: ceil(units / per_cta) clusters of `splits` CTAs.
+// One launch: `units` clusters of `splits` CTAs.
 template <typename K, typename... E>
 int launch_attn(K kernel, SmemConfig& config, size_t smem, int threads, const AttnArgs& a, cudaStream_t s, E... extra) {
   cudaError_t e = config.ensure(kernel, smem, true);
   ARTAB_REQUIRE(e == cudaSuccess, ARTAB_ELAUNCH, "cache_attention: %s", cudaGetErrorString(e));
-  const long ctas = (a.units + a.per_cta - 1) / a.per_cta * a.splits;
+  const long ctas = a.units * a.splits;
   ARTAB_REQUIRE(ctas <= 0x7fffffffL, ARTAB_EINVAL, "cache_attention: too many query rows");
   PlainLaunchScope plain;   // the caller's earlier launches are unknown: see common.cuh
   count_launch();
