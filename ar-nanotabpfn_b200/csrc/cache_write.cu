@@ -23,6 +23,7 @@ struct WriteArgs {
   int n_rows;
   int fresh;               // the whole cache is laid out: every block of it is given scales and bounds
   int set_lens;            // lens[g] = end of the rows written here
+  int by_group;            // a CTA (of cache_append_row_kernel) has all heads of a group: it may move the lens[g] that it reads
   int vec_k, vec_v;
   int per_cta;             // blocks of a CTA
 };
@@ -283,22 +284,25 @@ __global__ void __launch_bounds__(2 * Half<DH>::N, (FRESH ? 1024 : 1280) / (2 * 
 
 // One new row a context: the step of a decode.  A warp does a (group, head): the new row's codes by a lane or two a channel,
 // the bounds from the block's older keys, which 16 bytes a lane hold while they are looked through; older codes are
-// written only where a scale rises.  512 contexts x 6 heads of size 32: 5 us; 15.4 with cache_write_kernel,
-// which goes through whole blocks with a CTA each.
+// written only where a scale rises.  512 contexts x 6 heads of size 32: 15.4 us with cache_write_kernel, which goes through
+// whole blocks with a CTA each, 5 here.  Up to kGroupHeads heads a CTA takes a group, and the length moves in the same launch;
+// beyond, four warps of any groups, and cache_advance_kernel.
+constexpr int kGroupHeads = 16;
 __device__ __forceinline__ int value_place(int row) { return 16 * ((row >> 1) & 3) + 4 * (row >> 4) + 2 * ((row >> 3) & 1) + (row & 1); }
 
 template <typename T, int DH>
-__global__ void __launch_bounds__(128) cache_append_row_kernel(const WriteArgs a) {
+__global__ void __launch_bounds__(32 * kGroupHeads) cache_append_row_kernel(const WriteArgs a) {
   constexpr int NV = DH / 16;          // new numbers of a lane: number v = lane + 32 i is channel v % DH of keys (v < DH) or values
   constexpr int NQ = DH / 8;           // 16-byte pieces of a lane: piece lane + 32 i, 16 channels of a key
   constexpr int PARTS = DH / 16;       // pieces of a row
   const int lane = threadIdx.x & 31, H = a.c.n_heads;
-  const long unit = (long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const long unit = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (unit >= (long)a.c.n_groups * H) return;
   const int g = (int)(unit / H), h = (int)(unit % H);
   int start, end;
   write_range(a, g, start, end);
-  if (a.set_lens && h == 0 && lane == 0) a.c.lens[g] = end;
+  if (a.by_group) __syncthreads();                                 // every warp has read lens
+  if ((a.by_group || a.set_lens) && h == 0 && lane == 0) a.c.lens[g] = end;
   const int blk = start / kCacheBlock, at = start % kCacheBlock;   // `at` rows of the block are kept
   const bool fresh_row = end > start;
   if (blk >= a.c.n_blocks || at + fresh_row == 0) return;
@@ -522,7 +526,7 @@ template <typename T, int DH>
 struct LaunchAppendRow {
   static int go(const WriteArgs& a, dim3 grid, cudaStream_t s) {
     count_launch();
-    cache_append_row_kernel<T, DH><<<grid, 128, 0, s>>>(a);
+    cache_append_row_kernel<T, DH><<<grid, a.by_group ? 32 * a.c.n_heads : 128, 0, s>>>(a);
     return check_launch("cache_append_row");
   }
 };
@@ -588,12 +592,14 @@ int artab_cache_write(int dtype, const void* k, const int64_t* k_strides, const 
   // several blocks a CTA once there are many: the rows of the next are on their way while one is worked on
   const long all = nb * c->n_heads * c->n_groups;
   a.per_cta = !fresh || all / (148L * 16) < 1 ? 1 : all / (148L * 16) > 8 ? 8 : (int)(all / (148L * 16));
+  a.by_group = !fresh && n_rows == 1 && !a.set_lens && c->n_heads <= kGroupHeads;
   if (!fresh && n_rows == 1)
-    rc = by_type_and_size<LaunchAppendRow>(dtype, c->head_dim, a, dim3((unsigned)(((long)c->n_groups * c->n_heads + 3) / 4)), s);
+    rc = by_type_and_size<LaunchAppendRow>(dtype, c->head_dim, a,
+                                           dim3(a.by_group ? c->n_groups : (unsigned)(((long)c->n_groups * c->n_heads + 3) / 4)), s);
   else
     rc = by_type_and_size<LaunchWrite>(dtype, c->head_dim, a,
                                        dim3((unsigned)((nb + a.per_cta - 1) / a.per_cta), c->n_heads, c->n_groups), s);
-  if (rc || a.set_lens) return rc;
+  if (rc || a.set_lens || a.by_group) return rc;
   count_launch();
   cache_advance_kernel<<<(c->n_groups + 255) / 256, 256, 0, s>>>(a);
   return check_launch("cache_advance");

@@ -280,7 +280,7 @@ def test_rows_appended_step_by_step(shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
-@pytest.mark.parametrize("shape", [(1, 1, 16), (7, 3, 32), (5, 2, 64)], ids=str)
+@pytest.mark.parametrize("shape", [(1, 1, 16), (7, 3, 32), (5, 2, 64), (1, 16, 64), (3, 17, 32)], ids=str)
 def test_single_rows_one_after_another(shape, dtype):
     """The step of a decode over more than two blocks: scales that rise and stay, contexts that take no row, rows that
     are taken back, rows of zeros, from strided tensors; the last rows one beyond the capacity."""
