@@ -460,22 +460,25 @@ double rounds(double workers, double cap) {
 // Small CTAs spread better, larger ones need fewer partial results.  64 contexts x heads of 65536 rows of size 64: 2 CTAs of eight
 // warps 86 us, 8 of two 82; 160 of 8192: 46 and, 4 of two, 33; 384 of 8192 of size 32: 4 of four 43, one of four 41; 240 of 4096 of
 // size 16: 8 of two 16, one of eight 12; 512 contexts x 6 heads of 256 rows of size 32: one of eight 43, one of one 13.
+struct FewPlan {
+  double time;
+  int warps, splits;
+};
 template <int DH>
-int plan_warps(AttnArgs& a, long blocks) {
+FewPlan plan_few(long units, long blocks) {
   constexpr double alone = DH == 16 ? 0.2 : DH == 32 ? 0.36 : 0.5, shared = DH == 16 ? 0.047 : DH == 32 ? 0.062 : 0.09;
   constexpr int kRegisters = 72, kShared = 227 * 1024;
-  double least = 0.0;
-  int best = 0;
+  FewPlan best = {0.0, 0, 0};
   for (int warps = 1; warps <= 8; warps *= 2) {
     const int by_shared = kShared / (warps * Ring<DH>::kBytes + 1024), by_registers = 65536 / (32 * kRegisters * warps);
     const int fit = by_shared < by_registers ? by_shared : by_registers;
     for (int s = 1; s <= (warps == 1 ? 1 : 8); s *= 2) {
-      const long ctas = a.units * s, per_sm = (ctas + kSms - 1) / kSms, per = (long)warps * s;
+      const long ctas = units * s, per_sm = (ctas + kSms - 1) / kSms, per = (long)warps * s;
       const double full = s == 1 ? kSms * fit : 8 * (18 * fit / s * s), quotient = (double)ctas / full;
       const double rounds = ctas <= full ? 1.0 : 0.25 * quotient + 0.75 * (double)(long)(quotient + 0.999);
       const double block = alone + shared * (warps == 1 ? 1.2 : warps) * (per_sm < fit ? per_sm : fit);
       const double t = rounds * ((double)((blocks + per - 1) / per) * block + (s > 1 ? 4.0 : 2.5)) + (s > 1 && ctas > 600 ? 0.007 * (ctas - 600) : 0.0);
-      if (!best || t < least) least = t, best = warps, a.splits = s;
+      if (!best.warps || t < best.time) best = {t, warps, s};
     }
   }
   return best;
@@ -489,8 +492,9 @@ int launch(const AttnArgs& a, cudaStream_t s) {
   return launch_attn(cache_attn_kernel<T, DH, PARTS, LIST, W>, config, part > ring ? part : ring, W * 32, a, s);
 }
 template <typename T, int DH, int PARTS, bool LIST>
-int launch_few(AttnArgs& a, long blocks, cudaStream_t s) {
-  switch (plan_warps<DH>(a, blocks)) {
+int launch_few(AttnArgs& a, const FewPlan& plan, cudaStream_t s) {
+  a.splits = plan.splits;
+  switch (plan.warps) {
     case 1: return launch<T, DH, PARTS, LIST, 1>(a, s);
     case 2: return launch<T, DH, PARTS, LIST, 2>(a, s);
     case 4: return launch<T, DH, PARTS, LIST, 4>(a, s);
@@ -504,20 +508,15 @@ int launch_rows(const AttnArgs& a, cudaStream_t s) {
 }
 
 // Which kernel, and how many CTAs share a unit's blocks: the least of the times that these figures give, in us.  Measured
-// (B200) over 16 - 4096 rows, 1 - 384 contexts x heads and 500 - 32768 context rows.
-//   few rows: start and merge, and the whole GPU's time for a block against one tile of 8 (bf16) or 4 (fp32) rows;
+// (B200) over 12 - 4096 rows, 1 - 384 contexts x heads and 500 - 32768 context rows: the pick is 1 - 2 % from the fastest in the
+// mean, up to 20 % where two are close.  Few rows: plan_few, a fifth more for size 32, which full tiles slow down there.
 //   tiles of many rows: one CTA's time for a block when it has an SM to itself and when the SM is full; start and merge of a
 //   wave; CTAs of an SM; rows of a tile.
 struct TileCost {
   double alone, full, start;
   int per_sm, rows;
 };
-constexpr double kFewStart = 4.5, kPerSplit = 0.4;
-template <typename T, int DH>
-constexpr double few_cost() {
-  if (sizeof(T) == 2) return DH == 16 ? 0.5e-3 : DH == 32 ? 0.85e-3 : 1.8e-3;
-  return DH == 16 ? 0.43e-3 : DH == 32 ? 0.77e-3 : 1.65e-3;
-}
+constexpr double kPerSplit = 0.4;
 // cache_attn_tc_kernel
 template <typename T, int DH>
 constexpr TileCost tc_cost() {
@@ -548,10 +547,12 @@ template <typename T, int DH>
 int by_form(AttnArgs& a, long blocks, cudaStream_t s) {
   constexpr int kParts = sizeof(T) == 2 ? 1 : 2;
   const auto tiles = [&a](int rows) { a.tiles = (a.rows + rows - 1) / rows, a.units *= a.tiles; };
-  if (a.list) return launch_few<T, DH, 2, true>(a, blocks, s);
+  if (a.list) return launch_few<T, DH, 2, true>(a, plan_few<DH>(a.units, blocks), s);
   const int form = debug_cache_form();
+  const bool eight = kParts == 1 && a.rows > 4;
+  FewPlan few = plan_few<DH>(a.units * ((a.rows + (eight ? 7 : 3)) / (eight ? 8 : 4)), blocks);
   if (form >= 2 || (form == 0 && a.rows > 8)) {
-    const double few = kFewStart + few_cost<T, DH>() * (double)(a.units * ((a.rows + 8 / kParts - 1) / (8 / kParts))) * (double)blocks;
+    if (DH == 32) few.time *= 1.2;
     constexpr TileCost tc = tc_cost<T, DH>();
     int tc_splits = 1;
     const double tc_time = tiles_time(tc, a, blocks, tc_splits);
@@ -559,21 +560,20 @@ int by_form(AttnArgs& a, long blocks, cudaStream_t s) {
       constexpr TileCost rows = rows_cost<DH>();
       int splits = 1;
       const double time = tiles_time(rows, a, blocks, splits);
-      if (form == 2 || (form == 0 && time < tc_time && time < few)) {
+      if (form == 2 || (form == 0 && time < tc_time && time < few.time)) {
         tiles(rows.rows);
         a.splits = splits;
         return launch_rows<DH>(a, s);
       }
     }
-    if (form >= 2 || tc_time < few) {
+    if (form >= 2 || tc_time < few.time) {
       tiles(tc.rows);
       a.splits = tc_splits;
       return launch_cache_attn_tc<T>(a, s);
     }
   }
-  const bool eight = kParts == 1 && a.rows > 4;
   tiles(eight ? 8 : 4);
-  return eight ? launch_few<T, DH, kParts, false>(a, blocks, s) : launch_few<T, DH, 2, false>(a, blocks, s);
+  return eight ? launch_few<T, DH, kParts, false>(a, few, s) : launch_few<T, DH, 2, false>(a, few, s);
 }
 
 int attention(int dtype, const void* q, const int64_t* strides, int n_streams, int n_q, const artab_cache* c,
