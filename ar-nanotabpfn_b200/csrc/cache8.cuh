@@ -83,6 +83,18 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[4], float scale, f
   }
   return low_bytes(w);
 }
+// Four codes of bf16 numbers x whose largest magnitude gave the step.  x = a 2^i and that magnitude b 2^j have a, b < 256, so
+// 127 x / (b 2^j) is either a tie or more than 2^-16 of itself away from one; the step is off from b 2^j / 127 by at most 2^-24.  A
+// reciprocal that is 2^-19 too small (`over`: step * 127 above the magnitude) or too large decides every tie as the exact
+// quotient by the step does, and nothing else.  `over` 0: ties of the step itself, which this cannot decide.
+constexpr float kTieShift = 1.9073486328125e-6f;
+__device__ __forceinline__ float shifted(float inv, float over) { return inv * (over > 0.0f ? 1.0f - kTieShift : 1.0f + kTieShift); }
+__device__ __forceinline__ uint32_t codes_of_bf16(const float (&x)[4], float inv_shifted) {
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = __float_as_uint(fmaf(x[j], inv_shifted, kRound));
+  return low_bytes(w);
+}
 // Four codes of x * was (whole numbers x at an older step `was`) at a step of `scale`.  The first quotient is off by less
 // than 3e-5: closer than 5e-5 to a tie it is formed again.
 __device__ __forceinline__ uint32_t kept_codes(const float (&x)[4], float was, float scale, float inv) {

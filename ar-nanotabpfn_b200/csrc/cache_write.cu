@@ -195,6 +195,8 @@ __global__ void __launch_bounds__(2 * Half<DH>::N, (FRESH ? 1024 : 1280) / (2 * 
     for (int w = 0; w < F::WARPS; ++w) block_top = max(block_top, s_top[(vals ? F::WARPS : 0) + w]);
     // a step of zero (or NaN) has zero codes
     const float step = larger_step(was, step_of(block_top)), inv = 1.0f / step;
+    const float over = fmaf(step, 127.0f, -__uint_as_float(block_top)), inv_shifted = shifted(inv, over);
+    const bool shift = FRESH && sizeof(T) == 2 && step > 2e-38f && over != 0.0f;
     // rows that stay, at a scale that stays, are not written again
     const bool stays = !FRESH && n_old > 0 && !(step > was);
     if (n_old && vals && !mine && !stays) load_old();
@@ -206,7 +208,10 @@ __global__ void __launch_bounds__(2 * Half<DH>::N, (FRESH ? 1024 : 1280) / (2 * 
       if (FRESH || (row >= n_old && row < n_live)) {   // of a whole cache, rows that are not in use are zeros
         float x[4];
         Four<T>::values(raw[i], x);
-        if (step > 0.0f) w[i] = codes_of(x, step, inv);
+        if (shift)
+          w[i] = codes_of_bf16(x, inv_shifted);
+        else if (step > 0.0f)
+          w[i] = codes_of(x, step, inv);
       } else if (row < n_old) {
         w[i] = old[i];
         if (step > was) {
