@@ -50,7 +50,17 @@ __device__ __forceinline__ void turn(uint32_t (&w)[4]) {
 __device__ __forceinline__ int first_row(int word) { return 16 * (word & 3) + 2 * (word >> 2); }
 
 __device__ __forceinline__ float step_of(uint32_t top_bits) {
-  return top_bits >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : __fdiv_rn(__uint_as_float(top_bits), 127.0f);
+  const float x = __uint_as_float(top_bits);
+  if (x < 1e-30f) return __fdiv_rn(x, 127.0f);
+  // the quotient by 127, correctly rounded: a first value, its exact rest, one correction
+  const float c = 1.0f / 127.0f, q = x * c;
+  return top_bits >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : fmaf(fmaf(-127.0f, q, x), c, q);
+}
+// 1 / x to one step in the last place, for what is checked or moved by more than that afterwards
+__device__ __forceinline__ float reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 // a block with a value that is not finite has NaN for its scale, for good
 __device__ __forceinline__ float larger_step(float a, float b) { return a != a ? a : b != b ? b : fmaxf(a, b); }
@@ -97,13 +107,13 @@ struct Four<__nv_bfloat16> {
   }
   __device__ static __forceinline__ Raw zero() { return make_uint2(0u, 0u); }
   __device__ static __forceinline__ float largest(const Raw (&r)[4]) {
-    __nv_bfloat162 top = __floats2bfloat162_rn(0.0f, 0.0f);
+    uint32_t top = 0u;                               // magnitudes; the signs are of no use
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&r[i].x)));
-      top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&r[i].y)));
+      asm("max.NaN.xorsign.abs.bf16x2 %0, %0, %1;" : "+r"(top) : "r"(r[i].x));
+      asm("max.NaN.xorsign.abs.bf16x2 %0, %0, %1;" : "+r"(top) : "r"(r[i].y));
     }
-    return larger_or_nan(__low2float(top), __high2float(top));
+    return larger_or_nan(__uint_as_float(top << 16 & 0x7fffffffu), __uint_as_float(top & 0x7fff0000u));
   }
 };
 template <typename T>
@@ -194,7 +204,7 @@ __global__ void __launch_bounds__(2 * Half<DH>::N, (FRESH ? 1024 : 1280) / (2 * 
 #pragma unroll
     for (int w = 0; w < F::WARPS; ++w) block_top = max(block_top, s_top[(vals ? F::WARPS : 0) + w]);
     // a step of zero (or NaN) has zero codes
-    const float step = larger_step(was, step_of(block_top)), inv = 1.0f / step;
+    const float step = larger_step(was, step_of(block_top)), inv = reciprocal(step);
     const float over = fmaf(step, 127.0f, -__uint_as_float(block_top)), inv_shifted = shifted(inv, over);
     const bool shift = FRESH && sizeof(T) == 2 && step > 2e-38f && over != 0.0f;
     // rows that stay, at a scale that stays, are not written again
