@@ -73,12 +73,18 @@ class ContextCache:
             raise ValueError("ContextCache: tensors must be contiguous")
         if not scales.get_device() == bounds.get_device() == lens.get_device() == codes.get_device():
             raise ValueError("ContextCache: all tensors must live on one device")
+        self._set(codes, scales, bounds, lens, blocks * CONTEXT_BLOCK if length is None else length)
+
+    def _set(self, codes: Tensor, scales: Tensor, bounds: Tensor, lens: Tensor, length: int) -> "ContextCache":
+        G, H, blocks, _, size = codes.shape
+        Dh = size // CONTEXT_BLOCK
         self.codes, self.scales, self.bounds, self.lens = codes, scales, bounds, lens
         self.n_groups, self.n_heads, self.head_dim, self.capacity = G, H, Dh, blocks * CONTEXT_BLOCK
-        self.length = self.capacity if length is None else min(int(length), self.capacity)
+        self.length = min(int(length), self.capacity)
         self.captured = False      # a graph may have moved lens since `length` was set
         self._c = _lib.Cache(G, H, Dh, blocks, codes.data_ptr(), scales.data_ptr(), bounds.data_ptr(), lens.data_ptr())
         self._ref = C.byref(self._c)
+        return self
 
     @property
     def device(self) -> torch.device:
@@ -193,9 +199,9 @@ def quantize_context(k_ctx: Tensor, v_ctx: Tensor, lens: Optional[Lengths] = Non
     blocks = (capacity + CONTEXT_BLOCK - 1) // CONTEXT_BLOCK
     with _Launch(k.get_device()) as (lib, stream):
         new = k.new_zeros if N == 0 else k.new_empty      # without rows nothing is launched
-        cache = ContextCache(k.new_empty((G, H, blocks, 2, CONTEXT_BLOCK * Dh), dtype=torch.uint8),
-                             new((G, H, blocks, 2), dtype=torch.float32), new((G, H, blocks, 2, Dh), dtype=torch.float16),
-                             new((G,), dtype=torch.int32), N)
+        cache = ContextCache.__new__(ContextCache)._set(
+            k.new_empty((G, H, blocks, 2, CONTEXT_BLOCK * Dh), dtype=torch.uint8), new((G, H, blocks, 2), dtype=torch.float32),
+            new((G, H, blocks, 2, Dh), dtype=torch.float16), new((G,), dtype=torch.int32), N)
         if N:
             _write(lib, stream, cache, code, k, v, None, counts, 1)
     return cache
@@ -286,7 +292,7 @@ def context_cache_attention(q: Tensor, cache: ContextCache, scale: Optional[floa
     """Attention of q [B,H,Lq,Dh] over every row in use of its context: out [B,H,Lq,Dh] (q dtype), lse [B,H,Lq] fp32
     (natural log), as ``triton_context_attention``.  A context without rows gives 0 and -inf."""
     (B, H, Lq, Dh), code, device = _queries(q, cache, "context_cache_attention")
-    out, lse = q.new_empty((B, H, Lq, Dh)), q.new_empty((B, H, Lq), dtype=torch.float32)
+    out, lse = torch.empty_like(q, memory_format=torch.contiguous_format), q.new_empty((B, H, Lq), dtype=torch.float32)
     if B and Lq:
         q, at, strides = _strided(q)
         with _Launch(device) as (lib, stream):
@@ -329,7 +335,7 @@ def block_context_attention(q: Tensor, cache: ContextCache, blocks: Tensor,
         raise ValueError(f"block_context_attention: {shape[3]} blocks a query")
     if blocks.get_device() != device:
         raise ValueError("block_context_attention: blocks must live on the device of the queries")
-    out, lse = q.new_empty((B, H, Lq, Dh)), q.new_empty((B, H, Lq), dtype=torch.float32)
+    out, lse = torch.empty_like(q, memory_format=torch.contiguous_format), q.new_empty((B, H, Lq), dtype=torch.float32)
     if shape[3] == 0:
         return out.zero_(), lse.fill_(float("-inf"))
     if B and Lq:
