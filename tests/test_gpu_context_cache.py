@@ -737,3 +737,34 @@ def test_many_rows_again_and_on_another_stream(form):
         torch.cuda.synchronize()
         for a, b in got:
             assert all(torch.equal(x, y) for x, y in zip(a, want)) and all(torch.equal(x, y) for x, y in zip(b, listed))
+
+
+# contexts x heads x rows for which few queries are spread in different ways: one warp a unit up to clusters of eight CTAs
+SPREADS = [(512, 6, 200), (300, 8, 700), (64, 6, 700), (96, 4, 2000), (20, 8, 8000), (8, 8, 9000), (8, 6, 8192), (1, 6, 8192),
+           (3, 2, 300), (12, 8, 4096), (16, 8, 9000), (64, 6, 8192)]
+
+
+@pytest.mark.parametrize("D", [16, 32, 64])
+@pytest.mark.parametrize("case", SPREADS, ids=str)
+def test_few_queries_however_the_rows_are_spread(case, D):
+    G, H, N = case
+    c = cc()
+    k, v = rows(110, G, H, N, D, torch.bfloat16)
+    cache = c.quantize_context(k, v, lens=lens_of("ragged" if G > 1 else "full", G, N))
+    del k, v
+    for dtype, L in ((torch.float32, 1), (torch.bfloat16, 1), (torch.bfloat16, 5)):
+        q = torch.randn(G, H, L, D, device="cuda", generator=gen(111)).to(dtype)
+        check_attention(c.context_cache_attention(q, cache), attention(q, cache, D ** -0.5), dtype, D)
+
+
+@pytest.mark.parametrize("D", [16, 32, 64])
+@pytest.mark.parametrize("case", [(64, 6, 2000, 4, 8), (200, 8, 900, 1, 4), (8, 6, 8192, 1, 32), (1, 6, 16384, 1, 64), (1, 6, 5000, 1, 9)], ids=str)
+def test_listed_blocks_however_they_are_spread(case, D):
+    G, H, N, L, S = case
+    c = cc()
+    k, v = rows(112, G, H, N, D, torch.bfloat16)
+    cache = c.quantize_context(k, v, lens=lens_of("ragged" if G > 1 else "full", G, N))
+    for dtype in (torch.float32, torch.bfloat16):
+        q = torch.randn(G, H, L, D, device="cuda", generator=gen(113)).to(dtype)
+        blocks = c.select_context_blocks(q, cache, S)
+        check_attention(c.block_context_attention(q, cache, blocks), attention(q, cache, D ** -0.5, times_of(blocks, cache.capacity // BLOCK)), dtype, D)
