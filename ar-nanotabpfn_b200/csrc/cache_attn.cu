@@ -13,8 +13,8 @@
 // walks blocks of its own with a running maximum; its ring of records is filled by 16-byte asynchronous copies
 // and no warp waits for another until the end, where the warps of a unit and the CTAs of a cluster (up to eight
 // share the rows of a context) merge maximum, sum and output through shared memory.
-// Measured (B200), queries of one row each: 8 contexts x 65536 rows x 8 heads of size 64, 82.5 us for 537 MB (6.5 TB/s, 0.99
-// of a copy's rate; half of the issue slots busy), size 32 51 us (5.3 TB/s), size 16 36 us (3.8 TB/s: 16 codes a lane between two
+// Measured (B200), queries of one row each: 8 contexts x 65536 rows x 8 heads of size 64, 82.5 us for 537 MB, called again and again
+// (6.5 TB/s, a copy's rate; half of the issue slots busy), 90 - 96 with the launch and other data in between; size 32 51 us (5.3 TB/s), size 16 36 us (3.8 TB/s: 16 codes a lane between two
 // shuffles); 64 x 2048 x 6 of size 32 14 us and one context of 8192 rows 7 us: a chain of loads, products and merges.
 #include "cache_tile.cuh"
 

@@ -5,8 +5,8 @@
 // it, and the older rows are then rounded again to the new step.
 // Keys go out as they came in; of the values a thread holds the four rows that are neighbours in a channel's order, so
 // that it turns 4 x 4 bytes with permutes, and shared memory brings the words into the order of the record.
-// 64 contexts x 2048 rows x 6 heads of size 32 (B200): fp32 49 us for 251 MB (5.1 TB/s, HBM), bf16 46 us for 151 MB: some 400
-// instructions a warp and block (81 % of issue slots), a quarter of them for quotients next to ties.  Reading the same back
+// 64 contexts x 2048 rows x 6 heads of size 32 (B200): fp32 48 us for 251 MB (5.2 TB/s, HBM), bf16 38 us for 151 MB: some 310
+// instructions a warp and block (80 % of issue slots).  Reading the same back
 // as fp32: 40 us for 252 MB (6.3 TB/s).
 #include "cache8.cuh"
 
