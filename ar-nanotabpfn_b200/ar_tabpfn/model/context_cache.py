@@ -49,7 +49,8 @@ class ContextCache:
 
     They are worked on in place, where they are now: another tensor put in a field's place is not seen.
     ``length``: a bound of ``lens`` known to the host (default: the capacity).  A captured ``append_context`` counts once
-    in it, however often it is replayed; appending and reading outside a capture then look ``lens`` up."""
+    in it, however often it is replayed; appending and reading outside a capture then look ``lens`` up.  Attention picks its
+    kernel and how it splits the rows by ``length``: the same rows with another ``length`` may differ in the last bits."""
 
     __slots__ = ("codes", "scales", "bounds", "lens", "length", "n_groups", "n_heads", "head_dim", "capacity", "captured", "_c", "_ref")
 

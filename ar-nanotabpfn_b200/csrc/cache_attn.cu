@@ -448,15 +448,15 @@ __global__ void __launch_bounds__(128, DH == 64 ? 2 : 3) cache_attn_rows_kernel(
   if (a.splits > 1) cluster_meet();
 }
 
-// Rounds of work on a GPU that holds `cap` workers at a time: they end one by one, so between the quotient and the whole
-// number above it.
-double rounds(double workers, double cap) {
-  return workers <= cap ? 1.0 : 0.5 * (workers / cap + (double)(long)((workers + cap - 1) / cap));
+// CTAs that the GPU holds, `per_sm` an SM: a cluster of more than two has to fit into a part of the GPU of some 18 SMs, one
+// of which is smaller
+double held_ctas(int per_sm, int splits) {
+  return splits <= 2 ? kSms * per_sm : (8 * (18 * per_sm / splits) - 1) * splits;
 }
 // Warps of a CTA and CTAs of a unit, the few-row kernel: the least of the times, in us, that a warp's blocks take on the SM with the
 // most warps.  A block takes a warp `alone` + `shared` times the warps of its SM (measured, B200, 4 - 32 warps an SM; CTAs of one
-// warp a fifth more); start and merge of a round 2.5, of clusters 4; these have to fit into a part of the GPU of some
-// 18 SMs, and many are slow to find their places.
+// warp a fifth more); start and merge of a round 2.5, of clusters 4, and many of these are slow to find their
+// places.
 // Small CTAs spread better, larger ones need fewer partial results.  64 contexts x heads of 65536 rows of size 64: 2 CTAs of eight
 // warps 86 us, 8 of two 82; 160 of 8192: 46 and, 4 of two, 33; 384 of 8192 of size 32: 4 of four 43, one of four 41; 240 of 4096 of
 // size 16: 8 of two 16, one of eight 12; 512 contexts x 6 heads of 256 rows of size 32: one of eight 43, one of one 13.
@@ -474,7 +474,7 @@ FewPlan plan_few(long units, long blocks) {
     const int fit = by_shared < by_registers ? by_shared : by_registers;
     for (int s = 1; s <= (warps == 1 ? 1 : 8); s *= 2) {
       const long ctas = units * s, per_sm = (ctas + kSms - 1) / kSms, per = (long)warps * s;
-      const double full = s == 1 ? kSms * fit : 8 * (18 * fit / s * s), quotient = (double)ctas / full;
+      const double full = held_ctas(fit, s), quotient = (double)ctas / full;
       const double rounds = ctas <= full ? 1.0 : 0.25 * quotient + 0.75 * (double)(long)(quotient + 0.999);
       const double block = alone + shared * (warps == 1 ? 1.2 : warps) * (per_sm < fit ? per_sm : fit);
       const double t = rounds * ((double)((blocks + per - 1) / per) * block + (s > 1 ? 4.0 : 2.5)) + (s > 1 && ctas > 600 ? 0.007 * (ctas - 600) : 0.0);
@@ -510,35 +510,44 @@ int launch_rows(const AttnArgs& a, cudaStream_t s) {
 // Which kernel, and how many CTAs share a unit's blocks: the least of the times that these figures give, in us.  Measured
 // (B200) over 12 - 4096 rows, 1 - 384 contexts x heads and 500 - 32768 context rows: the pick is 1 - 2 % from the fastest in the
 // mean, up to 20 % where two are close.  Few rows: plan_few, a fifth more for size 32, which full tiles slow down there.
-//   tiles of many rows: one CTA's time for a block when it has an SM to itself and when the SM is full; start and merge of a
-//   wave; CTAs of an SM; rows of a tile.
+//   tiles of many rows: a CTA's time for a block when it has an SM to itself and when the SM is full; start and merge in either
+//   case; CTAs of an SM; rows of a tile.  Splits that fill the last round matter: 4096 bf16 queries x 8192 rows x 6 heads of
+//   size 32, 192 tiles, 120 us in one piece and 98 in two; 2048 x 32768, 96 tiles, 231 in two and 180 in four.
 struct TileCost {
-  double alone, full, start;
+  double alone, full, start, start_full;
   int per_sm, rows;
 };
-constexpr double kPerSplit = 0.4;
 // cache_attn_tc_kernel
 template <typename T, int DH>
 constexpr TileCost tc_cost() {
-  if (sizeof(T) == 2) return DH == 16 ? TileCost{0.56, 0.75, 8.0, 2, 128} : DH == 32 ? TileCost{0.62, 0.87, 9.0, 2, 128} : TileCost{0.73, 1.0, 10.0, 2, 128};
-  return DH == 16 ? TileCost{0.75, 1.3, 9.0, 2, 128} : DH == 32 ? TileCost{0.75, 1.3, 9.5, 2, 128} : TileCost{0.82, 1.75, 11.5, 2, 128};
+  if (sizeof(T) == 2) return DH == 16 ? TileCost{0.53, 0.8, 6.0, 9.0, 2, 128} : DH == 32 ? TileCost{0.56, 0.87, 6.0, 9.0, 2, 128} : TileCost{0.7, 1.0, 10.5, 13.5, 2, 128};
+  return DH == 16 ? TileCost{0.77, 1.03, 8.0, 13.0, 2, 128} : DH == 32 ? TileCost{0.74, 1.06, 9.6, 15.0, 2, 128} : TileCost{0.78, 1.2, 13.8, 16.0, 2, 128};
 }
 // cache_attn_rows_kernel.  It starts sooner and has half the rows a tile, tcgen05 is faster once it runs (6 heads x 2000 rows of size
-// 32: 512 queries 14.5 and 22.4 us; 8192 rows: 1024 queries 64 and 49, 4096 queries 227 and 149).
+// 32: 512 queries 14.5 and 22.4 us; 8192 rows: 1024 queries 64 and 46, 4096 queries 227 and 133).
 template <int DH>
 constexpr TileCost rows_cost() {
   constexpr int rows = RowTile<DH>::ROWS;
-  return DH == 16 ? TileCost{0.83, 1.7, 4.0, 3, rows} : DH == 32 ? TileCost{0.96, 2.0, 4.0, 3, rows} : TileCost{1.3, 2.3, 5.0, 2, rows};
+  return DH == 16 ? TileCost{0.83, 1.7, 4.0, 4.0, 3, rows} : DH == 32 ? TileCost{0.96, 2.0, 4.0, 4.0, 3, rows} : TileCost{1.3, 2.3, 5.0, 5.0, 2, rows};
 }
-// least time over the splits of a unit, and those splits
+// least time over the splits of a unit, and those splits.  Of several rounds, the last one starts before the one before it has
+// ended: between the sum of the rounds and what the work alone would take, the nearer to the sum the larger the clusters.
 double tiles_time(const TileCost& c, const AttnArgs& a, long blocks, int& splits) {
-  const double units = (double)a.units * (double)((a.rows + c.rows - 1) / c.rows), cap = (double)kSms * c.per_sm;
+  const double units = (double)a.units * (double)((a.rows + c.rows - 1) / c.rows);
   double least = 0.0;
-  for (int s = 1; s <= 8; s *= 2) {
-    const double ctas = units * s;
-    const double crowd = ctas <= kSms ? 0.0 : ctas >= cap ? 1.0 : (ctas / kSms - 1.0) / (c.per_sm - 1);
-    const double t = rounds(ctas, cap) * ((c.alone + (c.full - c.alone) * crowd) * (double)((blocks + s - 1) / s) + c.start + kPerSplit * s);
-    if (s == 1 || t < least) least = t, splits = s;
+  for (const int s : {1, 2, 4, 5, 8}) {
+    const double ctas = units * s, cap = held_ctas(c.per_sm, s), each = (double)((blocks + s - 1) / s), merge = 0.9 * s;
+    const auto round = [&](double n) {               // n CTAs at a time
+      const double crowd = n <= 0.0 ? 0.0 : (double)(long)((n + kSms - 1) / kSms - 1.0) / (c.per_sm - 1), x = crowd < 1.0 ? crowd : 1.0;
+      return n <= 0.0 ? 0.0 : (c.alone + (c.full - c.alone) * x) * each + c.start + (c.start_full - c.start) * x + merge;
+    };
+    double t = round(ctas);
+    if (ctas > cap) {
+      const double whole = (double)(long)(ctas / cap), rounds = whole * round(cap) + round(ctas - whole * cap);
+      const double work = ctas / cap * c.full * each + c.start_full + merge, share = s <= 2 ? 0.5 : s == 4 ? 0.7 : 0.86;
+      t = share * rounds + (1.0 - share) * work;
+    }
+    if (s == 1 || t < 0.96 * least) least = t, splits = s;   // more partial results have to be worth it
   }
   return least;
 }

@@ -23,7 +23,7 @@
 // both halves of a block unrolled, the next scores as soon as these are read 208 -> 176.  A share of the exponentials on the FMA
 // pipe (degree four, packed pairs) cost more issue slots than it freed at every share: 242 us with none, 246 with an eighth,
 // 255 with a quarter of them.
-// fp32, 4096 queries x 8192 rows x 6 heads: size 32 149 us (register tiles of cache_attn.cu 227), 16 144 (164), 64 162 (380).
+// fp32, 4096 queries x 8192 rows x 6 heads: size 32 133 us (register tiles of cache_attn.cu 227), 16 127 (164), 64 150 (380).
 // Every wait is bounded; a CTA that gives up lets its MMAs end, frees its tensor memory and writes NaN for its rows.
 #include "cache_attn.cuh"
 
