@@ -768,3 +768,17 @@ def test_listed_blocks_however_they_are_spread(case, D):
         q = torch.randn(G, H, L, D, device="cuda", generator=gen(113)).to(dtype)
         blocks = c.select_context_blocks(q, cache, S)
         check_attention(c.block_context_attention(q, cache, blocks), attention(q, cache, D ** -0.5, times_of(blocks, cache.capacity // BLOCK)), dtype, D)
+
+
+@pytest.mark.parametrize("D", [16, 32, 64])
+@pytest.mark.parametrize("case", [(1, 100, 300), (1, 100, 640), (1, 100, 1280), (1, 100, 2500), (1, 100, 5100), (1, 100, 8000), (2, 700, 2560),
+                                  (3, 1000, 5100), (6, 1000, 300)], ids=str)
+def test_many_rows_however_the_context_is_split(case, D, form):
+    """Clusters of one, two, four, five and eight CTAs, with shares of blocks that are not equal."""
+    H, L, N = case
+    c = cc()
+    k, v = rows(114, 1, H, N, D, torch.bfloat16)
+    cache = c.quantize_context(k, v)
+    for dtype in (torch.float32, torch.bfloat16):
+        q = torch.randn(1, H, L, D, device="cuda", generator=gen(115)).to(dtype)
+        check_attention(c.context_cache_attention(q, cache), attention(q, cache, D ** -0.5), dtype, D)
