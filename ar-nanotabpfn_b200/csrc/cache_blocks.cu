@@ -6,8 +6,9 @@
 // that hold it, eight (bf16) or four (fp32) a warp, and writes for each entry the partial result of its block: output not
 // yet divided, maximum, sum.  cache_join_kernel merges the entries of a query in the order of its list.  The
 // order in which a CTA finds entries varies, what it computes for an entry does not.
-// 1024 queries x 6 heads x 16 of 256 blocks of size 32 (B200): 40 us, 32 + 7 (75 us one by one, 402 MB out of L2); half of
-// the issue slots busy, of some 1700 instructions a warp two fifths are the products and a fifth the look-up.
+// 1024 queries x 6 heads x 16 of 256 blocks of size 32 (B200): 34.5 us, 27 + 7 (64 us one by one, 402 MB out of L2); with 5 CTAs
+// an SM that look at 4096 entries at a time 40 us, with 6 and 8192 34.5.  Of some 1700 instructions a warp two fifths are the products
+// and a fifth the look-up.
 #include <type_traits>
 
 #include "cache_tile.cuh"
@@ -15,7 +16,7 @@
 namespace artab {
 namespace {
 
-constexpr int kWarps = 8, kThreads = 32 * kWarps, kChunk = 16 * kThreads;   // entries looked at between two rounds of work
+constexpr int kWarps = 8, kThreads = 32 * kWarps, kChunk = 32 * kThreads;   // entries looked at between two rounds of work
 
 struct JoinArgs {
   AttnArgs a;
@@ -24,7 +25,7 @@ struct JoinArgs {
 };
 
 template <typename T, int DH, int PARTS>
-__global__ void __launch_bounds__(kThreads) cache_by_block_kernel(const JoinArgs j) {
+__global__ void __launch_bounds__(kThreads, 6) cache_by_block_kernel(const JoinArgs j) {
   using Tl = Tile<DH, PARTS>;
   const AttnArgs& a = j.a;
   constexpr int kRecord = 2 * kCacheBlock * DH;
@@ -160,8 +161,9 @@ int launch_by_block(const JoinArgs& j, cudaStream_t s) {
 }  // namespace
 
 // Going through the blocks pays from so many entries a block on (in the mean), as long as looking an entry up in every
-// block does not cost more than the records that are read once less, and the partial results stay below a gigabyte.
-constexpr int kLeastShared = 8;
+// block does not cost more than the records that are read once less, and the partial results stay below a gigabyte.  6 heads
+// of size 32, 16 of 256 blocks: 128 queries (8 entries a block) 15.1 us by block, 13.7 one by one; 256 17.6 and 21.1; 512 22 and 36.
+constexpr int kLeastShared = 12;
 constexpr int64_t kMostWorkspace = 1LL << 30;
 int64_t by_block_workspace(const artab_cache* c, int n_streams, int n_q, int n_list) {
   const int64_t rows = c->n_groups == 1 ? (int64_t)n_streams * n_q : n_q;
