@@ -782,3 +782,21 @@ def test_many_rows_however_the_context_is_split(case, D, form):
     for dtype in (torch.float32, torch.bfloat16):
         q = torch.randn(1, H, L, D, device="cuda", generator=gen(115)).to(dtype)
         check_attention(c.context_cache_attention(q, cache), attention(q, cache, D ** -0.5), dtype, D)
+
+
+@pytest.mark.parametrize("p", [-118, -60, 0, 90])
+def test_every_quotient_of_bf16_magnitudes(p):
+    """Blocks whose largest magnitude is b 2^p, b = 128 .. 255, with every a 2^(p - i) up to it: among the quotients are all the
+    ties and near ties that bf16 rows can have."""
+    c = cc()
+    a = torch.arange(1, 256, device="cuda", dtype=torch.float64)
+    x = (a[None] * 2.0 ** -torch.arange(16, device="cuda", dtype=torch.float64)[:, None]).flatten()        # 4080 numbers
+    x = torch.cat([x, torch.zeros(16, device="cuda", dtype=torch.float64)])
+    b = torch.arange(128, 256, device="cuda", dtype=torch.float64)
+    k = torch.where(x[None] <= b[:, None], x[None], x[None] / 2) * torch.where(torch.arange(4096, device="cuda") % 2 == 0, 1.0, -1.0)
+    k[:, -1] = b
+    k = (k * 2.0 ** p).view(128, 1, 64, 64).bfloat16()
+    v = (k.float() * 0.5).bfloat16().flip(0)
+    lens = torch.full((128,), 64, dtype=torch.int32, device="cuda")
+    ck, cv, scales, _ = quantized(k, v, lens, 1)
+    check_fields(c.quantize_context(k, v), ck, cv, scales, lens)
