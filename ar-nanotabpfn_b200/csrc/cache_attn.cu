@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnArgs a) {
 // warps owns 64 queries and walks the blocks of its share together: each warp turns a quarter of a block's codes into
 // half-precision fragments in shared memory, in the order in which a lane reads them with 16-byte loads, while the
 // block before is worked on; the numerators go from the accumulators of one product straight into the operand
-// registers of the next.  The value scale of a block is folded into the exponent, relative to the largest of the
+// registers of the next.  The value scale of a block is folded into the exponent and the maximum, relative to the largest of the
 // context, so that one accumulator serves all blocks.  (bf16 queries and larger jobs: cache_attn_tc.cu.)
 // B200, 6 heads of size 32: 512 queries x 2000 rows 14.3 us, 512 x 8192 34 us.  Two CTAs (size 64) or three of 168 registers an
 // SM; with 1024 queries x 8192 rows (64 us) the tensor pipe is 40 % busy, issue slots 40 %: latency of a block's chain (scores,
@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(128, DH == 64 ? 2 : 3) cache_attn_rows_kernel(
     float ratio = vmax > 0.0f ? sc.y / vmax : 0.0f;
     if (ratio != ratio) poison = sc.y, ratio = 1.0f;   // a block with values that are not finite: the weights are sound
     ratio = fmaxf(ratio, kLeastRatio);
-    const float lift = kLift + __log2f(ratio), unlift = 1.0f / ratio;
+    const float part_of = __log2f(ratio), lift = kLift + part_of, unlift = 1.0f / ratio;
     float c[MT][8][4];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(128, DH == 64 ? 2 : 3) cache_attn_rows_kernel(
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       const float x = f[mt] * sc.x, slope = !(x <= 1e-37f) ? x : 1e-37f;      // never 0 (a masked score stays -inf), NaN as it is
-      mx = fmaxf(m[mt], mx * slope);
+      mx = fmaxf(m[mt], fmaf(mx, slope, part_of));
       const float base = mx == -CUDART_INF_F ? 0.0f : mx, alpha = ex2(m[mt] - base), add = lift - base;
       m[mt] = mx;
       if (__any_sync(0xffffffffu, alpha != 1.0f)) {

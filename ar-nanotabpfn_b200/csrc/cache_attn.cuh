@@ -24,9 +24,11 @@ struct AttnArgs {
 };
 
 constexpr int kSms = 148;
-// Smallest value scale, relative to the largest of the context, that is told apart where value scales are factors of the
-// numerators: below it codes count as much as they would at it, an error of 2^-20 of the largest value.
-constexpr float kLeastRatio = 9.5367431640625e-7f;
+// Where value scales are factors of the numerators (the kernels of many rows), they are so relative to the largest of the context, and
+// a row's maximum is that of score + log2(ratio): a numerator is as large as what its row adds to the output, so a block of small
+// values keeps all its bits wherever the output is made of it.  Ratios below 2^-80, blocks of zeros among them, count as 2^-80
+// (sums of numerators over their ratios stay within fp32: 2^41 numerators, times 2^80).
+constexpr float kLeastRatio = 8.271806125530277e-25f;
 
 template <typename T>
 int launch_cache_attn_tc(const AttnArgs& a, cudaStream_t s);

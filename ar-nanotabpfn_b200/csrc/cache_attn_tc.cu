@@ -9,8 +9,8 @@
 //   warps 10, 11     issue the MMAs of one warpgroup each, by an elected lane of a warp that walks and waits as a whole
 // S = Q . codes^T is M 128, N 64; O += P . codes is M 128, N = Dh with P from tensor memory.  All operands are halves:
 // queries of bf16 are exact in them (scaled by a power of two per row), codes are whole numbers, numerators keep
-// 11 bits.  fp32: queries and numerators in two parts of 11 bits, each product once per part into the same accumulator.  Scales of keys go into the exponent's factor, scales of values into its offset (relative to the largest of the
-// context, taken out of the row sum again), so O accumulates over all blocks.
+// 11 bits.  fp32: queries and numerators in two parts of 11 bits, each product once per part into the same accumulator.  Scales of keys go into the exponent's factor, scales of values into its offset and the reference (relative to the
+// largest of the context, taken out of the row sum again), so O accumulates over all blocks.
 // Two CTAs share an SM (256 TMEM columns each), so four warpgroups are in different phases of their blocks.  Head size 64
 // and two parts have no room for P beside S: it overwrites the scores it came from, and the next scores wait for P . V.
 // Measured (B200), bf16, 8192 queries x 8192 rows x 6 heads: head size 32 176 us (292 TFLOP/s, 2.28e12 exponentials a second),
@@ -253,7 +253,8 @@ __device__ __forceinline__ float largest(const uint32_t (&r)[32], int live) {
 // time, the upper ones first (where numerators overwrite scores, they overwrite those).  MASKED: the block's last rows
 // are not in use.  False when a wait gave up.
 //
-// The scores are read once: the reference m is a score of the row's first block, and stays until the sum of 32
+// The scores are read once: the reference m is a score of the row's first block (plus log2 of its value scale, `lift` - kLiftTc),
+// and stays until the sum of 32
 // numerators shows that one may have passed the range of halves (2^10 above m).  Then, rarely on ordinary
 // scores, m rises by a whole number k and all that was taken against it shrinks by 2^-k, exactly: sums, the numerators
 // that are in tensor memory, the output.  The result does not depend on m.
@@ -277,8 +278,8 @@ __device__ __forceinline__ bool softmax_block(TcSmem<T, DH>* sm, uint32_t t_row,
       fence_before();
       mbar_arrive(&sm->s_free[wg]);
     }
-    if (i == 0 && c == 1) m = MASKED && lv <= 0 ? m : largest<MASKED>(r, lv) * slope;   // no row of these in use: not yet
-    if (MASKED && i == 0 && c == 0 && live <= 32) m = largest<MASKED>(r, lv) * slope;
+    if (i == 0 && c == 1) m = MASKED && lv <= 0 ? m : fmaf(largest<MASKED>(r, lv), slope, lift - kLiftTc);   // no row of these in use: not yet
+    if (MASKED && i == 0 && c == 0 && live <= 32) m = fmaf(largest<MASKED>(r, lv), slope, lift - kLiftTc);
     float part = numerators<MASKED, Pl::kParts>(r, pk, slope, lift - m, lv);
     if (c == 1 && i > 0) {                        // the P . V before this one has read P and written O
       if (!kAlias) ok = __all_sync(0xffffffffu, mbar_wait(&sm->o_full[wg], (i - 1) & 1, ctl));
@@ -290,7 +291,7 @@ __device__ __forceinline__ bool softmax_block(TcSmem<T, DH>* sm, uint32_t t_row,
         tmem_ld32(t_row + 32 * c, r);
         wait_ld();
       }
-      if (!(part < kMostSum)) k = fmaxf(ceilf(largest<MASKED>(r, lv) * slope - m), 0.0f);
+      if (!(part < kMostSum)) k = fmaxf(ceilf(fmaf(largest<MASKED>(r, lv), slope, lift - kLiftTc) - m), 0.0f);
       m += k;
       const float alpha = ex2(-k);
       part = numerators<MASKED, Pl::kParts>(r, pk, slope, lift - m, lv);

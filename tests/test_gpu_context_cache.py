@@ -800,3 +800,67 @@ def test_every_quotient_of_bf16_magnitudes(p):
     lens = torch.full((128,), 64, dtype=torch.int32, device="cuda")
     ck, cv, scales, _ = quantized(k, v, lens, 1)
     check_fields(c.quantize_context(k, v), ck, cv, scales, lens)
+
+
+# ------------------------------------------------------------------ value scales far apart
+
+def far_apart(seed, B, H, D, dtype, ratio, gap):
+    """A cache of 300 rows whose values are `ratio` of those of one block (the first of every other head, else the third), and
+    queries that score the rows of that block some `gap` below the others."""
+    g = gen(seed)
+    N = 300
+    axis = torch.randn(D, device="cuda", generator=g)
+    axis = axis / axis.norm()
+    large = torch.zeros(H, N, dtype=torch.bool, device="cuda")
+    large[0::2, :64] = True
+    large[1::2, 128:192] = True
+    k = 0.5 * torch.randn(H, N, D, device="cuda", generator=g) - gap * large[..., None] * axis
+    v = torch.randn(H, N, D, device="cuda", generator=g) * torch.where(large, 1.0, ratio)[..., None]
+    q = axis * D ** 0.5 + 0.2 * torch.randn(B, H, 1, D, device="cuda", generator=g)
+    q = q - ((q @ axis)[..., None] - D ** 0.5) * axis                  # along the axis all the same
+    return cc().quantize_context(k.to(dtype), v.to(dtype)), q.to(dtype), large
+
+
+@pytest.mark.parametrize("ratio", [1e-3, 1e-5, 1e-7, 1e-8, 1e-9, 1e-20])
+@pytest.mark.parametrize("B", [3, 200])
+@pytest.mark.parametrize("D", [16, 32, 64])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_values_far_below_those_of_a_block_that_nothing_attends(dtype, D, B, ratio, form):
+    """The block of large values has weights of exp(-40) * ratio or less: what is left of it is far below the bounds, which
+    are those of check_attention over the small rows alone.  Exponents of up to log2(1 / ratio) < 67 are sums of
+    numbers of that size, a weight then off by another 2^-17; the log-sum-exp is a difference of such numbers."""
+    cache, q, large = far_apart(120, B, 2, D, dtype, ratio, 40.0 - math.log(ratio))
+    seen = torch.nn.functional.pad(~large, (0, 20), value=False)[:, ::BLOCK]                # [H,blocks]
+    o, l, _, _, N = attention(q, cache, D ** -0.5, seen[None, :, None].expand(B, -1, 1, -1))
+    k, v = values(cache)
+    small = ~large[None, :, :, None]
+    k, v = k[:, :, :300] * small, v[:, :, :300] * small
+    A = float((q.double().abs() @ k.abs().transpose(-1, -2)).max()) * D ** -0.5
+    out, lse = cc().context_cache_attention(q, cache)
+    far = 2.0 ** -17
+    rel = 2 * (D + 8) * U * A + (N / 64 + 100) * U + far + (2.0 ** -11 if dtype is torch.bfloat16 else 0.0)
+    err = (out.double() - o).abs()
+    tol = float(v.abs().max()) * rel + o.abs() * torch.finfo(dtype).eps / 2
+    assert bool((err <= tol).all()), (float(err.max()), float((err / tol).max()))
+    err = (lse.double() - l).abs()
+    tol = (D + 8) * U * A + (N / 64 + 100) * U + 4 * U * (l.abs() + A + 14) + 2 * far
+    assert bool((err <= tol).all()), (float(err.max()), float((err / tol).max()))
+
+
+@pytest.mark.parametrize("ratio", [1e-2, 1e-4, 1e-6])
+@pytest.mark.parametrize("B", [3, 200])
+@pytest.mark.parametrize("D", [16, 32, 64])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_small_values_beside_large_ones_of_as_small_a_weight(dtype, D, B, ratio, form):
+    """Both kinds of rows make up the output: every row's share w |v| of it may be off by its weight's relative error."""
+    cache, q, _ = far_apart(121, B, 2, D, dtype, ratio, -math.log(ratio))
+    k, v = (x[:, :, :300] for x in values(cache))
+    s = q.double() @ k.transpose(-1, -2) * D ** -0.5
+    p = torch.softmax(s, -1)
+    o, share = p @ v, p @ v.abs()
+    A = float((q.double().abs() @ k.abs().transpose(-1, -2)).max()) * D ** -0.5
+    rel = 2 * (D + 8) * U * A + 105 * U + 2.0 ** -17 + (2.0 ** -11 if dtype is torch.bfloat16 else 0.0)
+    out, _ = cc().context_cache_attention(q, cache)
+    err = (out.double() - o).abs()
+    tol = share * rel + o.abs() * torch.finfo(dtype).eps / 2
+    assert bool((err <= tol).all()), (float(err.max()), float((err / tol).max()))
