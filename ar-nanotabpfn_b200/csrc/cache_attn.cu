@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(128, DH == 64 ? 2 : 3) cache_attn_rows_kernel(
     const int live = len - blk * kCacheBlock;
     // value scale: a factor of the numerators (in the exponent) and, back, of their sum
     float ratio = vmax > 0.0f ? sc.y / vmax : 0.0f;
-    if (ratio != ratio) poison = sc.y, ratio = 1.0f;   // a block with values that are not finite: the weights are sound
+    if (sc.y != sc.y) poison = sc.y, ratio = 1.0f;     // a block with values that are not finite: the weights are sound
     ratio = fmaxf(ratio, kLeastRatio);
     const float part_of = __log2f(ratio), lift = kLift + part_of, unlift = 1.0f / ratio;
     float c[MT][8][4];

@@ -864,3 +864,23 @@ def test_small_values_beside_large_ones_of_as_small_a_weight(dtype, D, B, ratio,
     err = (out.double() - o).abs()
     tol = share * rel + o.abs() * torch.finfo(dtype).eps / 2
     assert bool((err <= tol).all()), (float(err.max()), float((err / tol).max()))
+
+
+@pytest.mark.parametrize("B", [3, 200])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("N", [50, 64, 300, 1500])
+def test_values_that_are_not_finite_show_beside_nothing_but_zeros(N, dtype, B, form):
+    """No block has a value scale that is a positive number: the only block, every block, or one beside blocks of zeros is
+    not finite.  Outputs are NaN, the weights and so the log-sum-exp are sound."""
+    c = cc()
+    k, v = rows(130, 1, 3, N, 32, dtype)
+    v[0, 0, ::7, 3] = float("nan")                                     # in every block
+    v[0, 1], v[0, 1, N // 2, 0] = 0.0, float("-inf")                   # in one, zeros in the others
+    v[0, 2] = 0.0                                                      # nothing wrong
+    q = torch.randn(B, 3, 1, 32, device="cuda", generator=gen(131)).to(dtype)
+    cache = c.quantize_context(k, v)
+    out, lse = c.context_cache_attention(q, cache)
+    assert bool(torch.isnan(out[:, :2]).all()) and bool((out[:, 2] == 0).all())
+    sound = c.quantize_context(k, torch.zeros_like(v))
+    want = attention(q, sound, 32 ** -0.5)
+    check_attention((torch.zeros_like(out), lse), want, dtype, 32)
