@@ -32,7 +32,8 @@ from .. import _lib
 
 CONTEXT_BLOCK = 64
 _MOST_ROWS = 1 << 30          # of a cache; also of a call
-_MOST_LISTED = (1 << 31) - 1
+_MOST_LISTED = 1 << 30        # blocks of a query
+_MOST_INT = (1 << 31) - 1
 _Strides = C.c_int64 * 3
 Lengths = Union[Tensor, Sequence[int]]
 
@@ -151,7 +152,7 @@ def _lengths(x: Optional[Lengths], G: int, device: torch.device, what: str) -> O
     if x.shape != (G,):
         raise ValueError(f"{what} must have one entry per context: ({G},), not {tuple(x.shape)}")
     if x.dtype is torch.int64:
-        x = x.clamp(-1, _MOST_LISTED)                        # what does not fit 32 bits stays out of range
+        x = x.clamp(-1, _MOST_INT)                        # what does not fit 32 bits stays out of range
     if x.dtype is not torch.int32 or x.device != device or not x.is_contiguous():
         x = x.to(device=device, dtype=torch.int32).contiguous()
     return x

@@ -20,6 +20,7 @@
 namespace artab {
 
 constexpr int kCacheBlock = 64;
+constexpr int kMostListed = 1 << 30;   // blocks of a list: the kernels step through it, and past its end, in 32 bits
 
 // Rows of a [.., .., rows, Dh] tensor by strides (in elements) of its three leading axes.
 struct RowView {

@@ -654,6 +654,7 @@ int artab_cache_block_attention(int dtype, const void* q, const int64_t* q_strid
                                 const artab_cache* c, const int32_t* blocks, int n_list, float scale, void* out,
                                 float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
   ARTAB_REQUIRE(blocks && n_list >= 1, ARTAB_EINVAL, "cache_block_attention: no blocks");
+  ARTAB_REQUIRE(n_list <= kMostListed, ARTAB_EINVAL, "cache_block_attention: %d blocks a query", n_list);
   int rc = check_cache(c, "cache_block_attention");
   if (rc) return rc;
   rc = check_queries(dtype, q, n_streams, n_q, c, "cache_block_attention");

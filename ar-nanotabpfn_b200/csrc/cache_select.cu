@@ -264,6 +264,7 @@ extern "C" int artab_cache_select(int dtype, const void* q, const int64_t* q_str
   rc = check_queries(dtype, q, n_streams, n_q, c, "cache_select");
   if (rc) return rc;
   ARTAB_REQUIRE(index && n_pick >= 1, ARTAB_EINVAL, "cache_select: no blocks asked for");
+  ARTAB_REQUIRE(n_pick <= kMostListed, ARTAB_EINVAL, "cache_select: %d blocks a query", n_pick);
   ARTAB_REQUIRE(c->n_blocks <= kMaxBlocks, ARTAB_EINVAL, "cache_select: a cache of more than %d rows is not supported",
                 kMaxBlocks * kCacheBlock);
   (void)max_len;

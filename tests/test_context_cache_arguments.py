@@ -245,3 +245,24 @@ def test_sizes_beyond_32_bits_are_refused(fake):
     assert not fake.calls
     counts = cc._lengths(torch.tensor([2 ** 32, -2 ** 40, 7]), G, q.device, "counts")
     assert counts.dtype is torch.int32 and counts[0] >= 2 ** 30 and counts[1] < 0 and counts[2] == 7
+
+
+def test_lists_that_a_step_would_carry_beyond_32_bits_are_refused(fake):
+    """Warps step through a list by up to 2048 entries: a list that ends less than that below 2^31 would be left at the
+    wrong end, so lists are as long as a cache has rows at most."""
+    q = torch.zeros(G, H, 1, D)
+    most = 1 << 30
+    for n in (most + 1, 2 ** 31 - 64, 2 ** 31 - 1):
+        listed = torch.zeros(1, dtype=torch.int32).expand(G, H, 1, n)
+        with pytest.raises(ValueError, match=f"{n} blocks"):
+            cc.block_context_attention(q, cache(), listed)
+        with pytest.raises(ValueError, match=f"{n} blocks"):
+            cc.select_context_blocks(q, cache(), n)
+    assert not fake.calls
+    import ctypes as C
+    lib, p = _lib.load_library(), 4096
+    st = (C.c_int64 * 3)(1, 1, 1)
+    r = C.byref(_lib.Cache(n_groups=1, n_heads=2, head_dim=32, n_blocks=2, codes=p, scales=p, bounds=p, lens=p))
+    for n in (most + 1, 2 ** 31 - 1):
+        assert lib.artab_cache_select(0, p, st, 1, 1, r, 0, n, p, None) == -1
+        assert lib.artab_cache_block_attention(0, p, st, 1, 1, r, p, n, 1.0, p, p, None, 0, None) == -1
