@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnArgs a) {
     const int row = row0 + r;
     if (row >= n_rows) return;
     const size_t at = ((size_t)stream_of(row) * H + h) * a.n_q + query_of(row);
-    reinterpret_cast<T*>(a.out)[at * DH + d] = from_f32<T>(l == 0.0f ? 0.0f : o / l);
+    reinterpret_cast<T*>(a.out)[at * DH + d] = from_f32<T>(l == 0.0f ? 0.0f : o / (kUnlift * l));
     if (d == 0) a.lse[at] = l == 0.0f ? -CUDART_INF_F : (m - kLift) * kLn2 + logf(l);
   };
   for (int e = tid; e < ROWS * DH; e += W * 32) {
@@ -437,14 +437,14 @@ __global__ void __launch_bounds__(128, DH == 64 ? 2 : 3) cache_attn_rows_kernel(
 #pragma unroll
     for (int j = 0; j < ND; ++j)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) part[row * P + 8 * j + 2 * t + e] = (o[mt][j][e] + o[mt][j][2 + e]) * vmax + poison;
+      for (int e = 0; e < 2; ++e) part[row * P + 8 * j + 2 * t + e] = o[mt][j][e] + o[mt][j][2 + e] + poison;
     if (t == 0) part[row * P + DH] = m[mt], part[row * P + DH + 1] = s;
   }
   if (a.splits == 1)
     __syncthreads();
   else
     cluster_meet();
-  merge_rows<float, DH>(a, smem_u32(part), 1, rank * 32 * NW + tid, a.splits * 32 * NW, RT::ROWS, row0, h, group, kLift);
+  merge_rows<float, DH>(a, smem_u32(part), 1, rank * 32 * NW + tid, a.splits * 32 * NW, RT::ROWS, row0, h, group, kLift, vmax);
   if (a.splits > 1) cluster_meet();
 }
 

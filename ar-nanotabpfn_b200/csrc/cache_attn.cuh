@@ -59,10 +59,11 @@ constexpr int kPartial = DH + 4;
 
 // Merges the partial results of `rows` query rows and writes output and log-sum-exp: `per_cta` of them lie in every CTA of
 // the cluster, [per_cta][rows][kPartial] from shared-memory address `base` on.  The calling thread takes every `step`-th
-// group of four channels from `first` on.
+// group of four channels from `first` on.  `factor`: of quotients of outputs and sums; a factor of sums would not fit fp32 where
+// values are large.
 template <typename T, int DH>
 __device__ __forceinline__ void merge_rows(const AttnArgs& a, uint32_t base, int per_cta, int first, int step, int rows,
-                                           int row0, int h, int group, float lift) {
+                                           int row0, int h, int group, float lift, float factor) {
   constexpr int P = kPartial<DH>;
   const int count = per_cta * a.splits;
   for (int e = first; e < rows * (DH / 4); e += step) {
@@ -85,11 +86,12 @@ __device__ __forceinline__ void merge_rows(const AttnArgs& a, uint32_t base, int
     const int b = one ? row / a.n_q : group, l = one ? row % a.n_q : row;
     const size_t to = ((size_t)b * a.c.n_heads + h) * a.n_q + l;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    out.x = out.x * inv * factor, out.y = out.y * inv * factor, out.z = out.z * inv * factor, out.w = out.w * inv * factor;
     T* dst = reinterpret_cast<T*>(a.out) + to * DH + d;
     if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(dst) = make_float4(out.x * inv, out.y * inv, out.z * inv, out.w * inv);
+      *reinterpret_cast<float4*>(dst) = make_float4(out.x, out.y, out.z, out.w);
     } else {
-      __nv_bfloat162 y[2] = {__floats2bfloat162_rn(out.x * inv, out.y * inv), __floats2bfloat162_rn(out.z * inv, out.w * inv)};
+      __nv_bfloat162 y[2] = {__floats2bfloat162_rn(out.x, out.y), __floats2bfloat162_rn(out.z, out.w)};
       *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(y);
     }
     if (d == 0) a.lse[to] = sum == 0.0f ? -CUDART_INF_F : (top - lift) * kLn2 + logf(sum);

@@ -453,8 +453,16 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
   fence_after();
   const uint32_t tmem = sm->tmem_base;
 
+  // value scales are relative to 1 / inverse_scale(), which is the largest unless that is subnormal
+  const auto inverse_scale = [&]() {
+    float top = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) top = fmaxf(top, sm->vmax[w]);
+    return fminf(1.0f / top, 3e38f);
+  };
+
   bool ok = true;
-  float m = -CUDART_INF_F, l = 0.0f, vref = 0.0f;
+  float m = -CUDART_INF_F, l = 0.0f;
   const uint32_t t_row = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (wg & 1) * kColsWg;
   const int steps = wg < 2 ? (nb - wg + 1) / 2 : 0;   // blocks of the warpgroup
 
@@ -561,11 +569,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
     cp_wait<0>();
   } else {
     // --------------------------------- softmax ---------------------------------
-    vmax = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) vmax = fmaxf(vmax, sm->vmax[w]);
-    const float vinv = fminf(1.0f / vmax, 3e38f);     // relative to vref = 1 / vinv, which is vmax unless that is subnormal
-    vref = 1.0f / vinv;
+    const float vinv = inverse_scale();
     if (wg == 0) mbar_arrive(&sm->q_full);
     float2 next = steps > 0 ? scales[rank + wg * a.splits] : make_float2(0.0f, 0.0f);
     for (int i = 0; i < steps; ++i) {
@@ -607,11 +611,8 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
   const bool gave_up = ctl->abort_flag != 0;
   if (wg < 2) {
     float* to = part + (wg * BM + row) * P;
-    const float factor = bad_k || bad_v ? CUDART_NAN_F : vref;
 #pragma unroll
-    for (int d = 0; d < DH; d += 4)
-      *reinterpret_cast<float4*>(to + d) = make_float4(__uint_as_float(o[d]) * factor, __uint_as_float(o[d + 1]) * factor,
-                                                       __uint_as_float(o[d + 2]) * factor, __uint_as_float(o[d + 3]) * factor);
+    for (int d = 0; d < DH; d += 4) *reinterpret_cast<uint4*>(to + d) = make_uint4(o[d], o[d + 1], o[d + 2], o[d + 3]);
     to[DH] = m;
     to[DH + 1] = gave_up || bad_k ? CUDART_NAN_F : l;
   }
@@ -619,7 +620,8 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_tc_kernel(const AttnAr
     __syncthreads();
   else
     cluster_meet();
-  merge_rows<T, DH>(a, smem_u32(part), 2, rank * kThreads + tid, a.splits * kThreads, BM, row0, h, group, kLiftTc);
+  const float factor = bad_k || bad_v ? CUDART_NAN_F : 1.0f / inverse_scale();
+  merge_rows<T, DH>(a, smem_u32(part), 2, rank * kThreads + tid, a.splits * kThreads, BM, row0, h, group, kLiftTc, factor);
   if (a.splits > 1) cluster_meet();
 }
 

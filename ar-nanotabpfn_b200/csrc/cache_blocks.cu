@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const JoinArgs j) {
     out = fmaf(out, x, o * y);
     top = m;
   }
-  reinterpret_cast<T*>(a.out)[u * DH + d] = from_f32<T>(sum == 0.0f ? 0.0f : out / sum);
+  reinterpret_cast<T*>(a.out)[u * DH + d] = from_f32<T>(sum == 0.0f ? 0.0f : out / (kUnlift * sum));
   if (d == 0) a.lse[u] = sum == 0.0f ? -CUDART_INF_F : (top - kLift) * kLn2 + logf(sum);
 }
 

@@ -6,6 +6,8 @@ namespace artab {
 
 // numerators are 2^14 times exp(s - max): halves keep 11 bits of them down to 2^-28 of the largest
 constexpr float kLift = 14.0f;
+// outputs are kept without that factor: of the size of the sums that they stand for, which fit where those do
+constexpr float kUnlift = 6.103515625e-5f;
 
 template <int DH, int PARTS>
 struct Tile {
@@ -133,7 +135,7 @@ struct Tile {
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int r = 0; r < R; ++r)
-          o[md][j][r] = fmaf(o[md][j][r], alpha[r], vs * (PARTS == 2 ? c[2 * j] + c[2 * j + 1] : c[2 * j + r]));
+          o[md][j][r] = fmaf(o[md][j][r], alpha[r], vs * (kUnlift * (PARTS == 2 ? c[2 * j] + c[2 * j + 1] : c[2 * j + r])));
     }
   }
 

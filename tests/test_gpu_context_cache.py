@@ -884,3 +884,20 @@ def test_values_that_are_not_finite_show_beside_nothing_but_zeros(N, dtype, B, f
     sound = c.quantize_context(k, torch.zeros_like(v))
     want = attention(q, sound, 32 ** -0.5)
     check_attention((torch.zeros_like(out), lse), want, dtype, 32)
+
+
+@pytest.mark.parametrize("size", [1e-37, 1e31, 1e34, 1e36])
+@pytest.mark.parametrize("B", [3, 200])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_attended_values_near_the_ends_of_the_range(dtype, B, size, form):
+    """Thirty rows of values up to some 3 size: even all of them at their largest add up to a finite number."""
+    c = cc()
+    k, v = rows(140, 1, 2, 30, 32, torch.float32)
+    cache = c.quantize_context(k.to(dtype), (v.double() * size).to(dtype))
+    q = torch.randn(B, 2, 2, 32, device="cuda", generator=gen(141)).to(dtype)
+    want = attention(q, cache, 32 ** -0.5)
+    assert want[3] * 30 < 3e38
+    check_attention(c.context_cache_attention(q, cache), want, dtype, 32)
+    listed = torch.zeros(B, 2, 2, 2, dtype=torch.int32, device="cuda")
+    listed[..., 1] = -1
+    check_attention(c.block_context_attention(q, cache, listed), want, dtype, 32)
