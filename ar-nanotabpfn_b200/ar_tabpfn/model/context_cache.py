@@ -75,6 +75,8 @@ class ContextCache:
             raise ValueError("ContextCache: tensors must be contiguous")
         if not scales.get_device() == bounds.get_device() == lens.get_device() == codes.get_device():
             raise ValueError("ContextCache: all tensors must live on one device")
+        if length is not None and length < 0:
+            raise ValueError(f"ContextCache: a length of {length}")
         self._set(codes, scales, bounds, lens, blocks * CONTEXT_BLOCK if length is None else length)
 
     def _set(self, codes: Tensor, scales: Tensor, bounds: Tensor, lens: Tensor, length: int) -> "ContextCache":

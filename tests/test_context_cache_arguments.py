@@ -266,3 +266,11 @@ def test_lists_that_a_step_would_carry_beyond_32_bits_are_refused(fake):
     for n in (most + 1, 2 ** 31 - 1):
         assert lib.artab_cache_select(0, p, st, 1, 1, r, 0, n, p, None) == -1
         assert lib.artab_cache_block_attention(0, p, st, 1, 1, r, p, n, 1.0, p, p, None, 0, None) == -1
+
+
+def test_a_length_that_bounds_nothing_is_refused():
+    """`length` is what room is counted from: below zero it would let rows fall behind the capacity unseen."""
+    for length in (-1, -2 ** 40):
+        with pytest.raises(ValueError, match="length"):
+            cc.ContextCache(**tensors(), length=length)
+    assert cc.ContextCache(**tensors(), length=0).length == 0 and cc.ContextCache(**tensors(), length=10 ** 9).length == 128
