@@ -148,13 +148,13 @@ def _lengths(x: Optional[Lengths], G: int, device: torch.device, what: str) -> O
     if x is None:
         return None
     if not isinstance(x, Tensor):
-        x = torch.tensor(list(x), dtype=torch.int32)
-    elif x.dtype.is_floating_point or x.dtype.is_complex or x.dtype is torch.bool:
+        x = torch.tensor(list(x))
+    if x.dtype.is_floating_point or x.dtype.is_complex or x.dtype in (torch.bool, torch.uint64):
         raise ValueError(f"{what} must be whole numbers")
     if x.shape != (G,):
         raise ValueError(f"{what} must have one entry per context: ({G},), not {tuple(x.shape)}")
-    if x.dtype is torch.int64:
-        x = x.clamp(-1, _MOST_INT)                        # what does not fit 32 bits stays out of range
+    if x.dtype in (torch.int64, torch.uint32):
+        x = x.to(torch.int64).clamp(-1, _MOST_INT)           # what does not fit 32 bits stays out of range
     if x.dtype is not torch.int32 or x.device != device or not x.is_contiguous():
         x = x.to(device=device, dtype=torch.int32).contiguous()
     return x

@@ -274,3 +274,18 @@ def test_a_length_that_bounds_nothing_is_refused():
         with pytest.raises(ValueError, match="length"):
             cc.ContextCache(**tensors(), length=length)
     assert cc.ContextCache(**tensors(), length=0).length == 0 and cc.ContextCache(**tensors(), length=10 ** 9).length == 128
+
+
+def test_row_counts_are_whole_numbers_however_they_are_handed_over(fake):
+    """Lists go the way of tensors: no fraction is cut off, what does not fit 32 bits stays out of range."""
+    dev = torch.device("cpu")
+    for x in ([1.5, 2, 3], [True, False, True], [1.0, 2.0, 3.0], torch.tensor([1, 2, 3], dtype=torch.uint64)):
+        with pytest.raises(ValueError, match="whole numbers"):
+            cc._lengths(x, G, dev, "counts")
+    with pytest.raises(ValueError, match="whole numbers"):
+        cc.quantize_context(torch.zeros(G, H, N, D), torch.zeros(G, H, N, D), lens=[99.7, 3, 4])
+    assert not fake.calls
+    for x in ([2 ** 40, -2 ** 40, 7], torch.tensor([2 ** 32 - 1, 0, 7], dtype=torch.uint32), (300, 0, 7),
+              torch.tensor([200, 0, 7], dtype=torch.uint8)):
+        got = cc._lengths(x, G, dev, "counts")
+        assert got.dtype is torch.int32 and got[0] >= 200 and got[1] <= 0 and got[2] == 7
