@@ -312,7 +312,8 @@ def select_context_blocks(q: Tensor, cache: ContextCache, n_blocks: int) -> Tens
 
     The bound of a block is sum_d max(q_d lo_d, q_d hi_d) over the extreme keys of its channels, with the query rounded
     to whole numbers (largest magnitude 127): whole-number arithmetic, so the choice is reproducible to the bit; equal
-    bounds go to the lower index.  A query that is not finite gets the first blocks.  Capacities of up to 221184 rows."""
+    bounds go to the lower index.  A query that is not finite gets the first blocks, a block whose scale is NaN ranks before
+    all others.  Capacities of up to 221184 rows, whatever is in use of them."""
     (B, H, Lq, _), code, device = _queries(q, cache, "select_context_blocks")
     n = int(n_blocks)
     if not 1 <= n <= _MOST_LISTED:
@@ -329,7 +330,7 @@ def select_context_blocks(q: Tensor, cache: ContextCache, n_blocks: int) -> Tens
 def block_context_attention(q: Tensor, cache: ContextCache, blocks: Tensor,
                             scale: Optional[float] = None) -> Tuple[Tensor, Tensor]:
     """``context_cache_attention`` over the rows of the listed blocks only: blocks int32 [B,H,Lq,S], as
-    ``select_context_blocks`` gives them.  An index that is no block in use counts for nothing, one listed twice counts
+    ``select_context_blocks`` gives them (at most 2^30 a query).  An index that is no block in use counts for nothing, one listed twice counts
     twice, a query whose list holds no block gets 0 and -inf."""
     (B, H, Lq, Dh), code, device = _queries(q, cache, "block_context_attention")
     shape = blocks.shape

@@ -13,9 +13,10 @@
 // walks blocks of its own with a running maximum; its ring of records is filled by 16-byte asynchronous copies
 // and no warp waits for another until the end, where the warps of a unit and the CTAs of a cluster (up to eight
 // share the rows of a context) merge maximum, sum and output through shared memory.
-// Measured (B200), queries of one row each: 8 contexts x 65536 rows x 8 heads of size 64, 82.5 us for 537 MB, called again and again
-// (6.5 TB/s, a copy's rate; half of the issue slots busy), 90 - 96 with the launch and other data in between; size 32 51 us (5.3 TB/s), size 16 36 us (3.8 TB/s: 16 codes a lane between two
-// shuffles); 64 x 2048 x 6 of size 32 14 us and one context of 8192 rows 7 us: a chain of loads, products and merges.
+// Measured (B200), queries of one row each: 8 contexts x 65536 rows x 8 heads of size 64, 81 us for 537 MB, called again and again
+// (6.6 TB/s, a copy's rate; half of the issue slots busy), 97 with the launch and other data in between; size 32 51 us (5.3 TB/s),
+// size 16 36 us (3.8 TB/s: 16 codes a lane between two shuffles).  64 contexts x 2048 rows x 6 heads, two queries each: size 16 9.5 us,
+// 32 13, 64 18.4, fp32 the same; one context of 8192 rows 7 us: a chain of loads, products and merges.
 #include "cache_tile.cuh"
 
 namespace artab {
@@ -199,8 +200,8 @@ __global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnArgs a) {
 // block before is worked on; the numerators go from the accumulators of one product straight into the operand
 // registers of the next.  The value scale of a block is folded into the exponent and the maximum, relative to the largest of the
 // context, so that one accumulator serves all blocks.  (bf16 queries and larger jobs: cache_attn_tc.cu.)
-// B200, 6 heads of size 32: 512 queries x 2000 rows 14.3 us, 512 x 8192 34 us.  Two CTAs (size 64) or three of 168 registers an
-// SM; with 1024 queries x 8192 rows (64 us) the tensor pipe is 40 % busy, issue slots 40 %: latency of a block's chain (scores,
+// B200, 6 heads of size 32: 512 queries x 2000 rows 16.6 us, 512 x 8192 41 us.  Two CTAs (size 64) or three of 168 registers an
+// SM; with 1024 queries x 8192 rows (62 us) the tensor pipe is 40 % busy, issue slots 40 %: latency of a block's chain (scores,
 // maximum, exponentials, second product) with twelve warps to hide it.
 template <int DH>
 struct RowTile {
@@ -467,7 +468,7 @@ struct FewPlan {
 template <int DH>
 FewPlan plan_few(long units, long blocks) {
   constexpr double alone = DH == 16 ? 0.2 : DH == 32 ? 0.36 : 0.5, shared = DH == 16 ? 0.047 : DH == 32 ? 0.062 : 0.09;
-  constexpr int kRegisters = 72, kShared = 227 * 1024;
+  constexpr int kRegisters = 72, kShared = 227 * 1024;    // the instances use 50 - 80 registers
   FewPlan best = {0.0, 0, 0};
   for (int warps = 1; warps <= 8; warps *= 2) {
     const int by_shared = kShared / (warps * Ring<DH>::kBytes + 1024), by_registers = 65536 / (32 * kRegisters * warps);
@@ -508,8 +509,10 @@ int launch_rows(const AttnArgs& a, cudaStream_t s) {
 }
 
 // Which kernel, and how many CTAs share a unit's blocks: the least of the times that these figures give, in us.  Measured
-// (B200) over 12 - 4096 rows, 1 - 384 contexts x heads and 500 - 32768 context rows: the pick is 1 - 2 % from the fastest in the
-// mean, up to 20 % where two are close.  Few rows: plan_few, a fifth more for size 32, which full tiles slow down there.
+// (B200) over 12 - 4096 rows, 1 - 384 contexts x heads and 500 - 32768 context rows: the pick is 1 - 3 % from the fastest in the
+// mean, up to 26 % where two are close (1024 fp32 rows x 500 of size 64: few rows 19.6 us, tcgen05 15.6).  Few rows: plan_few, for size
+// 32 a fifth more: over 64 - 1024 bf16 rows x 500 - 8192 x 6 heads the picks are then 0.2 % from the fastest in the mean and 4 % at
+// most; without it 1.5 % and 19 %.  Sizes 16 and 64 have no such factor.
 //   tiles of many rows: a CTA's time for a block when it has an SM to itself and when the SM is full; start and merge in either
 //   case; CTAs of an SM; rows of a tile.  Splits that fill the last round matter: 4096 bf16 queries x 8192 rows x 6 heads of
 //   size 32, 192 tiles, 120 us in one piece and 98 in two; 2048 x 32768, 96 tiles, 231 in two and 180 in four.
@@ -523,8 +526,8 @@ constexpr TileCost tc_cost() {
   if (sizeof(T) == 2) return DH == 16 ? TileCost{0.53, 0.8, 6.0, 9.0, 2, 128} : DH == 32 ? TileCost{0.56, 0.87, 6.0, 9.0, 2, 128} : TileCost{0.7, 1.0, 10.5, 13.5, 2, 128};
   return DH == 16 ? TileCost{0.77, 1.03, 8.0, 13.0, 2, 128} : DH == 32 ? TileCost{0.74, 1.06, 9.6, 15.0, 2, 128} : TileCost{0.78, 1.2, 13.8, 16.0, 2, 128};
 }
-// cache_attn_rows_kernel.  It starts sooner and has half the rows a tile, tcgen05 is faster once it runs (6 heads x 2000 rows of size
-// 32: 512 queries 14.5 and 22.4 us; 8192 rows: 1024 queries 64 and 46, 4096 queries 227 and 133).
+// cache_attn_rows_kernel.  It starts sooner and has half the rows a tile, tcgen05 is faster once it runs (6 heads of size 32: 1024 queries x
+// 500 rows 11.7 and 13.3 us, x 2000 20.5 and 22.6, x 8192 62 and 44; 4096 x 8192 227 and 134).
 template <int DH>
 constexpr TileCost rows_cost() {
   constexpr int rows = RowTile<DH>::ROWS;

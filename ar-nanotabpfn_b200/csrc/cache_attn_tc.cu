@@ -13,8 +13,8 @@
 // largest of the context, taken out of the row sum again), so O accumulates over all blocks.
 // Two CTAs share an SM (256 TMEM columns each), so four warpgroups are in different phases of their blocks.  Head size 64
 // and two parts have no room for P beside S: it overwrites the scores it came from, and the next scores wait for P . V.
-// Measured (B200), bf16, 8192 queries x 8192 rows x 6 heads: head size 32 176 us (292 TFLOP/s, 2.28e12 exponentials a second),
-// 16 162 us, 64 213 us (484 TFLOP/s); 87 us is what the special-function units need for the exponentials.  They are 63 % busy,
+// Measured (B200), bf16, 8192 queries x 8192 rows x 6 heads: head size 32 174 us (296 TFLOP/s, 2.3e12 exponentials a second),
+// 16 161 us, 64 220 us (468 TFLOP/s); 87 us is what the special-function units need for the exponentials.  They are 65 % busy,
 // issue slots 57 % (of some 440 instructions a warp and block 160 are the 64 numerators' own), the tensor pipe 15 %.  Two
 // warpgroups alone on an SM take 2200 cycles a block each, four 3400: latency of a chain of loads, exponentials, stores and
 // barriers with four warps a scheduler.  What was measured on the way at head size 32: masked blocks in
@@ -23,7 +23,8 @@
 // both halves of a block unrolled, the next scores as soon as these are read 208 -> 176.  A share of the exponentials on the FMA
 // pipe (degree four, packed pairs) cost more issue slots than it freed at every share: 242 us with none, 246 with an eighth,
 // 255 with a quarter of them.
-// fp32, 4096 queries x 8192 rows x 6 heads: size 32 133 us (register tiles of cache_attn.cu 227), 16 127 (164), 64 150 (380).
+// fp32, 4096 queries x 8192 rows x 6 heads: size 32 134 us (register tiles of cache_attn.cu 227), 16 123 (164), 64 148 (380).  Two
+// parts of 32 numerators beside their scores do not fit 80 registers: sizes 16 and 32 spill 80 - 88 bytes a thread, read back in 164.
 // Every wait is bounded; a CTA that gives up lets its MMAs end, frees its tensor memory and writes NaN for its rows.
 #include "cache_attn.cuh"
 

@@ -6,9 +6,12 @@
 // that hold it, eight (bf16) or four (fp32) a warp, and writes for each entry the partial result of its block: output not
 // yet divided, maximum, sum.  cache_join_kernel merges the entries of a query in the order of its list.  The
 // order in which a CTA finds entries varies, what it computes for an entry does not.
-// 1024 queries x 6 heads x 16 of 256 blocks of size 32 (B200): 34.5 us, 27 + 7 (64 us one by one, 402 MB out of L2); with 5 CTAs
-// an SM that look at 4096 entries at a time 40 us, with 6 and 8192 34.5.  Of some 1700 instructions a warp two fifths are the products
-// and a fifth the look-up.
+// 1024 queries x 6 heads x 16 of 256 blocks (B200), bf16 / fp32, beside one by one: size 32 35 / 43.5 us (63; 402 MB out of L2), 16
+// 31 / 37 (44), 64 51 / 61 (99); of the 35 us 28 + 7.  With 5 CTAs an SM that look at 4096 entries at a time 40 us, with 6 and 8192
+// 34.5.  Of some 1500 instructions a warp two fifths are the products and a fifth the look-up; issue slots are 60 % busy, waits for
+// queries and entries (long scoreboard) the largest stall.  Six CTAs an SM take 40 registers a thread, at the cost of spills (size 32, bf16:
+// 28 bytes stored and 24 read a thread); at size 64 shared memory lets five onto an SM, and the bound spills
+// 200 bytes there (bf16).
 #include <type_traits>
 
 #include "cache_tile.cuh"
@@ -161,8 +164,13 @@ int launch_by_block(const JoinArgs& j, cudaStream_t s) {
 }  // namespace
 
 // Going through the blocks pays from so many entries a block on (in the mean), as long as looking an entry up in every
-// block does not cost more than the records that are read once less, and the partial results stay below a gigabyte.  6 heads
-// of size 32, 16 of 256 blocks: 128 queries (8 entries a block) 15.1 us by block, 13.7 one by one; 256 17.6 and 21.1; 512 22 and 36.
+// block does not cost more than the records that are read once less, and the partial results stay below a gigabyte.  By block / one
+// by one (us), 6 heads, 16 of 256 blocks, 128, 192 and 256 queries (8, 12 and 16 entries a block):
+//   size 16 bf16 13.4 / 9.9, 14.4 / 11.7, 15.3 / 15.6; fp32 13.5 / 9.9, 15.2 / 11.7, 16.4 / 15.6   (16 would suit it better)
+//   size 32 bf16 14.3 / 12.8, 15.4 / 15.4, 16.0 / 20.1; fp32 14.7 / 12.7, 16.4 / 15.6, 18.1 / 20.3
+//   size 64 bf16 19.1 / 16.7, 20.8 / 23.2, 22.4 / 30.8; fp32 19.2 / 17.0, 21.3 / 23.0, 23.8 / 30.6
+// 16 of 1024 blocks, 1024 queries: size 16 64 / 44.5, 32 71 / 63, 64 102 / 99.  Blocks are those of the capacity: the rows in use are
+// known on the device only, so a cache with much room (16384 rows in a capacity of 65536: 63 us, in one of 16384 35) goes one by one.
 constexpr int kLeastShared = 12;
 constexpr int64_t kMostWorkspace = 1LL << 30;
 int64_t by_block_workspace(const artab_cache* c, int n_streams, int n_q, int n_list) {

@@ -8,8 +8,9 @@
 //
 // One CTA = 16 queries of a (group, head): scores of all blocks into shared memory as ordered keys (products of
 // 16 queries x 8 blocks a warp), then a warp takes two queries at a time, finds their n-th largest keys by bisection
-// and writes the chosen indices in ascending order.  1024 queries x 6 heads x 256 blocks (B200): 12.3 us; one CTA alone takes 8:
-// a chain of loads, barriers and some 15 steps of bisection, of which 384 CTAs fill the GPU once.
+// and writes the chosen indices in ascending order.  1024 queries x 6 heads x 256 blocks (B200): 12.4 us; one CTA alone takes 8.
+// 384 CTAs fill the GPU once, with 53 % of the issue slots busy: each of some 15 steps of bisection counts every key of a row (eight
+// compares and sums a lane, a reduction), behind a chain of loads and barriers.
 #include "cache8.cuh"
 
 namespace artab {
@@ -20,7 +21,7 @@ constexpr int kThreads = 256, kRows = 16, kMaxBlocks = 3456;   // 16 rows of key
 struct SelectArgs {
   artab_cache c;
   RowView q;
-  int n_streams, n_q, rows, tiles, n_pick;
+  int n_q, rows, tiles, n_pick;
   int pitch;               // keys of a row
   int vec_q;
   int32_t* index;          // [B][H][Lq][n_pick]
@@ -267,11 +268,10 @@ extern "C" int artab_cache_select(int dtype, const void* q, const int64_t* q_str
   ARTAB_REQUIRE(n_pick <= kMostListed, ARTAB_EINVAL, "cache_select: %d blocks a query", n_pick);
   ARTAB_REQUIRE(c->n_blocks <= kMaxBlocks, ARTAB_EINVAL, "cache_select: a cache of more than %d rows is not supported",
                 kMaxBlocks * kCacheBlock);
-  (void)max_len;
+  (void)max_len;   // room for keys goes by the capacity: lens may have grown past the bound in a replayed graph
   SelectArgs a;
   a.c = *c;
   a.q = row_view(q, q_strides, c->n_heads, n_q, c->head_dim);
-  a.n_streams = n_streams;
   a.n_q = n_q;
   a.rows = c->n_groups == 1 ? n_streams * n_q : n_q;
   a.tiles = (a.rows + kRows - 1) / kRows;

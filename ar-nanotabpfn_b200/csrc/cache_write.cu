@@ -7,7 +7,8 @@
 // that it turns 4 x 4 bytes with permutes, and shared memory brings the words into the order of the record.
 // 64 contexts x 2048 rows x 6 heads of size 32 (B200): fp32 48 us for 251 MB (5.2 TB/s, HBM), bf16 38 us for 151 MB: some 310
 // instructions a warp and block (80 % of issue slots).  Reading the same back
-// as fp32: 40 us for 252 MB (6.3 TB/s).
+// as fp32: 40 us for 252 MB (6.3 TB/s), as bf16 32 us for 151 MB.  100 rows behind 2000 of 64 contexts: 8 heads of size 64 16 us (fp32;
+// bf16 15.5), 6 of size 32 7.5: two or three blocks a (group, head), a CTA each, a chain of lengths, rows, barrier, codes and stores.
 #include "cache8.cuh"
 
 namespace artab {
@@ -52,7 +53,8 @@ __device__ __forceinline__ int first_row(int word) { return 16 * (word & 3) + 2 
 __device__ __forceinline__ float step_of(uint32_t top_bits) {
   const float x = __uint_as_float(top_bits);
   if (x < 1e-30f) return __fdiv_rn(x, 127.0f);
-  // the quotient by 127, correctly rounded: a first value, its exact rest, one correction
+  // the quotient by 127, correctly rounded: a first value, its exact rest, one correction (Markstein, "Computation of elementary
+  // functions on the IBM RISC System/6000 processor", 1990)
   const float c = 1.0f / 127.0f, q = x * c;
   return top_bits >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : fmaf(fmaf(-127.0f, q, x), c, q);
 }
@@ -300,7 +302,7 @@ __global__ void __launch_bounds__(2 * Half<DH>::N, (FRESH ? 1024 : 1280) / (2 * 
 // One new row a context: the step of a decode.  A warp does a (group, head): the new row's codes by a lane or two a channel,
 // the bounds from the block's older keys, which 16 bytes a lane hold while they are looked through; older codes are
 // written only where a scale rises.  512 contexts x 6 heads of size 32: 15.4 us with cache_write_kernel, which goes through
-// whole blocks with a CTA each, 5 here.  Up to kGroupHeads heads a CTA takes a group, and the length moves in the same launch;
+// whole blocks with a CTA each, 4.8 here (17 heads, in two launches, 10).  Up to kGroupHeads heads a CTA takes a group, and the length moves in the same launch;
 // beyond, four warps of any groups, and cache_advance_kernel.
 constexpr int kGroupHeads = 16;
 __device__ __forceinline__ int value_place(int row) { return 16 * ((row >> 1) & 3) + 4 * (row >> 4) + 2 * ((row >> 3) & 1) + (row & 1); }

@@ -398,6 +398,7 @@ ARTAB_API int artab_cache_read(int dtype, const artab_cache* c, const int32_t* s
 /* Attention of q [B][H][Lq][Dh] (HOST array of three strides: stream, head, query; NULL: contiguous) over the rows in use:
  * out [B][H][Lq][Dh] of `dtype` (16-byte aligned), lse [B][H][Lq] (natural log).  A context of no rows gives 0 and -inf.
  * max_len: a bound of lens known to the host, for the choice of kernel and launch only (any value gives a right result).
+ * A block's values come out right however far its scale is below that of other blocks (down to 2^-80 of the largest).
  * A bounded wait that gives up shows as NaN in the rows of out and lse that it concerns. */
 ARTAB_API int artab_cache_attention(int dtype, const void* q, const int64_t* q_strides, int n_streams, int n_q,
                                     const artab_cache* c, int max_len, float scale, void* out, float* lse,
@@ -405,15 +406,17 @@ ARTAB_API int artab_cache_attention(int dtype, const void* q, const int64_t* q_s
 
 /* For every query the n_pick blocks with the largest upper bound of a score, index [B][H][Lq][n_pick] int32 in
  * ascending order, -1 behind them where a context has fewer blocks.  The bound is formed with the query rounded to
- * whole numbers (largest magnitude 127), exactly; equal bounds go to the lower index.  At most 221184 rows of capacity;
- * n_pick at most 2^30. */
+ * whole numbers (largest magnitude 127), exactly; equal bounds go to the lower index, a block whose
+ * scale is NaN ranks first.  At most 221184 rows of capacity, whatever is in use of it (max_len is not looked at: lens may have grown
+ * past it in a replayed graph); n_pick at most 2^30. */
 ARTAB_API int artab_cache_select(int dtype, const void* q, const int64_t* q_strides, int n_streams, int n_q,
                                  const artab_cache* c, int max_len, int n_pick, int32_t* index, void* stream);
 
 /* artab_cache_attention over the rows of the blocks that blocks [B][H][Lq][n_list] int32 lists for every query: an index
  * that is no block in use counts for nothing, one that is listed twice counts twice.  n_list is at most 2^30.
  * artab_cache_block_workspace: bytes of workspace (16-byte aligned) with which many queries of one context are worked
- * on block by block, 0 where that does not pay; without it (NULL) every query takes its blocks one by one. */
+ * on block by block, 0 where that does not pay (by the capacity's blocks); without it (NULL) every query takes its blocks
+ * one by one. */
 ARTAB_API int64_t artab_cache_block_workspace(const artab_cache* c, int n_streams, int n_q, int n_list);
 ARTAB_API int artab_cache_block_attention(int dtype, const void* q, const int64_t* q_strides, int n_streams, int n_q,
                                           const artab_cache* c, const int32_t* blocks, int n_list, float scale,
