@@ -298,8 +298,7 @@ __device__ __forceinline__ bool softmax_block(TcSmem<T, DH>* sm, uint32_t t_row,
       part = numerators<MASKED, Pl::kParts>(r, pk, slope, lift - m, lv);
       l *= alpha;
       sum *= alpha;
-      if (c == 0) {                               // the other half of this block's numerators
-        const __half2 al = __float2half2_rn(alpha);
+      if (c == 0) {                               // the other half of this block's numerators, by way of fp32: as a half, alpha is 0 from 2^-25 on
         wait_st();
 #pragma unroll 1
         for (int part = 0; part < Pl::kParts; ++part) {
@@ -307,7 +306,10 @@ __device__ __forceinline__ bool softmax_block(TcSmem<T, DH>* sm, uint32_t t_row,
           tmem_ld16(t_row + Pl::col_p(1, part), u);
           wait_ld();
 #pragma unroll
-          for (int e = 0; e < 16; ++e) u[e] = h2_bits(__hmul2(*reinterpret_cast<const __half2*>(&u[e]), al));
+          for (int e = 0; e < 16; ++e) {
+            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&u[e]));
+            u[e] = h2_bits(__floats2half2_rn(y.x * alpha, y.y * alpha));
+          }
           tmem_st16(t_row + Pl::col_p(1, part), u);
         }
       }

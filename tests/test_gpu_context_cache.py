@@ -901,3 +901,35 @@ def test_attended_values_near_the_ends_of_the_range(dtype, B, size, form):
     listed = torch.zeros(B, 2, 2, 2, dtype=torch.int32, device="cuda")
     listed[..., 1] = -1
     check_attention(c.block_context_attention(q, cache, listed), want, dtype, 32)
+
+
+@pytest.mark.parametrize("rise", [20.0, 24.6, 30.0, 37.0])
+@pytest.mark.parametrize("D", [16, 32, 64])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_a_maximum_that_rises_within_a_block_keeps_its_other_rows(dtype, D, rise, form):
+    """One block has a row some 2^9 above the weights before it, and one 2^rise above them whose values are zero in half of
+    the channels: there the output is made of the other rows.  A numerator is rounded to a multiple of 2^-24 (the smallest half)
+    where the largest row's is 2^5 at least: each is off by at most 2^-25 / 2^5 = 2^-30 of the largest weight, and the output by
+    that times the sum of all |v|, beside what the weights themselves are off by."""
+    c = cc()
+    g = gen(150)
+    B, H, N = 200, 2, 40 * BLOCK
+    axis = torch.randn(D, device="cuda", generator=g)
+    axis = axis / axis.norm()
+    length = torch.zeros(N, device="cuda")
+    length[20 * BLOCK + 40], length[20 * BLOCK + 3] = 9 * math.log(2), rise * math.log(2)
+    k = (length[:, None] * axis).expand(1, H, N, D).to(dtype)
+    v = torch.randn(1, H, N, D, device="cuda", generator=g)
+    v[:, :, 20 * BLOCK + 3, D // 2:] = 0
+    q = (axis * D ** 0.5 * (1 + 0.02 * torch.rand(B, H, 1, 1, device="cuda", generator=g))).to(dtype)
+    cache = c.quantize_context(k, v.to(dtype))
+    kk, vv = values(cache)
+    s = q.double() @ kk.transpose(-1, -2) * D ** -0.5
+    p = torch.softmax(s, -1)
+    o, share = p @ vv, p @ vv.abs()
+    A = float((q.double().abs() @ kk.abs().transpose(-1, -2)).max()) * D ** -0.5
+    rel = 2 * (D + 8) * U * A + (N / 64 + 100) * U + 2.0 ** -17 + (2.0 ** -11 if dtype is torch.bfloat16 else 0.0)
+    out, _ = c.context_cache_attention(q, cache)
+    err = (out.double() - o).abs()
+    tol = share * rel + o.abs() * torch.finfo(dtype).eps / 2 + 2.0 ** -30 * vv.abs().sum(2, keepdim=True)
+    assert bool((err <= tol).all()), (float(err.max()), float((err / tol).max()))
