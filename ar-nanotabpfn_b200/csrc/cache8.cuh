@@ -38,9 +38,9 @@ inline RowView row_view(const void* p, const int64_t* strides, int n1, int n2, i
 // The nearest whole number to x / scale in exact arithmetic, ties to even.  A first value c comes from one fused product
 // with the reciprocal, rounded by adding 1.5 * 2^23 (the low byte of the sum is then the code).  Next to a tie it may be
 // off by one, and ties are not rare (rows of eight-bit numbers such as bf16 meet one in some 200): the rest x - c * scale,
-// one fused operation that is exact next to a tie, is compared with half the scale.  Steps near the smallest normal
-// number, and kept rows next to a tie (whose x is a product itself), go through 64 bits.
+// one fused operation that is exact next to a tie, is compared with half the scale.  Steps below 2^-125, and kept rows next to a tie (whose x is a product itself), go through 64 bits.
 constexpr float kRound = 12582912.0f + 128.0f;   // 1.5 * 2^23, and the 128 that is added to a code
+constexpr float kLeastStep = 2.350988701644575e-38f;   // 2^-125: half of it is a normal number, so halves of steps are exact
 
 __device__ __forceinline__ uint32_t low_bytes(const uint32_t (&w)[4]) {
   return __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
@@ -66,7 +66,7 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[4], float scale, f
   uint32_t w[4];
   float rest[4];
   const float half = 0.5f * scale;
-  bool sure = scale > 2e-38f;
+  bool sure = scale >= kLeastStep;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const float r = fmaf(x[j], inv, kRound);
@@ -75,7 +75,7 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[4], float scale, f
     w[j] = __float_as_uint(r);
   }
   if (!sure) {
-    if (scale <= 2e-38f) return exact_codes(x[0], x[1], x[2], x[3], 1.0f, scale);
+    if (scale < kLeastStep) return exact_codes(x[0], x[1], x[2], x[3], 1.0f, scale);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const bool off = fabsf(rest[j]) > half || (fabsf(rest[j]) == half && (w[j] & 1u));
@@ -100,7 +100,7 @@ __device__ __forceinline__ uint32_t codes_of_bf16(const float (&x)[4], float inv
 // than 3e-5: closer than 5e-5 to a tie it is formed again.
 __device__ __forceinline__ uint32_t kept_codes(const float (&x)[4], float was, float scale, float inv) {
   uint32_t w[4];
-  bool sure = scale > 2e-38f;
+  bool sure = scale >= kLeastStep;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const float y = x[j] * was, r = fmaf(y, inv, kRound);

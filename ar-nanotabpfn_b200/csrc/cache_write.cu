@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(2 * Half<DH>::N, (FRESH ? 1024 : 1280) / (2 * 
     // a step of zero (or NaN) has zero codes
     const float step = larger_step(was, step_of(block_top)), inv = reciprocal(step);
     const float over = fmaf(step, 127.0f, -__uint_as_float(block_top)), inv_shifted = shifted(inv, over);
-    const bool shift = FRESH && sizeof(T) == 2 && step > 2e-38f && over != 0.0f;
+    const bool shift = FRESH && sizeof(T) == 2 && step >= kLeastStep && over != 0.0f;
     // rows that stay, at a scale that stays, are not written again
     const bool stays = !FRESH && n_old > 0 && !(step > was);
     if (n_old && vals && !mine && !stays) load_old();

@@ -933,3 +933,36 @@ def test_a_maximum_that_rises_within_a_block_keeps_its_other_rows(dtype, D, rise
     err = (out.double() - o).abs()
     tol = share * rel + o.abs() * torch.finfo(dtype).eps / 2 + 2.0 ** -30 * vv.abs().sum(2, keepdim=True)
     assert bool((err <= tol).all()), (float(err.max()), float((err / tol).max()))
+
+
+@pytest.mark.parametrize("p", [-133, -127, -126, -125, -124])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_ties_at_steps_near_the_smallest_normal_number(dtype, p):
+    """Blocks whose largest magnitude is b 2^p, b = 128 .. 255: steps on either side of 2^-126 and 2^-125, where a step or its half
+    has fewer bits.  Written at once, appended, and each first row by itself; queries of such a size choose blocks."""
+    c = cc()
+    a = torch.arange(1, 256, device="cuda", dtype=torch.float64)
+    x = (a[None] * 2.0 ** -torch.arange(16, device="cuda", dtype=torch.float64)[:, None]).flatten()        # 4080 numbers
+    x = torch.cat([x, torch.zeros(16, device="cuda", dtype=torch.float64)])
+    b = torch.arange(128, 256, device="cuda", dtype=torch.float64)
+    k = torch.where(x[None] <= b[:, None], x[None], x[None] / 2) * torch.where(torch.arange(4096, device="cuda") % 2 == 0, 1.0, -1.0)
+    k[:, 63] = b                                             # in the first row, that all but it may be appended to
+    k = (k * 2.0 ** p).view(128, 1, 64, 64).to(dtype)
+    v = (k.double() * 0.5).to(dtype).flip(0)
+    lens = torch.full((128,), 64, dtype=torch.int32, device="cuda")
+    ck, cv, scales, _ = quantized(k, v, lens, 1)
+    check_fields(c.quantize_context(k, v), ck, cv, scales, lens)
+    cache = c.quantize_context(k[:, :, :1], v[:, :, :1], capacity=64)
+    one = quantized(k[:, :, :1], v[:, :, :1], lens.clamp(max=1), 1)
+    check_fields(cache, *one[:3], lens.clamp(max=1))
+    zero = torch.zeros_like(lens)
+    c.append_context(cache, k, v, start=zero)
+    check_fields(cache, ck, cv, scales, lens)
+    c.append_context(cache, k[:, :, :1], v[:, :, :1], start=zero)
+    check_fields(cache, *one[:3], lens.clamp(max=1))
+    c.append_context(cache, k[:, :, 1:], v[:, :, 1:])
+    check_fields(cache, *_append_reference(one[:3] + (lens.clamp(max=1),), k[:, :, 1:], v[:, :, 1:], lens.clamp(max=1), lens - 1, 64))
+    keys = torch.randn(1, 1, 640, 64, device="cuda", generator=gen(160))
+    other = c.quantize_context(keys, keys)
+    q = k.reshape(128 * 64, 1, 1, 64)[::7]
+    assert torch.equal(c.select_context_blocks(q, other, 3), chosen(q, other, 3))
